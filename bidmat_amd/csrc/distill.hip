@@ -1,0 +1,244 @@
+// Distillation from a teacher's largest logits: the loss of a dense matrix of student logits Z (vocabulary x columns)
+// against a sparse one of teacher logits T, and its gradient. With x = z / tau, t = T / tau, over one column:
+//
+//   p = softmax over the column's stored entries of t,   lse = log sum exp(x) over all rows
+//   loss = weight * tau^2 * sum_j p_j (log p_j - x_{r_j} + lse),   dz_i = weight * tau * (exp(x_i - lse) - sum_{r_j = i} p_j)
+//
+// A column without stored entries, or with weight 0, has loss 0 and gradient 0, whatever its logits hold. A row may be
+// stored twice; its shares add. Entries whose row lies outside the matrix are left out.
+#include "columns.hpp"
+#include "elems.hpp"
+#include "kernels.hpp"
+#include "workspace.hpp"
+
+namespace bm {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// What a column's teacher entries come to. at0: the largest student logit x among them, subtracted before the sum so
+// that loss = tau^2 * weight * (part + mass * (lse - at0)) cancels nothing large.
+struct Teacher { float lse, part, mass, at0; };      // lse = -inf: no entries
+
+// A running log-sum in base 2: sum of 2^(v - top).
+struct LogSum { float top, sum; };
+__device__ __forceinline__ LogSum join(LogSum a, LogSum b) {
+    const float top = fmaxf(a.top, b.top);
+    if (top == -INFINITY) return {top, a.sum + b.sum};          // both empty; a NaN in a sum stays
+    return {top, a.sum * __builtin_amdgcn_exp2f(a.top - top) + b.sum * __builtin_amdgcn_exp2f(b.top - top)};
+}
+__device__ __forceinline__ LogSum wave_join(LogSum x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        LogSum y;
+        y.top = __shfl_xor(x.top, m, 64);
+        y.sum = __shfl_xor(x.sum, m, 64);
+        x = join(x, y);
+    }
+    return x;
+}
+// All threads of a workgroup of 64 * waves get the joined log-sum.
+__device__ __forceinline__ LogSum block_join(LogSum x, LogSum* sh, int waves) {
+    x = wave_join(x);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = sh[0];
+    for (int w = 1; w < waves; ++w) x = join(x, sh[w]);
+    return x;
+}
+__device__ __forceinline__ float natural_lse(LogSum x) { return (x.top + __log2f(x.sum)) * kLn2; }
+
+__device__ __forceinline__ void column_entries(const DistillArgs& a, long long c, int& lo, int& hi) {
+    lo = min(max(a.tjc[c], 0), a.nnz);
+    hi = min(max(a.tjc[c + 1], lo), a.nnz);
+}
+__device__ __forceinline__ float column_scale(const DistillArgs& a, long long c) { return a.weight != nullptr ? a.weight[c] : 1.f; }
+
+// One wave: statistics of a column's teacher entries; at[] receives the student's x at each of them.
+template <class T>
+__device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, float* at) {
+    const int lane = threadIdx.x & 63;
+    int lo, hi;
+    column_entries(a, c, lo, hi);
+    const T* z = (const T*)a.Z + c * a.ldz;
+    float top = -INFINITY, xtop = -INFINITY;
+    for (int j = lo + lane; j < hi; j += 64) {
+        const int r = a.tir[j];
+        const bool in = (unsigned)r < (unsigned)a.nrows;
+        const float x = in ? (float)z[r] * it : 0.f;
+        at[j] = x;
+        if (in) {
+            top = fmaxf(top, a.tdata[j] * it);
+            xtop = fmaxf(xtop, x);
+        }
+    }
+    top = group_allmax<64>(top);
+    xtop = group_allmax<64>(xtop);
+    if (xtop == -INFINITY || xtop == INFINITY) xtop = 0.f;
+    float sum = 0.f;
+    bool any = false;
+    for (int j = lo + lane; j < hi; j += 64)
+        if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
+            const float t = a.tdata[j] * it;
+            any = any || !(t == -INFINITY);
+            sum += t == -INFINITY ? 0.f : expf(t - top);
+        }
+    sum = group_allsum<64>(sum);
+    Teacher r;
+    r.lse = __ballot(any) != 0 ? top + logf(sum) : -INFINITY;
+    float part = 0.f, mass = 0.f;
+    for (int j = lo + lane; j < hi; j += 64)
+        if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
+            const float logp = a.tdata[j] * it - r.lse, p = expf(logp);
+            if (p != 0.f) {
+                part += p * (logp - (at[j] - xtop));
+                mass += p;
+            }
+        }
+    r.part = group_allsum<64>(part);
+    r.mass = group_allsum<64>(mass);
+    r.at0 = xtop;
+    return r;
+}
+
+// Chunk `chunk` of column c: its log-sum (base 2). Workgroups behind the chunks take the teacher's columns, one wave each.
+template <class T>
+__global__ __launch_bounds__(BM_BLOCK) void k_distill_parts(DistillArgs a, int nchunks, int chunk, LogSum* parts, Teacher* stats, float* at) {
+    __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
+    const float it = 1.f / a.temperature;
+    const long long nparts = (long long)nchunks * a.ncols;
+    if (blockIdx.x >= nparts) {
+        const long long c = (blockIdx.x - nparts) * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6);
+        if (c >= a.ncols) return;
+        const Teacher r = teacher_column<T>(a, c, it, at);
+        if ((threadIdx.x & 63) == 0) stats[c] = r;
+        return;
+    }
+    const long long c = blockIdx.x / nchunks;
+    const int b = (int)(blockIdx.x % nchunks);
+    const T* z = (const T*)a.Z + c * a.ldz;
+    const int lo = b * chunk, hi = min(a.nrows, lo + chunk);
+    const float k = it * kLog2e;
+    LogSum x = {-INFINITY, 0.f};
+    for (int i = lo + (int)threadIdx.x * 8; i < hi; i += BM_BLOCK * 8) {
+        const float8_t v = load_col8(z, i, hi, (T)(-INFINITY)).wide() * k;
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, v[j]);
+        top = fmaxf(top, x.top);
+        const float from = top == -INFINITY ? 0.f : top;
+        float sum = x.sum * __builtin_amdgcn_exp2f(x.top - from);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f(v[j] - from);
+        x = {top, sum};
+    }
+    x = block_join(x, sh, BM_WAVES_PER_BLOCK);
+    if (threadIdx.x == 0) parts[blockIdx.x] = x;
+}
+
+__device__ __forceinline__ LogSum join_parts(const LogSum* parts, int nchunks, int t, int step) {
+    LogSum x = {-INFINITY, 0.f};
+    for (int b = t; b < nchunks; b += step) x = join(x, parts[b]);
+    return x;
+}
+
+__device__ __forceinline__ void write_loss(const DistillArgs& a, long long c, float lse, const Teacher& t) {
+    if (a.lse != nullptr) a.lse[c] = lse;
+    if (a.loss != nullptr) {
+        const float w = column_scale(a, c);
+        const float v = w * a.temperature * a.temperature * (t.part + t.mass * (lse - t.at0));
+        a.loss[c] = t.lse == -INFINITY || w == 0.f ? 0.f : v;
+    }
+}
+
+// Loss and log-sum alone: one wave per column.
+__global__ __launch_bounds__(BM_BLOCK) void k_distill_loss(DistillArgs a, int nchunks, const LogSum* parts, const Teacher* stats) {
+    const long long c = (long long)blockIdx.x * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6);
+    if (c >= a.ncols) return;
+    const LogSum x = wave_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x & 63, 64));
+    if ((threadIdx.x & 63) == 0) write_loss(a, c, natural_lse(x), stats[c]);
+}
+
+// The gradient of rows [lo, hi) of column c, once every student logit at a teacher entry has been saved in at[].
+template <class T>
+__device__ void grad_chunk(const DistillArgs& a, long long c, int lo, int hi, float it, float lse, const Teacher& t, const float* at) {
+    const T* z = (const T*)a.Z + c * a.ldz;
+    T* dz = (T*)a.dZ + c * a.lddz;
+    const float w = column_scale(a, c) * a.temperature;
+    const bool none = t.lse == -INFINITY || w == 0.f;
+    const float k = it * kLog2e, from = lse * kLog2e;
+    for (int i = lo + (int)threadIdx.x * 8; i < hi; i += (int)blockDim.x * 8) {
+        float8_t v = (float8_t)(0.f);
+        if (!none) {
+            const float8_t x = load_col8(z, i, hi).wide();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(x[j], k, -from));
+        }
+        store_col8(dz, i, hi, v);
+    }
+    if (none) return;
+    __syncthreads();          // the entries' values go over what other threads of the workgroup wrote
+    int e0, e1;
+    column_entries(a, c, e0, e1);
+    for (int j = e0 + (int)threadIdx.x; j < e1; j += (int)blockDim.x) {
+        const int r = a.tir[j];
+        if (r < lo || r >= hi) continue;
+        float p = 0.f;
+        for (int q = e0; q < e1; ++q)
+            if (a.tir[q] == r) p += expf(a.tdata[q] * it - t.lse);
+        dz[r] = (T)(w * (__builtin_amdgcn_exp2f(fmaf(at[j], kLog2e, -from)) - p));
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(BM_BLOCK) void k_distill_grad(DistillArgs a, int nchunks, int chunk, int npart, const LogSum* parts,
+                                                           const Teacher* stats, const float* at) {
+    __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
+    const long long c = blockIdx.x / nchunks;
+    const int b = (int)(blockIdx.x % nchunks);
+    float lse;
+    const Teacher t = stats[c];
+    if (a.lse_in != nullptr) {
+        lse = a.lse_in[c];
+    } else {
+        lse = natural_lse(block_join(join_parts(parts + c * npart, npart, threadIdx.x, BM_BLOCK), sh, BM_WAVES_PER_BLOCK));
+        if (b == 0 && threadIdx.x == 0) write_loss(a, c, lse, t);
+    }
+    const int lo = b * chunk;
+    grad_chunk<T>(a, c, lo, min(a.nrows, lo + chunk), 1.f / a.temperature, lse, t, at);
+}
+
+template <class T>
+hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
+    // a chunk is a multiple of what a workgroup takes at once; smaller ones where there are few columns
+    int chunk = 4 * BM_BLOCK * 8;
+    while (chunk > BM_BLOCK * 8 && (long long)a.ncols * ((a.nrows + chunk - 1) / chunk) < 1024) chunk >>= 1;
+    const int nchunks = (a.nrows + chunk - 1) / chunk;
+    const long long nparts = (long long)nchunks * a.ncols;
+    hipError_t err;
+    char* buf = (char*)ws_get(WS_DISTILL, sizeof(Teacher) * (size_t)a.ncols + sizeof(LogSum) * (size_t)nparts, &err, s);
+    if (!buf) return err;
+    float* at = (float*)ws_get(WS_DISTILL_AT, sizeof(float) * (size_t)a.nnz, &err, s);
+    if (!at) return err;
+    Teacher* stats = (Teacher*)buf;
+    LogSum* parts = (LogSum*)(buf + sizeof(Teacher) * (size_t)a.ncols);
+    const int waves = (a.ncols + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK;
+    const long long first = a.lse_in != nullptr ? waves : nparts + waves;
+    if (first > 0x7fffffffLL || nparts > 0x7fffffffLL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_distill_parts<T>), dim3((unsigned)first), dim3(BM_BLOCK), 0, s, a, a.lse_in != nullptr ? 0 : nchunks, chunk, parts,
+                       stats, at);
+    if (a.dZ != nullptr)
+        hipLaunchKernelGGL((k_distill_grad<T>), dim3((unsigned)nparts), dim3(BM_BLOCK), 0, s, a, nchunks, chunk, nchunks, parts, stats, at);
+    else
+        hipLaunchKernelGGL(k_distill_loss, dim3((unsigned)waves), dim3(BM_BLOCK), 0, s, a, nchunks, parts, stats);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t distill(const DistillArgs& a, hipStream_t s) {
+    return a.type == ELEM_F32 ? distill_typed<float>(a, s) : a.type == ELEM_F16 ? distill_typed<f16_t>(a, s) : distill_typed<bf16_t>(a, s);
+}
+
+}  // namespace bm

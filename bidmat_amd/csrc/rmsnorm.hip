@@ -1,0 +1,274 @@
+// Root-mean-square normalisation of the columns of a dense matrix, with the residual's addition in front, an output in
+// 8 bits with scales behind, and its gradient.
+//
+//   h = x + r,   rs = 1 / sqrt(mean(h^2) + eps),   y_i = h_i * rs * w_i
+//   scale_g = max(max over group g of |y|) / 448, 2^-126),   q_i = e4m3(y_i / scale_g)
+//
+// y is formed from the sum in fp32, not from the rounded h that is written. 448 is the largest number of e4m3, so that no
+// code overflows; 2^-126 keeps 1 / scale finite for a group of zeros (whose codes are zeros).
+// TPC threads share a column and keep all of it in registers (8 * NV elements each): every input is read once and every
+// output written once, also where an output overwrites its input.
+#include "columns.hpp"
+#include "elems.hpp"
+#include "kernels.hpp"
+#include "workspace.hpp"
+
+namespace bm {
+namespace {
+
+constexpr float kE4M3Max = 448.f;
+constexpr float kScaleMin = 1.17549435e-38f;      // 2^-126
+
+constexpr int norm_block(int tpc) { return tpc <= 64 ? BM_BLOCK : tpc; }
+
+__device__ __forceinline__ float square_sum(float8_t x) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], s);
+    return s;
+}
+__device__ __forceinline__ float abs_max(float8_t x) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaxf(s, fabsf(x[j]));
+    return s;
+}
+
+// Eight e4m3 codes (OCP, round to nearest even).
+__device__ __forceinline__ uint2 e4m3_codes(float8_t x) {
+    int a = 0, b = 0;
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], a, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], a, true);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(x[4], x[5], b, false);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(x[6], x[7], b, true);
+    return make_uint2((unsigned)a, (unsigned)b);
+}
+__device__ __forceinline__ void store_codes(unsigned char* col, int i, int n, uint2 c) {
+    if (i + 8 <= n) { __builtin_memcpy(col + i, &c, 8); return; }
+    const unsigned long long bits = c.x | ((unsigned long long)c.y << 32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (i + j < n) col[i + j] = (unsigned char)(bits >> (8 * j));
+}
+
+// Largest value over the lanes of one group of rows (group / 8 lanes, or fewer when the column has fewer).
+__device__ __forceinline__ float lanes_allmax(float x, int lanes) {
+    if (lanes >= 2) x = fmaxf(x, dpp_mov<DPP_QUAD_XOR1>(x));
+    if (lanes >= 4) x = fmaxf(x, dpp_mov<DPP_QUAD_XOR2>(x));
+    if (lanes >= 8) x = fmaxf(x, dpp_mov<DPP_ROW_HALF_MIRROR>(x));
+    if (lanes >= 16) x = fmaxf(x, dpp_mov<DPP_ROW_MIRROR>(x));
+    return x;
+}
+
+template <class T, int TPC, int NV>
+__global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
+    constexpr int CPB = norm_block(TPC) / TPC;
+    __shared__ float sh[2][TPC > 64 ? TPC / 64 : 1];
+    const long long c = (long long)blockIdx.x * CPB + threadIdx.x / TPC;
+    if (c >= a.ncols) return;
+    const int t = threadIdx.x % TPC, n = a.nrows;
+    const T* x = (const T*)a.X + c * a.ldx;
+    float8_t h[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) h[v] = load_col8(x, (v * TPC + t) * 8, n).wide();
+    if (a.R != nullptr) {
+        const T* r = (const T*)a.R + c * a.ldr;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) h[v] += load_col8(r, (v * TPC + t) * 8, n).wide();
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) ss += square_sum(h[v]);
+    if (a.H != nullptr) {
+        T* o = (T*)a.H + c * a.ldh;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_col8(o, (v * TPC + t) * 8, n, h[v]);
+    }
+    if (a.Y == nullptr && a.Q == nullptr) return;
+    ss = column_allsum<TPC>(ss, sh[0]);
+    const float rs = 1.f / sqrtf(ss / (float)n + a.eps);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const float8_t w = load_col8(a.w, (v * TPC + t) * 8, n).wide();
+        h[v] = h[v] * rs * w;
+    }
+    if (a.Y != nullptr) {
+        T* o = (T*)a.Y + c * a.ldy;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_col8(o, (v * TPC + t) * 8, n, h[v]);
+    }
+    if (a.Q == nullptr) return;
+    unsigned char* q = a.Q + c * a.ldq;
+    if (a.group == 0) {
+        float m = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) m = fmaxf(m, abs_max(h[v]));
+        m = column_allmax<TPC>(m, sh[1]);
+        const float scale = fmaxf(m / kE4M3Max, kScaleMin), inv = 1.f / scale;
+        if (t == 0) a.scales[c] = scale;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_codes(q, (v * TPC + t) * 8, n, e4m3_codes(h[v] * inv));
+        return;
+    }
+    const int lanes = a.group >> 3, ng = (n + a.group - 1) / a.group;
+    const int span = lanes < TPC ? lanes : TPC;          // TPC < lanes: the column is one group
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int i = (v * TPC + t) * 8;
+        const float m = lanes_allmax(abs_max(h[v]), span);
+        const float scale = fmaxf(m / kE4M3Max, kScaleMin), inv = 1.f / scale;
+        if (i < n) {
+            if ((t & (span - 1)) == 0) a.scales[c * ng + i / a.group] = scale;
+            store_codes(q, i, n, e4m3_codes(h[v] * inv));
+        }
+    }
+}
+
+// Gradients. With g = dy * w (elementwise) and u = h * rs:
+//   dx = rs * (g - u * mean(g * u)) + dh,   dw_i = sum over columns of dy_i * u_i
+// Every workgroup walks columns c0, c0 + slots, ... and keeps its share of dw in registers; the shares go to partial
+// (one row of nrows floats per workgroup) and are added in a fixed order by k_add_shares.
+template <class T, int TPC, int NV>
+__global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
+    constexpr int CPB = norm_block(TPC) / TPC;
+    __shared__ float sh[2][2][TPC > 64 ? TPC / 64 : 1];
+    const int t = threadIdx.x % TPC, n = a.nrows;
+    float8_t dw[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) dw[v] = (float8_t)(0.f);
+    int turn = 0;
+    for (long long c = (long long)blockIdx.x * CPB + threadIdx.x / TPC; c < a.ncols; c += (long long)gridDim.x * CPB) {
+        const T* hp = (const T*)a.H + c * a.ldh;
+        const T* gp = (const T*)a.dY + c * a.lddy;
+        Raw8<T> h[NV], g[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            h[v] = load_col8(hp, (v * TPC + t) * 8, n);
+            g[v] = load_col8(gp, (v * TPC + t) * 8, n);
+        }
+        float hh = 0.f, gh = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const float8_t x = h[v].wide(), y = g[v].wide() * load_col8(a.w, (v * TPC + t) * 8, n).wide();
+            hh += square_sum(x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) gh = fmaf(x[j], y[j], gh);
+        }
+        hh = column_allsum<TPC>(hh, sh[turn][0]);
+        gh = column_allsum<TPC>(gh, sh[turn][1]);
+        turn ^= 1;
+        const float rs = 1.f / sqrtf(hh / (float)n + a.eps);
+        const float k = rs * rs * (gh / (float)n);
+        T* o = (T*)a.dX + c * a.lddx;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int i = (v * TPC + t) * 8;
+            const float8_t x = h[v].wide(), y = g[v].wide();
+            float8_t d = rs * (y * load_col8(a.w, i, n).wide() - x * k);
+            dw[v] += y * x * rs;
+            if (a.dH != nullptr) d += load_col8((const T*)a.dH + c * a.lddh, i, n).wide();
+            store_col8(o, i, n, d);
+        }
+    }
+    if (a.dw == nullptr) return;
+    float* share = partial + (size_t)blockIdx.x * n;
+    if constexpr (CPB > 1) {
+        __shared__ float sum[TPC * 8 * NV];
+        for (int i = threadIdx.x; i < TPC * 8 * NV; i += BM_BLOCK) sum[i] = 0.f;
+        for (int p = 0; p < CPB; ++p) {
+            __syncthreads();
+            if ((int)threadIdx.x / TPC == p) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum[(v * TPC + t) * 8 + j] += dw[v][j];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += BM_BLOCK) share[i] = sum[i];
+    } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_col8(share, (v * TPC + t) * 8, n, dw[v]);
+    }
+}
+
+// dw[i] = beta * dw[i] + sum over shares of partial[share][i]: 16 rows x 64 threads per workgroup, thread (x, y) adds
+// shares y, y + 64, ... of row x, then the 64 sums of a row are added by halves.
+__global__ __launch_bounds__(1024) void k_add_shares(int n, int nshares, const float* __restrict__ partial, float* __restrict__ dw,
+                                                     int beta) {
+    __shared__ float sh[64][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int i = blockIdx.x * 16 + x;
+    float s = 0.f;
+    if (i < n)
+        for (int p = y; p < nshares; p += 64) s += partial[(size_t)p * n + i];
+    sh[y][x] = s;
+    for (int step = 32; step > 0; step >>= 1) {
+        __syncthreads();
+        if (y < step) sh[y][x] += sh[y + step][x];
+    }
+    if (y == 0 && i < n) dw[i] = beta ? dw[i] + sh[0][x] : sh[0][x];
+}
+
+template <class T, int TPC, int NV>
+hipError_t launch_norm(const NormArgs& a, hipStream_t s) {
+    constexpr int CPB = norm_block(TPC) / TPC;
+    const unsigned grid = (unsigned)((a.ncols + CPB - 1LL) / CPB);
+    hipLaunchKernelGGL((k_rmsnorm<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a);
+    return hipGetLastError();
+}
+constexpr int kShares = 512;      // workgroups of the gradient, at most
+template <class T, int TPC, int NV>
+hipError_t launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
+    constexpr int CPB = norm_block(TPC) / TPC;
+    const long long want = (a.ncols + CPB - 1LL) / CPB;
+    const unsigned grid = (unsigned)(want < kShares ? want : kShares);
+    float* partial = nullptr;
+    if (a.dw != nullptr) {
+        hipError_t err;
+        partial = (float*)ws_get(WS_NORM_SHARES, sizeof(float) * (size_t)kShares * (size_t)a.nrows, &err, s);
+        if (!partial) return err;
+    }
+    hipLaunchKernelGGL((k_rmsnorm_grad<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a, partial);
+    if (a.dw != nullptr)
+        hipLaunchKernelGGL(k_add_shares, dim3((a.nrows + 15) / 16), dim3(1024), 0, s, a.nrows, (int)grid, partial, a.dw, a.beta);
+    return hipGetLastError();
+}
+
+// Threads per column and vectors per thread: the fewest that hold n elements.
+template <class T, class F>
+hipError_t by_height(int n, F&& f) {
+    const int vecs = (n + 7) / 8;
+    if (vecs <= 8) return f.template go<T, 8, 1>();
+    if (vecs <= 16) return f.template go<T, 16, 1>();
+    if (vecs <= 32) return f.template go<T, 32, 1>();
+    if (vecs <= 64) return f.template go<T, 64, 1>();
+    if (vecs <= 128) return f.template go<T, 64, 2>();
+    if (vecs <= 256) return f.template go<T, 256, 1>();
+    if (vecs <= 512) return f.template go<T, 256, 2>();
+    if (vecs <= 1024) return f.template go<T, 512, 2>();
+    if (vecs <= 2048) return f.template go<T, 1024, 2>();
+    return f.template go<T, 1024, 4>();
+}
+struct Norm {
+    const NormArgs& a;
+    hipStream_t s;
+    template <class T, int TPC, int NV> hipError_t go() { return launch_norm<T, TPC, NV>(a, s); }
+};
+struct NormGrad {
+    const NormGradArgs& a;
+    hipStream_t s;
+    template <class T, int TPC, int NV> hipError_t go() { return launch_norm_grad<T, TPC, NV>(a, s); }
+};
+template <class F>
+hipError_t by_type(int type, int n, F f) {
+    return type == ELEM_F32 ? by_height<float>(n, f) : type == ELEM_F16 ? by_height<f16_t>(n, f) : by_height<bf16_t>(n, f);
+}
+
+}  // namespace
+
+hipError_t rmsnorm(const NormArgs& a, hipStream_t s) { return by_type(a.type, a.nrows, Norm{a, s}); }
+
+hipError_t rmsnorm_grad(const NormGradArgs& a, hipStream_t s) { return by_type(a.type, a.nrows, NormGrad{a, s}); }
+
+}  // namespace bm

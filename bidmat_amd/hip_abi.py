@@ -68,6 +68,17 @@ SIGNATURES = {
     "bidmat_sdmult_plan": (C.c_int, [vp, C.c_int, vp, vp, C.c_int, vp, C.c_int, vp]),
     "bidmat_transpose": (C.c_int, [C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp]),
     "bidmat_applyop_flat": (C.c_int, [vp, vp, vp, C.c_longlong, C.c_int, vp]),
+    # operators over a model's columns
+    "bidmat_rmsnorm": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_float, vp, C.c_int, vp, C.c_int, vp, C.c_int,
+                                 vp, C.c_int, vp]),
+    "bidmat_rmsnorm_grad": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_float, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp,
+                                      C.c_int, vp]),
+    "bidmat_route": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, vp, vp,
+                               vp, vp, vp, vp]),
+    "bidmat_route_grad": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, vp, vp, vp, vp, C.c_int, vp]),
+    "bidmat_distill": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, C.c_float, vp, vp, vp, vp, C.c_int, vp]),
+    "bidmat_distill_grad": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, C.c_float, vp, vp, vp, C.c_int, vp]),
+    "bidmat_dsmult_q8_csc": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp, vp, vp, vp, C.c_int, vp]),
     # memory / runtime
     "bidmat_device_count": (C.c_int, [c_int_p]),
     "bidmat_set_device": (C.c_int, [C.c_int]),
@@ -103,6 +114,10 @@ SIGNATURES = {
     "bidmat_get_option": (C.c_longlong, [C.c_char_p]),
     "bidmat_release_caches": (C.c_int, []),
 }
+
+# element types and kinds of scores (the enums of the header)
+F32, F16, BF16 = 0, 1, 2
+SOFTMAX, SIGMOID = 0, 1
 
 _lib = None
 

@@ -363,7 +363,77 @@ int bidmat_applyop_flat(const float *A, const float *B, float *C, long long n, i
                         void *stream);
 
 /* ------------------------------------------------------------------------------------
- * 3. Device memory and runtime helpers (what the reference does through JCuda:
+ * 3. Operators over a model's columns (no counterpart in the reference): a column is a token, a document or another
+ *    example, a row a feature, an expert or a word.  Dense matrices are column-major with a leading dimension of their
+ *    own (in elements, >= the rows) and hold fp32, fp16 or bf16 elements (`type`); addresses need the alignment of one
+ *    element.  Everything is computed and summed in fp32 and rounded to nearest even once, when it is written.  Weights,
+ *    scales and values of sparse matrices are fp32.  They only enqueue work on `stream`.  An output may be one of the
+ *    call's dense inputs (same address and leading dimension); any other overlap returns hipErrorInvalidValue.
+ * ------------------------------------------------------------------------------------ */
+enum { BIDMAT_F32 = 0, BIDMAT_F16 = 1, BIDMAT_BF16 = 2 };
+enum { BIDMAT_SOFTMAX = 0, BIDMAT_SIGMOID = 1 };
+
+/* Root-mean-square normalisation of columns behind a residual's addition:
+ *   h = x + r (R nullable: h = x),   y_i = h_i * w_i / sqrt(mean(h^2) + eps)
+ * H (nullable) receives h, Y (nullable) y.  Q and scales (both or neither) receive y in 8 bits: e4m3 codes (OCP, nrows x
+ * ncols, leading dimension ldq) and one scale per `group` rows (0 = the column; 32, 64 or 128; the last group of a column
+ * may be short; scales is ceil(nrows / group) x ncols): scale = max(largest |y| / 448, 2^-126), code = e4m3(y / scale).
+ * y is formed from the unrounded sum.  A NaN or an infinity in a column of h makes its y and codes NaN.
+ * nrows <= 32768 (a column stays in the registers of one workgroup). */
+int bidmat_rmsnorm(int nrows, int ncols, int type, const void *X, int ldx, const void *R, int ldr, const float *w,
+                   float eps, void *H, int ldh, void *Y, int ldy, unsigned char *Q, int ldq, float *scales, int group,
+                   void *stream);
+/* Its gradient, from the h that was written: dX = the gradient with respect to x (and to r, which has the same one), given
+ * dY and, nullable, dH: what arrives at h itself.  dw (nullable, nrows floats) = beta*dw + the gradient of w. */
+int bidmat_rmsnorm_grad(int nrows, int ncols, int type, const void *H, int ldh, const float *w, float eps, const void *dY,
+                        int lddy, const void *dH, int lddh, void *dX, int lddx, float *dw, int beta, void *stream);
+
+/* Routing of columns to experts: Z (nexperts x ncols) scores; the result is a CSC matrix G (nexperts x ncols) with topk
+ * nonzeros in every column, rows ascending: data Gdata, rows Gir, nullable Gic and Gjc (ncols+1), for A*S, A *^ S, DDS
+ * and the transpose (whose columns list the tokens of each expert).
+ *   p = softmax or sigmoid (`kind`) of a column;  key = p + bias (bias nullable; without bias and with one group: the score)
+ *   the experts lie in ngroups equal groups in order; the topgroups groups with the largest sum of their two largest keys
+ *   stay open, and of their experts the topk largest keys are taken; the lower index first among equals
+ *   weight = scale * p, or with renorm scale * p / (sum of the taken p); the bias takes no part in it
+ * Keys are compared as their values in 64 bits compare.  A score of -inf closes an expert to its column; where fewer than
+ * topk are open, the remaining entries are the lowest other experts with weight 0 (a column of -inf is padding).  A NaN
+ * among a column's scores (softmax: or +inf) makes its weights NaN, its experts 0 .. topk-1.
+ * counts (nullable, nexperts ints): how many columns took each expert (entries of weight 0 by the rule above, and columns
+ * with NaN, not counted).  nexperts <= 1024, ngroups <= 64, topk <= min(64, experts in topgroups groups). */
+int bidmat_route(int nexperts, int ncols, int type, const void *Z, int ldz, const float *bias, int kind, int ngroups,
+                 int topgroups, int topk, int renorm, float scale, float *Gdata, int *Gir, int *Gic, int *Gjc, int *counts,
+                 void *stream);
+/* The gradient of the weights: dZ (whole, zeros where nothing arrives) from dG, the gradient of Gdata (bidmat_dds of the
+ * experts' columns with the gradient of a product A*G, for one).  Gdata, Gir: what bidmat_route wrote; an entry of weight
+ * 0 counts as not taken.  No gradient goes through the choice of experts, and none to the bias. */
+int bidmat_route_grad(int nexperts, int ncols, int type, const void *Z, int ldz, int kind, int topk, int renorm, float scale,
+                      const float *Gdata, const int *Gir, const float *dG, void *dZ, int lddz, void *stream);
+
+/* Distillation from a teacher's largest logits.  Z (nrows x ncols) the student's logits; the teacher's are the stored
+ * values of a CSC matrix T of the same shape (nnz, Tdata, Tir, Tjc), any number in a column.  With x = z / temperature,
+ * p = softmax of a column's stored values / temperature, q = softmax(x) over all rows:
+ *   loss[c] = weight[c] * temperature^2 * sum_j p_j (log p_j - log q_j),   dZ = weight[c] * temperature * (q - p)
+ * weight (nullable = 1) is one float per column.  lse (nullable) receives log sum exp(x).  loss, lse and dZ are each
+ * nullable, not all.  dZ may be Z.  A column without stored values (or only -inf), or of weight 0, has loss 0 and
+ * gradient 0 whatever its logits are.  Rows need not be sorted; the shares of a row stored twice add.  Entries whose row lies outside
+ * the matrix are left out.  A row whose student logit is -inf has q = 0 (with p > 0: loss +inf); a column of them has no
+ * softmax: NaN.  nrows <= 2^30. */
+int bidmat_distill(int nrows, int ncols, int type, const void *Z, int ldz, int nnz, const float *Tdata, const int *Tir,
+                   const int *Tjc, float temperature, const float *weight, float *loss, float *lse, void *dZ, int lddz,
+                   void *stream);
+/* The gradient alone, from the lse that bidmat_distill wrote. */
+int bidmat_distill_grad(int nrows, int ncols, int type, const void *Z, int ldz, int nnz, const float *Tdata, const int *Tir,
+                        const int *Tjc, float temperature, const float *weight, const float *lse, void *dZ, int lddz,
+                        void *stream);
+
+/* C = beta*C + A*S with A in 8 bits, A[i, r] = scales[i / group, r] * e4m3(Q[i, r]): codes and scales as bidmat_rmsnorm
+ * writes them (Q k x nrowsS with leading dimension ldq, scales ceil(k / group) x nrowsS, group 0 = one per column).
+ * Otherwise bidmat_dsmult_csc: S and C fp32, columns longer than "seglen" cut into segments, the same bits every time. */
+int bidmat_dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char *Q, int ldq, const float *scales, int group,
+                         const float *Sdata, const int *Sir, const int *Sjc, float *C, int beta, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * 4. Device memory and runtime helpers (what the reference does through JCuda:
  *    cublasAlloc/cublasFree GSMat.scala:519-522,225-232; cudaMemcpy GSMat.scala:625-633;
  *    cudaMemset GMat.scala:562-566; cudaMemGetInfo GFunctions.scala:208-213).
  * ------------------------------------------------------------------------------------ */
