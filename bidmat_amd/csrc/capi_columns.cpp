@@ -83,6 +83,7 @@ API int bidmat_rmsnorm_grad(int nrows, int ncols, int type, const void* H, int l
 
 API int bidmat_route(int nexperts, int ncols, int type, const void* Z, int ldz, const float* bias, int kind, int ngroups, int topgroups,
                      int topk, int renorm, float scale, float* Gdata, int* Gir, int* Gic, int* Gjc, int* counts, void* stream) {
+    auto lock = bm::device_lock();
     if (nexperts < 1 || nexperts > bm::kRouteMaxExperts || ncols < 0 || !type_ok(type)) return kInvalid;
     if ((kind != BIDMAT_SOFTMAX && kind != BIDMAT_SIGMOID) || (renorm != 0 && renorm != 1)) return kInvalid;
     if (ngroups < 1 || ngroups > bm::kRouteMaxGroups || nexperts % ngroups != 0 || topgroups < 1 || topgroups > ngroups) return kInvalid;

@@ -19,6 +19,8 @@
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
+#include "workspace.hpp"
+#include <limits.h>
 
 namespace bm {
 namespace {
@@ -42,22 +44,41 @@ __device__ __forceinline__ V lanes_max(V x) {
     }
     return x;
 }
-// Largest value of the wave in a scalar register: shifts inside rows of 16 lanes, then row results broadcast onwards.
-__device__ __forceinline__ float wave_max(float x) {
-    constexpr int low = (int)0xff800000;      // -inf
-#define BM_STEP(ctrl, rows) x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(x), ctrl, rows, 0xf, false)))
-    BM_STEP(0x111, 0xf); BM_STEP(0x112, 0xf); BM_STEP(0x114, 0xf); BM_STEP(0x118, 0xf);      // row_shr 1, 2, 4, 8
-    BM_STEP(0x142, 0xa); BM_STEP(0x143, 0xc);                                                // row_bcast 15, 31
+// Reductions of the wave into a scalar register, and the inclusive prefix sum: shifts inside rows of 16 lanes, then row
+// results broadcast onwards. On whole numbers each step is one instruction (a float maximum takes three).
+#define BM_WAVE_STEPS(STEP) \
+    STEP(0x111, 0xf) STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf) /* row_shr 1, 2, 4, 8 */ \
+    STEP(0x142, 0xa) STEP(0x143, 0xc)                                   /* row_bcast 15, 31 */
+__device__ __forceinline__ int wave_max(int x) {
+#define BM_STEP(ctrl, rows) x = max(x, __builtin_amdgcn_update_dpp(INT_MIN, x, ctrl, rows, 0xf, false));
+    BM_WAVE_STEPS(BM_STEP)
 #undef BM_STEP
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ int wave_min(int x) {
+#define BM_STEP(ctrl, rows) x = min(x, __builtin_amdgcn_update_dpp(INT_MAX, x, ctrl, rows, 0xf, false));
+    BM_WAVE_STEPS(BM_STEP)
+#undef BM_STEP
+    return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ int wave_prefix(int x) {
+#define BM_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false);
+    BM_WAVE_STEPS(BM_STEP)
+#undef BM_STEP
+    return x;
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#define BM_STEP(ctrl, rows) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xf, false))
-    BM_STEP(0x111, 0xf); BM_STEP(0x112, 0xf); BM_STEP(0x114, 0xf); BM_STEP(0x118, 0xf);
-    BM_STEP(0x142, 0xa); BM_STEP(0x143, 0xc);
+#define BM_STEP(ctrl, rows) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xf, false));
+    BM_WAVE_STEPS(BM_STEP)
 #undef BM_STEP
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
+
+// Floats as whole numbers of the same order (and back: the map is its own inverse), -0 as 0. kShut stands below all of them.
+constexpr int kShut = INT_MIN;
+__device__ __forceinline__ int flip(int i) { return i ^ ((i >> 31) & 0x7fffffff); }
+__device__ __forceinline__ int ordered(float x) { return flip(__float_as_int(x + 0.f)); }
+__device__ __forceinline__ float number(int i) { return __int_as_float(flip(i)); }
 
 // Which of a column's experts are taken, from keys in 64 bits: bit j of the result is this lane's slot j. Rarely called: a
 // function of its own that reads its scores again (zp: of this lane's first expert), keeps its keys in LDS (slot j of lane
@@ -140,123 +161,111 @@ __device__ __noinline__ unsigned take_exact(const T* zp, const float* bias, doub
 }
 
 template <int N>
-__device__ __forceinline__ int count_from(const float (&key)[N], float t) {
+__device__ __forceinline__ int count_from(const int (&key)[N], int t) {
     int c = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) c += __popcll(__ballot(key[j] >= t));
     return c;
 }
 
-// The border below the `want` largest of the wave's keys (more than want are above -inf): they are the keys >= t, of
-// those that equal t only the first `ties` when ties > 0. `between`: t is no key but lies between two.
-struct Border { float t; int ties; bool between; };
+// The border below the `want` largest of the wave's keys, of which more than want are open: they are the keys >= t, and
+// where ties > 0 only the first `ties` of those that equal t.
+struct Border { int t, ties; };
 template <int N>
-__device__ __forceinline__ Border find_border(const float (&key)[N], int want) {
-    float best = key[0];
+__device__ __forceinline__ Border find_border(const int (&key)[N], int want) {
+    int best = key[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j) best = fmaxf(best, key[j]);
-    const float top = wave_max(best);
-    // every lane's largest key but those of lanes without an open one: at least as many keys reach the least of them
-    float lo = -wave_max(best > -INFINITY ? -best : -INFINITY);
+    for (int j = 1; j < N; ++j) best = max(best, key[j]);
+    int hi = wave_max(best) + 1, over = 0;
+    // the least of the lanes' largest keys is reached by at least as many keys as lanes have an open one
+    int lo = wave_min(best == kShut ? INT_MAX : best);
     int n = count_from(key, lo);
-    if (n < want) {
-        float least = INFINITY;
+    if (N > 1 && n < want) {
+        int least = INT_MAX;
 #pragma unroll
-        for (int j = 0; j < N; ++j) least = fminf(least, key[j] > -INFINITY ? key[j] : INFINITY);
-        lo = -wave_max(-least);
+        for (int j = 0; j < N; ++j) least = min(least, key[j] == kShut ? INT_MAX : key[j]);
+        lo = wave_min(least);
         n = count_from(key, lo);
     }
-    float hi = NAN;                 // none yet: no comparison with it holds
-    int above = 0;
-    if (n == want) return {lo, 0, false};
-    for (int i = 0; i < 14; ++i) {
-        const float end = hi < top ? hi : top, mid = 0.5f * lo + 0.5f * end;
-        if (!(mid > lo && mid < end)) break;
+    while (n != want && (unsigned)hi - (unsigned)lo > 1u) {
+        const int mid = lo + (int)(((unsigned)hi - (unsigned)lo) >> 1);
         const int c = count_from(key, mid);
-        if (c == want) return {mid, 0, true};
-        if (c > want) lo = mid; else { hi = mid; above = c; }
+        if (c >= want) { lo = mid; n = c; } else { hi = mid; over = c; }
     }
-    // what is left lies close together: one value at a time from above
-    for (;;) {
-        float next = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < N; ++j) next = fmaxf(next, key[j] >= hi ? -INFINITY : key[j]);
-        next = wave_max(next);
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) c += __popcll(__ballot(key[j] == next));
-        if (above + c >= want || !(next > -INFINITY)) return {next, above + c > want ? want - above : 0, false};
-        above += c;
-        hi = next;
-    }
+    return {lo, n > want ? want - over : 0};
 }
 // Whether keys that are off by at most e each have the same largest `want` as the exact ones.
 template <int N>
-__device__ __forceinline__ bool border_clear(const float (&key)[N], const Border& b, int want, float e) {
-    if (b.ties > 0) return false;
-    if (b.between) return count_from(key, b.t + e) == want && count_from(key, b.t - e) == want;
-    return count_from(key, b.t - 2.f * e) == want;
+__device__ __forceinline__ bool border_clear(const int (&key)[N], const Border& b, int want, float e) {
+    const float t = number(b.t);
+    return b.ties == 0 && count_from(key, wave_uniform(ordered(t + e))) == want && count_from(key, wave_uniform(ordered(t - e))) == want;
 }
 
 // The same in fp32; false: some key lies too close to a border.
-template <int VPL>
+template <class T, int VPL>
 __device__ __forceinline__ bool take_fast(const RouteArgs& a, const Deal& d, const float (&z)[VPL], const float (&bias)[VPL], float bmax,
                                           float top, float by, unsigned& taken) {
     const int l = threadIdx.x & 63;
+    int key[VPL];
     const bool plain = a.bias == nullptr && a.ngroups == 1;
-    float key[VPL];
+    if (plain) {
+        // scores of 16 bits differ in their upper bits only: fewer halvings until two that are equal are told so
+        constexpr int shift = sizeof(T) == 4 ? 0 : __is_same(T, f16_t) ? 13 : 16;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        if (plain) key[j] = z[j];
-        else if (a.kind == 0) key[j] = __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) * by;
-        else key[j] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[j] * kLog2e));
-        if (!plain) {
-            key[j] += bias[j];
-            key[j] = z[j] > -INFINITY && key[j] > -INFINITY ? key[j] : -INFINITY;
+        for (int j = 0; j < VPL; ++j) key[j] = z[j] > -INFINITY ? ordered(z[j]) >> shift : kShut;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            float p;
+            if (a.kind == 0) p = __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) * by;
+            else p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[j] * kLog2e));
+            p += bias[j];
+            key[j] = z[j] > -INFINITY && p > -INFINITY ? ordered(p) : kShut;
         }
     }
     // Error of a key near the value v: p = key - bias is off by up to 2^-16 of itself (exp of an argument of up to 88, the
     // sum), a sigmoid also by less than 2^-20 at all.
     const float most = a.kind == 0 ? INFINITY : 0x1p-20f * (1.f + bmax);
     if (a.ngroups > 1) {
-        float best = key[0], second = -INFINITY;
+        int best = key[0], second = kShut;
 #pragma unroll
         for (int j = 1; j < VPL; ++j) {
-            second = fmaxf(second, fminf(best, key[j]));
-            best = fmaxf(best, key[j]);
+            second = max(second, min(best, key[j]));
+            best = max(best, key[j]);
         }
-        auto merge = [&](float ob, float os) {
-            second = fmaxf(fminf(best, ob), fmaxf(second, os));
-            best = fmaxf(best, ob);
+        auto merge = [&](int ob, int os) {
+            second = max(min(best, ob), max(second, os));
+            best = max(best, ob);
         };
-        if (d.lanes >= 2) merge(dpp_mov<DPP_QUAD_XOR1>(best), dpp_mov<DPP_QUAD_XOR1>(second));
-        if (d.lanes >= 4) merge(dpp_mov<DPP_QUAD_XOR2>(best), dpp_mov<DPP_QUAD_XOR2>(second));
-        if (d.lanes >= 8) merge(dpp_mov<DPP_ROW_HALF_MIRROR>(best), dpp_mov<DPP_ROW_HALF_MIRROR>(second));
-        if (d.lanes >= 16) merge(dpp_mov<DPP_ROW_MIRROR>(best), dpp_mov<DPP_ROW_MIRROR>(second));
+#define BM_MERGE(ctrl) merge(__builtin_amdgcn_update_dpp(0, best, ctrl, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(0, second, ctrl, 0xf, 0xf, false))
+        if (d.lanes >= 2) BM_MERGE(DPP_QUAD_XOR1);
+        if (d.lanes >= 4) BM_MERGE(DPP_QUAD_XOR2);
+        if (d.lanes >= 8) BM_MERGE(DPP_ROW_HALF_MIRROR);
+        if (d.lanes >= 16) BM_MERGE(DPP_ROW_MIRROR);
         if (d.lanes >= 32) merge(__shfl_xor(best, 16, 64), __shfl_xor(second, 16, 64));
-        const float mine = second > -INFINITY ? best + second : best;
+#undef BM_MERGE
+        const int mine = best == kShut ? kShut : ordered(second == kShut ? number(best) : number(best) + number(second));
         // one lane of each group stands for it
-        float score[1] = {(l & (d.lanes - 1)) == 0 ? mine : -INFINITY};
-        if (__popcll(__ballot(score[0] > -INFINITY)) > a.topgroups) {
+        const int score[1] = {(l & (d.lanes - 1)) == 0 ? mine : kShut};
+        if (__popcll(__ballot(score[0] != kShut)) > a.topgroups) {
             const Border b = find_border(score, a.topgroups);
-            if (!border_clear(score, b, a.topgroups, fminf(2.f * most, 0x1p-15f * (fabsf(b.t) + 2.f * bmax)))) return false;
-            if (!(mine >= b.t)) {
+            if (!border_clear(score, b, a.topgroups, fminf(2.f * most, 0x1p-15f * (fabsf(number(b.t)) + 2.f * bmax)))) return false;
+            const bool shut = mine < b.t;
 #pragma unroll
-                for (int j = 0; j < VPL; ++j) key[j] = -INFINITY;
-            }
+            for (int j = 0; j < VPL; ++j) key[j] = shut ? kShut : key[j];
         }
     }
     taken = 0;
     int open = 0;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) open += __popcll(__ballot(key[j] > -INFINITY));
+    for (int j = 0; j < VPL; ++j) open += __popcll(__ballot(key[j] != kShut));
     if (open <= a.topk) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) taken |= key[j] > -INFINITY ? 1u << j : 0u;
+        for (int j = 0; j < VPL; ++j) taken |= key[j] != kShut ? 1u << j : 0u;
         return true;
     }
     const Border b = find_border(key, a.topk);
-    if (!plain && !border_clear(key, b, a.topk, fminf(most, 0x1p-16f * (fabsf(b.t) + bmax)))) return false;
+    if (!plain && !border_clear(key, b, a.topk, fminf(most, 0x1p-16f * (fabsf(number(b.t)) + bmax)))) return false;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) taken |= key[j] >= b.t ? 1u << j : 0u;
     if (b.ties > 0) {
@@ -264,19 +273,9 @@ __device__ __forceinline__ bool take_fast(const RouteArgs& a, const Deal& d, con
         unsigned equal = 0;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) equal |= key[j] == b.t ? 1u << j : 0u;
-        int mine = __popc(equal), before = mine;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int y = __shfl_up(before, m, 64);
-            if (l >= m) before += y;
-        }
-        int left = b.ties - (before - mine);
-#pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (equal >> j & 1) {
-                if (left <= 0) taken &= ~(1u << j);
-                --left;
-            }
+        int left = b.ties - (wave_prefix(__popc(equal)) - __popc(equal));
+        for (; equal != 0; equal &= equal - 1)
+            if (left-- <= 0) taken &= ~(equal & -equal);
     }
     return true;
 }
@@ -297,9 +296,48 @@ struct Chosen {                          // of one wave
     float top[kRouteBatch], by[kRouteBatch];            // softmax over all: p = exp(z - top) * by; top NaN: the column holds one
 };
 
-// BLOCK threads; ONE: a single workgroup, which writes the counts instead of adding to them.
+// The weights, rows and counts of columns c0 .. c0 + cols - 1, whose experts lie in ch: kp lanes per column.
+template <class T>
+__device__ __forceinline__ void write_weights(const RouteArgs& a, const Deal& d, const Chosen& ch, long long c0, int cols, int* hist) {
+    const int l = threadIdx.x & 63;
+    for (int b0 = 0; b0 < cols; b0 += 64 / d.kp) {
+        const int b = b0 + l / d.kp, s = l & (d.kp - 1);
+        const bool on = b < cols && s < a.topk;
+        const int e = on ? ch.row[b][s] : 0x8000, r = e & 0x7fff;
+        const bool valid = on && e < 0x8000;
+        const float top = b < cols ? ch.top[b] : 0.f, by = b < cols ? ch.by[b] : 0.f;
+        const long long c = c0 + b;
+        const float z = valid ? (float)((const T*)a.Z)[c * a.ldz + r] : -INFINITY;
+        float p;
+        if (a.renorm) {
+            const float high = lanes_max_rt(z, d.kp);
+            // Far below 0 sigmoid(z) is exp(z) to within a factor 1 + exp(z): with all taken scores below -30 their
+            // shares are a softmax's, where the sigmoids themselves may have left the range of fp32.
+            p = a.kind == 0 || high < -30.f ? expf(z - high) : 1.f / (1.f + expf(-z));
+            p = valid ? p : 0.f;
+            const float sum = lanes_sum_rt(p, d.kp);
+            p = sum > 0.f ? p * (a.scale / sum) : 0.f;
+        } else {
+            p = a.scale * (a.kind == 0 ? expf(z - top) * by : 1.f / (1.f + expf(-z)));
+            p = valid ? p : 0.f;
+        }
+        if (on) {
+            const long long q = c * a.topk + s;
+            a.ir[q] = r;
+            a.data[q] = top != top ? NAN : p;
+            if (a.ic != nullptr) a.ic[q] = (int)c;
+            if (valid && a.counts != nullptr) atomicAdd(&hist[r], 1);
+            if (s == 0 && a.jc != nullptr) {
+                a.jc[c] = (int)(c * a.topk);
+                if (c == a.ncols - 1) a.jc[c + 1] = (int)((c + 1) * a.topk);
+            }
+        }
+    }
+}
+
+// BLOCK threads; ONE: a single workgroup, which writes the counts; otherwise each workgroup its share of them.
 template <class T, int VPL, int BLOCK, bool ONE>
-__global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d) {
+__global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d, int* shares) {
     constexpr int WAVES = BLOCK / 64;
     __shared__ int hist[kRouteMaxExperts];
     __shared__ Chosen chosen[WAVES];
@@ -320,7 +358,7 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d) {
         bias[j] = a.bias != nullptr && j < own ? a.bias[first + j] : 0.f;
         bmax = fmaxf(bmax, fabsf(bias[j]));
     }
-    bmax = wave_max(bmax);
+    bmax = number(wave_max(ordered(bmax)));
     const bool sums = a.kind == 0 && (a.bias != nullptr || a.ngroups > 1 || !a.renorm);      // softmax over all is needed
     const long long end = (a.ncols - 1LL) * a.ldz + a.nexperts;                              // of the matrix, in elements
     const long long step = (long long)gridDim.x * WAVES * d.batch;
@@ -338,16 +376,18 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d) {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) z[j] = j < own ? (float)((const T*)a.Z)[at + j] : -INFINITY;
             }
+            // a NaN, or +inf where the softmax has no value
+            const int odd_class = a.kind == 0 ? 0x203 : 0x003;
             bool odd = false;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) odd = odd || z[j] != z[j] || (a.kind == 0 && z[j] == INFINITY);
+            for (int j = 0; j < VPL; ++j) odd = odd || __builtin_amdgcn_classf(z[j], odd_class);
             const bool bad = __ballot(odd) != 0;
             float top = 0.f, by = 1.f;
             if (sums) {
                 top = z[0];
 #pragma unroll
                 for (int j = 1; j < VPL; ++j) top = fmaxf(top, z[j]);
-                top = wave_max(top);
+                top = number(wave_max(ordered(top)));
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) sum += z[j] > -INFINITY ? __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) : 0.f;
@@ -355,45 +395,20 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d) {
                 by = sum > 0.f ? 1.f / sum : 0.f;
             }
             unsigned taken = 0;
-            if (!bad && !take_fast<VPL>(a, d, z, bias, bmax, top, by, taken)) 
+            if (!bad && !take_fast<T, VPL>(a, d, z, bias, bmax, top, by, taken)) 
                 taken = take_exact<T>((const T*)a.Z + at, a.bias != nullptr ? a.bias + first : nullptr, exact_keys + wave * 64 * d.each, own,
                                       d.each, a.kind, a.ngroups, a.topgroups, a.topk, d.lanes);
             // fewer than topk open: the lowest others fill the column
             const unsigned valid = taken;
-            const int mine = __popc(taken);
-            int before = mine, have;
-            {
-                // lanes hold at most a few: prefix over the wave
-                int s = mine;
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const int y = __shfl_up(s, m, 64);
-                    if (l >= m) s += y;
-                }
-                have = __builtin_amdgcn_readlane(s, 63);
-                before = s - mine;
-            }
+            int upto = wave_prefix(__popc(taken));
+            const int have = __builtin_amdgcn_readlane(upto, 63);
             if (have < a.topk) {
-                const unsigned rest = own > 0 ? ~taken & (own >= 32 ? ~0u : (1u << own) - 1u) : 0u;
-                const int n = __popc(rest);
-                int s = n;
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const int y = __shfl_up(s, m, 64);
-                    if (l >= m) s += y;
-                }
-                int left = a.topk - have - (s - n);
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-                    if ((rest >> j & 1) && left > 0) { taken |= 1u << j; --left; }
-                s = __popc(taken);
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const int y = __shfl_up(s, m, 64);
-                    if (l >= m) s += y;
-                }
-                before = s - __popc(taken);
+                unsigned rest = own > 0 ? ~taken & (own >= 32 ? ~0u : (1u << own) - 1u) : 0u;
+                int left = a.topk - have - (wave_prefix(__popc(rest)) - __popc(rest));
+                for (; rest != 0 && left > 0; rest &= rest - 1, --left) taken |= rest & -rest;
+                upto = wave_prefix(__popc(taken));
             }
+            int before = upto - __popc(taken);
             for (unsigned t = taken; t != 0; t &= t - 1) {
                 const int j = __builtin_ctz(t);
                 ch.row[b][before++] = (unsigned short)((first + j) | (valid >> j & 1 ? 0 : 0x8000));
@@ -405,49 +420,311 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d) {
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        // the weights: kp lanes per column
-        for (int b0 = 0; b0 < cols; b0 += 64 / d.kp) {
-            const int b = b0 + l / d.kp, s = l & (d.kp - 1);
-            const bool on = b < cols && s < a.topk;
-            const int e = on ? ch.row[b][s] : 0x8000, r = e & 0x7fff;
-            const bool valid = on && e < 0x8000;
-            const float top = b < cols ? ch.top[b] : 0.f, by = b < cols ? ch.by[b] : 0.f;
-            const long long c = c0 + b;
-            const float z = valid ? (float)((const T*)a.Z)[c * a.ldz + r] : -INFINITY;
-            float p;
-            if (a.renorm) {
-                const float high = lanes_max_rt(z, d.kp);
-                // Far below 0 sigmoid(z) is exp(z) to within a factor 1 + exp(z): with all taken scores below -30 their
-                // shares are a softmax's, where the sigmoids themselves may have left the range of fp32.
-                p = a.kind == 0 || high < -30.f ? expf(z - high) : 1.f / (1.f + expf(-z));
-                p = valid ? p : 0.f;
-                const float sum = lanes_sum_rt(p, d.kp);
-                p = sum > 0.f ? p * (a.scale / sum) : 0.f;
-            } else {
-                p = a.scale * (a.kind == 0 ? expf(z - top) * by : 1.f / (1.f + expf(-z)));
-                p = valid ? p : 0.f;
-            }
-            if (on) {
-                const long long q = c * a.topk + s;
-                a.ir[q] = r;
-                a.data[q] = top != top ? NAN : p;
-                if (a.ic != nullptr) a.ic[q] = (int)c;
-                if (valid && a.counts != nullptr) atomicAdd(&hist[r], 1);
-                if (s == 0 && a.jc != nullptr) {
-                    a.jc[c] = (int)(c * a.topk);
-                    if (c == a.ncols - 1) a.jc[c + 1] = (int)((c + 1) * a.topk);
-                }
-            }
-        }
+        write_weights<T>(a, d, ch, c0, cols, hist);
         __builtin_amdgcn_wave_barrier();
     }
     if (a.counts != nullptr) {
-        // whole numbers: the same total in any order
         __syncthreads();
         for (int e = threadIdx.x; e < a.nexperts; e += BLOCK) {
             if (ONE) a.counts[e] = hist[e];
-            else if (hist[e] != 0) atomicAdd(&a.counts[e], hist[e]);
+            else shares[(size_t)blockIdx.x * a.nexperts + e] = hist[e];
         }
+    }
+}
+
+// One column decided from keys in 64 bits by a whole wave; its experts (bit 15: named only to fill the column) go to out.
+template <class T>
+__device__ __forceinline__ void exact_column(const RouteArgs& a, const Deal& d, long long c, double* keys, unsigned short* out) {
+    const int l = threadIdx.x & 63, g = l / d.lanes, o = (l & (d.lanes - 1)) * d.each;
+    const int first = g * d.size + o, room = d.size - o < d.each ? d.size - o : d.each;
+    const int own = g < a.ngroups && room > 0 ? room : 0;
+    const unsigned valid = take_exact<T>((const T*)a.Z + c * a.ldz + first, a.bias != nullptr ? a.bias + first : nullptr, keys, own, d.each,
+                                         a.kind, a.ngroups, a.topgroups, a.topk, d.lanes);
+    unsigned taken = valid;
+    int upto = wave_prefix(__popc(taken));
+    const int have = __builtin_amdgcn_readlane(upto, 63);
+    if (have < a.topk) {
+        unsigned rest = own > 0 ? ~taken & (own >= 32 ? ~0u : (1u << own) - 1u) : 0u;
+        int left = a.topk - have - (wave_prefix(__popc(rest)) - __popc(rest));
+        for (; rest != 0 && left > 0; rest &= rest - 1, --left) taken |= rest & -rest;
+        upto = wave_prefix(__popc(taken));
+    }
+    int before = upto - __popc(taken);
+    for (unsigned t = taken; t != 0; t &= t - 1) {
+        const int j = __builtin_ctz(t);
+        out[before++] = (unsigned short)((first + j) | (valid >> j & 1 ? 0 : 0x8000));
+    }
+}
+
+// ---- 16 lanes per column
+// The same for up to 256 experts in up to 16 groups and up to 16 of them taken: four columns per wave, so that what lanes do
+// together costs a quarter per column and needs no step across rows of 16 lanes. A lane holds up to 16 experts; counts
+// run on the vector unit (a compare and an addition per slot).
+template <int CTRL>
+__device__ __forceinline__ int row_move(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true); }
+#define BM_ROW_ALL(x, op)                                                     \
+    x = op(x, row_move<DPP_QUAD_XOR1>(x)); x = op(x, row_move<DPP_QUAD_XOR2>(x)); \
+    x = op(x, row_move<DPP_ROW_HALF_MIRROR>(x)); x = op(x, row_move<DPP_ROW_MIRROR>(x))
+__device__ __forceinline__ int add_int(int x, int y) { return x + y; }
+__device__ __forceinline__ int row_max(int x) { BM_ROW_ALL(x, max); return x; }
+__device__ __forceinline__ int row_min(int x) { BM_ROW_ALL(x, min); return x; }
+__device__ __forceinline__ int row_sum(int x) { BM_ROW_ALL(x, add_int); return x; }
+__device__ __forceinline__ int row_prefix(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    return x;
+}
+template <int N>
+__device__ __forceinline__ int row_count(const int (&key)[N], int t) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) c += key[j] >= t;
+    return row_sum(c);
+}
+
+// Distance from lo to the smallest key of the column that reaches it.
+template <int N>
+__device__ __forceinline__ unsigned row_least_from(const int (&key)[N], int lo) {
+    unsigned x = ~0u;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x = min(x, (unsigned)key[j] - (unsigned)lo);
+#define BM_MIN(ctrl) x = min(x, (unsigned)row_move<ctrl>((int)x))
+    BM_MIN(DPP_QUAD_XOR1); BM_MIN(DPP_QUAD_XOR2); BM_MIN(DPP_ROW_HALF_MIRROR); BM_MIN(DPP_ROW_MIRROR);
+#undef BM_MIN
+    return x;
+}
+
+// How many groups' scores lie at or above lo, and above hi, among the other groups of the column (LG lanes per group).
+template <int LG, int N>
+__device__ __forceinline__ void row_rank(float score, float lo, float hi, int& reach, int& pass) {
+    if constexpr (N < 16) {
+        if constexpr (N % LG == 0) {
+            const float other = __int_as_float(row_move<0x120 + N>(__float_as_int(score)));      // row_ror N
+            reach += other >= lo;
+            pass += other > hi;
+        }
+        row_rank<LG, N + 1>(score, lo, hi, reach, pass);
+    }
+}
+
+// Exact keys (scores of 16 bits, no bias, no groups) get the expert's number into their lower bits, so that no two are
+// equal and the lower expert stands higher. Other keys are p + bias + bmax: never negative, so that their bits are in
+// order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
+template <class T, int VPL>
+__device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, const float (&z)[VPL], const float (&bias)[VPL], float bmax,
+                                             float top, float by, int first, bool& fine) {
+    const bool plain = a.bias == nullptr && a.ngroups == 1;
+    int key[VPL];
+    if (plain) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            int k = ordered(z[j]);
+            if constexpr (sizeof(T) == 2) k = ((k >> (__is_same(T, f16_t) ? 13 : 16)) << 8) | (255 - first - j);
+            key[j] = z[j] > -INFINITY ? k : kShut;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            float p;
+            if (a.kind == 0) p = __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) * by;
+            else p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[j] * kLog2e));
+            key[j] = z[j] > -INFINITY ? __float_as_int(p + bias[j]) : kShut;
+        }
+    }
+    // Error of a key: p is off by up to 2^-16 of itself (exp of an argument of up to 88, the sum; by is the largest p of a
+    // softmax), a sigmoid by less than 2^-21 at all; the additions of bias and bmax by 2^-23 of the result.
+    const float most = a.kind == 0 ? 0x1p-16f * by + 0x1p-21f * (by + bmax) : 0x1p-20f * (1.f + 3.f * bmax);
+    int best = key[0], second = kShut;
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) {
+        second = max(second, min(best, key[j]));
+        best = max(best, key[j]);
+    }
+    fine = true;
+    if (a.ngroups > 1) {
+        int b1 = best, b2 = second;
+        auto merge = [&](int ob, int os) {
+            b2 = max(min(b1, ob), max(b2, os));
+            b1 = max(b1, ob);
+        };
+        if (d.lanes >= 2) merge(row_move<DPP_QUAD_XOR1>(b1), row_move<DPP_QUAD_XOR1>(b2));
+        if (d.lanes >= 4) merge(row_move<DPP_QUAD_XOR2>(b1), row_move<DPP_QUAD_XOR2>(b2));
+        if (d.lanes >= 8) merge(row_move<DPP_ROW_HALF_MIRROR>(b1), row_move<DPP_ROW_HALF_MIRROR>(b2));
+        // each key carries bmax once: a group with a single open expert gets its second one here
+        const float score = b1 == kShut ? -INFINITY : __int_as_float(b1) + (b2 == kShut ? bmax : __int_as_float(b2));
+        const float e = 2.f * fminf(2.f * most + 0x1p-22f * score, 0x1p-14f * score);
+        int reach = 0, pass = 0;
+        switch (d.lanes) {
+        case 1: row_rank<1, 1>(score, score - e, score + e, reach, pass); break;
+        case 2: row_rank<2, 1>(score, score - e, score + e, reach, pass); break;
+        case 4: row_rank<4, 1>(score, score - e, score + e, reach, pass); break;
+        default: row_rank<8, 1>(score, score - e, score + e, reach, pass); break;
+        }
+        const bool in = reach < a.topgroups, out = pass >= a.topgroups;
+        if (b1 != kShut && !in && !out) fine = false;
+        if (!in) {
+            best = second = kShut;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) key[j] = kShut;
+        }
+    }
+    const int want = a.topk;
+    // [lo, hi): the border's bracket; n keys reach lo. First among the lanes' two largest, where want keys exist there.
+    int lo, hi = row_max(best), n;
+    hi = hi == kShut ? kShut + 2 : hi + 1;
+    {
+        int least = INT_MAX;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) least = min(least, key[j] == kShut ? INT_MAX : key[j]);
+        least = row_min(least);
+        const int two[2] = {best, second};
+        int first_lo = row_min(second == kShut ? (best == kShut ? INT_MAX : best) : second), first_hi = hi;
+        int c = row_count(two, first_lo);
+        const bool enough = c >= want;
+        while (__ballot(enough && c != want && (unsigned)first_hi - (unsigned)first_lo > 1u) != 0) {
+            const int mid = first_lo + (int)(((unsigned)first_hi - (unsigned)first_lo) >> 1);
+            const int m = row_count(two, mid);
+            if (m >= want) { first_lo = mid; c = m; } else first_hi = mid;
+        }
+        lo = enough ? first_lo : least;
+        n = row_count(key, lo);
+    }
+    while (__ballot(n > want) != 0) {
+        const bool wide = (unsigned)hi - (unsigned)lo > 1u;
+        if (__ballot(n > want + 3 && wide) != 0) {
+            const int mid = lo + (int)(((unsigned)hi - (unsigned)lo) >> 1);
+            const int m = row_count(key, mid);
+            if (m >= want) { lo = n > want ? mid : lo; n = n > want ? m : n; } else hi = n > want ? mid : hi;
+        } else {
+            // the smallest key of those that reach lo goes; equal ones are found out at the end
+            const int next = lo + (int)row_least_from(key, lo) + 1;
+            if (n > want) {
+                if (!wide) fine = false;
+                lo = wide ? next : lo;
+                n = wide ? n - 1 : want;
+            }
+        }
+    }
+    if (n > 0) lo += (int)row_least_from(key, lo);      // the border is a key: the smallest taken one
+    unsigned taken = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) taken |= key[j] != kShut && key[j] >= lo ? 1u << j : 0u;
+    const int have = row_sum(__popc(taken));
+    if (have > want) fine = false;
+    if (!(plain && sizeof(T) == 2)) {
+        // a border with open keys below it: exactly `want` above it, by more than their errors
+        const float t = plain ? 0.f : __int_as_float(lo);
+        const float e = 2.f * fminf(most, 0x1p-15f * t);
+        int open = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) open += key[j] != kShut;
+        open = row_sum(open);
+        const int reach = plain ? have : row_count(key, max(kShut + 1, __float_as_int(t - e)));
+        if (open > want && (have != want || reach != want)) fine = false;
+    }
+    return taken;
+}
+
+template <class T, int VPL>
+__global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, Deal d64, int* shares) {
+    constexpr int WAVES = BM_WAVES_PER_BLOCK;
+    __shared__ int hist[256];
+    __shared__ Chosen chosen[WAVES];
+    extern __shared__ double exact_keys[];      // 64 * d64.each per wave
+    if (a.counts != nullptr) {
+        for (int e = threadIdx.x; e < a.nexperts; e += BM_BLOCK) hist[e] = 0;
+        __syncthreads();
+    }
+    const int l = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
+    Chosen& ch = chosen[wave];
+    const int row = l >> 4, i = l & 15;
+    const int g = i / d.lanes, o = (i & (d.lanes - 1)) * d.each;
+    const int first = g * d.size + o;
+    const int room = d.size - o < d.each ? d.size - o : d.each;
+    const int own = g < a.ngroups && room > 0 ? room : 0;
+    float bias[VPL], bmax = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        bias[j] = a.bias != nullptr && j < own ? a.bias[first + j] : 0.f;
+        bmax = fmaxf(bmax, fabsf(bias[j]));
+    }
+    bmax = number(wave_max(ordered(bmax)));
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) bias[j] += bmax;
+    const bool sums = a.kind == 0 && (a.bias != nullptr || a.ngroups > 1 || !a.renorm);
+    const int odd_class = a.kind == 0 ? 0x203 : 0x003;
+    const long long end = (a.ncols - 1LL) * a.ldz + a.nexperts;
+    const long long step = (long long)gridDim.x * WAVES * d.batch;
+    for (long long c0 = ((long long)blockIdx.x * WAVES + wave) * d.batch; c0 < a.ncols; c0 += step) {
+        const int cols = (int)(a.ncols - c0 < d.batch ? a.ncols - c0 : d.batch);
+        for (int b0 = 0; b0 < cols; b0 += 4) {
+            const int b = b0 + row;
+            const long long c = c0 + (b < cols ? b : cols - 1);      // rows past the end repeat the last column
+            const long long at = c * a.ldz + first;
+            float z[VPL];
+            if (VPL >= 2 && at + VPL <= end) {
+                T raw[VPL];
+                __builtin_memcpy(raw, (const T*)a.Z + at, sizeof(raw));
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) z[j] = j < own ? (float)raw[j] : -INFINITY;
+            } else {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) z[j] = j < own ? (float)((const T*)a.Z)[at + j] : -INFINITY;
+            }
+            int odd = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) odd |= __builtin_amdgcn_classf(z[j], odd_class);
+            const bool bad = row_sum(odd) != 0;
+            float top = 0.f, by = 1.f;
+            if (sums) {
+                top = z[0];
+#pragma unroll
+                for (int j = 1; j < VPL; ++j) top = fmaxf(top, z[j]);
+                top = group_allmax<16>(top);
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) sum += z[j] > -INFINITY ? __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) : 0.f;
+                sum = group_allsum<16>(sum);
+                by = sum > 0.f ? 1.f / sum : 0.f;
+            }
+            bool fine;
+            unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, fine);
+            if (bad) { taken = 0; fine = true; }
+            // fewer than topk open: the lowest others fill the column
+            const unsigned valid = taken;
+            int upto = row_prefix(__popc(taken));
+            const int have = row_sum(__popc(taken));
+            if (__ballot(have < a.topk) != 0) {
+                unsigned rest = own > 0 ? ~taken & ((1u << own) - 1u) : 0u;
+                int left = a.topk - have - (row_prefix(__popc(rest)) - __popc(rest));
+                for (; rest != 0 && left > 0; rest &= rest - 1, --left) taken |= rest & -rest;
+                upto = row_prefix(__popc(taken));
+            }
+            int before = upto - __popc(taken);
+            const unsigned long long unclear = __ballot(!fine);
+            if (b < cols && (unclear >> (16 * row) & 0xffff) == 0) {
+                for (unsigned t = taken; t != 0; t &= t - 1) {
+                    const int j = __builtin_ctz(t);
+                    ch.row[b][before++] = (unsigned short)((first + j) | (valid >> j & 1 ? 0 : 0x8000));
+                }
+            }
+            if (b < cols && i == 0) {
+                ch.top[b] = bad ? NAN : top;
+                ch.by[b] = by;
+            }
+            for (int r = 0; r < 4 && b0 + r < cols; ++r)
+                if (unclear >> (16 * r) & 0xffff) exact_column<T>(a, d64, c0 + b0 + r, exact_keys + wave * 64 * d64.each, ch.row[b0 + r]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        write_weights<T>(a, d, ch, c0, cols, hist);
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (a.counts != nullptr) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < a.nexperts; e += BM_BLOCK) shares[(size_t)blockIdx.x * a.nexperts + e] = hist[e];
     }
 }
 
@@ -497,6 +774,33 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_grad(RouteGradArgs a) {
     }
 }
 
+// counts[e] = sum of the workgroups' shares (atomics of a thousand workgroups on one address took longer than the rest): 16
+// experts x 64 threads.
+__global__ __launch_bounds__(1024) void k_add_counts(int n, int nshares, const int* __restrict__ shares, int* __restrict__ counts) {
+    __shared__ int sh[64][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, e = blockIdx.x * 16 + x;
+    int c = 0;
+    if (e < n)
+        for (int p = y; p < nshares; p += 64) c += shares[(size_t)p * n + e];
+    sh[y][x] = c;
+    for (int step = 32; step > 0; step >>= 1) {
+        __syncthreads();
+        if (y < step) sh[y][x] += sh[y + step][x];
+    }
+    if (y == 0 && e < n) counts[e] = sh[0][x];
+}
+hipError_t count_shares(const RouteArgs& a, unsigned grid, int** shares, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    *shares = nullptr;
+    if (a.counts != nullptr) *shares = (int*)ws_get(WS_ROUTE, sizeof(int) * (size_t)grid * a.nexperts, &e, s);
+    return e;
+}
+hipError_t add_counts(const RouteArgs& a, unsigned grid, const int* shares, hipStream_t s) {
+    if (a.counts != nullptr)
+        hipLaunchKernelGGL(k_add_counts, dim3((a.nexperts + 15) / 16), dim3(1024), 0, s, a.nexperts, (int)grid, shares, a.counts);
+    return hipGetLastError();
+}
+
 constexpr int kOneColumns = 64;          // up to so many columns one workgroup does it all, in one launch
 // Waves per workgroup: as many as leave the keys of take_exact 32 KiB of LDS.
 constexpr int route_waves(int vpl, bool one) { return vpl <= 4 ? (one ? 16 : 8) : 64 / vpl; }
@@ -507,30 +811,55 @@ hipError_t launch_route(const RouteArgs& a, Deal d, hipStream_t s) {
     if (a.ncols <= kOneColumns) {
         constexpr int waves = route_waves(VPL, true);
         d.batch = (a.ncols + waves - 1) / waves < kRouteBatch ? (a.ncols + waves - 1) / waves : kRouteBatch;
-        hipLaunchKernelGGL((k_route<T, VPL, 64 * waves, true>), dim3(1), dim3(64 * waves), waves * keys, s, a, d);
+        hipLaunchKernelGGL((k_route<T, VPL, 64 * waves, true>), dim3(1), dim3(64 * waves), waves * keys, s, a, d, (int*)nullptr);
         return hipGetLastError();
-    }
-    if (a.counts != nullptr) {
-        const hipError_t e = fill_i32(a.counts, a.nexperts, 0, s);
-        if (e != hipSuccess) return e;
     }
     constexpr int waves = route_waves(VPL, false);
     const long long all = 16384;      // waves that keep the device busy: fewer columns per wave rather than fewer waves
     d.batch = a.ncols >= all * kRouteBatch ? kRouteBatch : (int)((a.ncols + all - 1) / all);
     const long long want = (a.ncols + (long long)waves * d.batch - 1) / (waves * d.batch), most = 8192 / waves;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    hipLaunchKernelGGL((k_route<T, VPL, 64 * waves, false>), dim3(grid), dim3(64 * waves), waves * keys, s, a, d);
-    return hipGetLastError();
+    int* shares;
+    const hipError_t e = count_shares(a, grid, &shares, s);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_route<T, VPL, 64 * waves, false>), dim3(grid), dim3(64 * waves), waves * keys, s, a, d, shares);
+    return add_counts(a, grid, shares, s);
+}
+
+template <class T, int VPL>
+hipError_t launch_route_rows(const RouteArgs& a, Deal d, const Deal& d64, hipStream_t s) {
+    const long long all = 8192;
+    d.batch = a.ncols >= all * 8 ? 8 : 4;
+    const long long want = (a.ncols + BM_WAVES_PER_BLOCK * (long long)d.batch - 1) / (BM_WAVES_PER_BLOCK * d.batch);
+    const unsigned grid = (unsigned)(want < all / BM_WAVES_PER_BLOCK ? want : all / BM_WAVES_PER_BLOCK);
+    int* shares;
+    const hipError_t e = count_shares(a, grid, &shares, s);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_route_rows<T, VPL>), dim3(grid), dim3(BM_BLOCK), BM_WAVES_PER_BLOCK * 64 * sizeof(double) * d64.each, s, a, d, d64,
+                       shares);
+    return add_counts(a, grid, shares, s);
+}
+
+Deal deal(const RouteArgs& a, int lanes) {
+    Deal d;
+    d.size = a.nexperts / a.ngroups;
+    d.lanes = lanes / pow2ceil(a.ngroups);
+    d.each = d.lanes > 0 ? (d.size + d.lanes - 1) / d.lanes : INT_MAX;
+    d.kp = pow2ceil(a.topk);
+    d.batch = 1;
+    return d;
 }
 
 template <class T>
 hipError_t route_typed(const RouteArgs& a, hipStream_t s) {
-    Deal d;
-    d.size = a.nexperts / a.ngroups;
-    d.lanes = 64 / pow2ceil(a.ngroups);
-    d.each = (d.size + d.lanes - 1) / d.lanes;
-    d.kp = pow2ceil(a.topk);
-    d.batch = 1;
+    const Deal d = deal(a, 64), d16 = deal(a, 16);
+    if (a.ncols > kOneColumns && d16.each <= 16 && a.nexperts <= 256 && a.topk <= 16) {
+        if (d16.each <= 1) return launch_route_rows<T, 1>(a, d16, d, s);
+        if (d16.each <= 2) return launch_route_rows<T, 2>(a, d16, d, s);
+        if (d16.each <= 4) return launch_route_rows<T, 4>(a, d16, d, s);
+        if (d16.each <= 8) return launch_route_rows<T, 8>(a, d16, d, s);
+        return launch_route_rows<T, 16>(a, d16, d, s);
+    }
     if (d.each <= 1) return launch_route<T, 1>(a, d, s);
     if (d.each <= 2) return launch_route<T, 2>(a, d, s);
     if (d.each <= 4) return launch_route<T, 4>(a, d, s);

@@ -25,6 +25,7 @@ enum WsSlot {
     WS_ROWSUM,        // bytes         exact row sums: block maxima, 64-bit accumulators, flags
     WS_ROWSUM_TABLES, // u64[...]      exact row sums: the accumulator tables of the workgroups
     WS_NORM_SHARES,   // float[...]    shares of the weight gradient of the column normalisation, one per workgroup
+    WS_ROUTE,         // int[...]      routing: how many columns of a workgroup took each expert
     WS_DISTILL,       // bytes         distillation: log-sum parts per chunk of a column, statistics per teacher column
     WS_DISTILL_AT,    // float[nnz]    distillation: the student's logits at the teacher's entries
     WS_NSLOTS
