@@ -465,6 +465,11 @@ __device__ __forceinline__ int row_move(int x) { return __builtin_amdgcn_update_
 #define BM_ROW_ALL(x, op)                                                     \
     x = op(x, row_move<DPP_QUAD_XOR1>(x)); x = op(x, row_move<DPP_QUAD_XOR2>(x)); \
     x = op(x, row_move<DPP_ROW_HALF_MIRROR>(x)); x = op(x, row_move<DPP_ROW_MIRROR>(x))
+__device__ __forceinline__ int middle(int x, int y, int z) {
+    int r;
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
 __device__ __forceinline__ int add_int(int x, int y) { return x + y; }
 __device__ __forceinline__ int row_max(int x) { BM_ROW_ALL(x, max); return x; }
 __device__ __forceinline__ int row_min(int x) { BM_ROW_ALL(x, min); return x; }
@@ -514,7 +519,7 @@ __device__ __forceinline__ void row_rank(float score, float lo, float hi, int& r
 // order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
 template <class T, int VPL>
 __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, const float (&z)[VPL], const float (&bias)[VPL], float bmax,
-                                             float top, float by, int first, bool& fine) {
+                                             float top, float by, int first, bool shut, bool& fine) {
     const bool plain = a.bias == nullptr && a.ngroups == 1;
     int key[VPL];
     if (plain) {
@@ -525,12 +530,16 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
             key[j] = z[j] > -INFINITY ? k : kShut;
         }
     } else {
+        if (a.kind == 0) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            float p;
-            if (a.kind == 0) p = __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) * by;
-            else p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[j] * kLog2e));
-            key[j] = z[j] > -INFINITY ? __float_as_int(p + bias[j]) : kShut;
+            for (int j = 0; j < VPL; ++j) key[j] = __float_as_int(__builtin_amdgcn_exp2f((z[j] - top) * kLog2e) * by + bias[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) key[j] = __float_as_int(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[j] * kLog2e)) + bias[j]);
+        }
+        if (shut) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) key[j] = z[j] > -INFINITY ? key[j] : kShut;
         }
     }
     // Error of a key: p is off by up to 2^-16 of itself (exp of an argument of up to 88, the sum; by is the largest p of a
@@ -539,7 +548,7 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     int best = key[0], second = kShut;
 #pragma unroll
     for (int j = 1; j < VPL; ++j) {
-        second = max(second, min(best, key[j]));
+        second = middle(second, best, key[j]);
         best = max(best, key[j]);
     }
     fine = true;
@@ -575,20 +584,25 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     int lo, hi = row_max(best), n;
     hi = hi == kShut ? kShut + 2 : hi + 1;
     {
-        int least = INT_MAX;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) least = min(least, key[j] == kShut ? INT_MAX : key[j]);
-        least = row_min(least);
         const int two[2] = {best, second};
-        int first_lo = row_min(second == kShut ? (best == kShut ? INT_MAX : best) : second), first_hi = hi;
-        int c = row_count(two, first_lo);
-        const bool enough = c >= want;
-        while (__ballot(enough && c != want && (unsigned)first_hi - (unsigned)first_lo > 1u) != 0) {
-            const int mid = first_lo + (int)(((unsigned)first_hi - (unsigned)first_lo) >> 1);
+        int end = hi;
+        lo = row_min(second == kShut ? (best == kShut ? INT_MAX : best) : second);
+        n = row_count(two, lo);
+        const bool enough = n >= want;
+        while (__ballot(enough && n != want && (unsigned)end - (unsigned)lo > 1u) != 0) {
+            const int mid = lo + (int)(((unsigned)end - (unsigned)lo) >> 1);
             const int m = row_count(two, mid);
-            if (m >= want) { first_lo = mid; c = m; } else first_hi = mid;
+            if (enough) {
+                if (m >= want) { lo = mid; n = m; } else end = mid;
+            }
         }
-        lo = enough ? first_lo : least;
+        if (__ballot(!enough) != 0) {
+            int least = INT_MAX;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) least = min(least, key[j] == kShut ? INT_MAX : key[j]);
+            least = row_min(least);
+            lo = enough ? lo : least;
+        }
         n = row_count(key, lo);
     }
     while (__ballot(n > want) != 0) {
@@ -610,19 +624,13 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     if (n > 0) lo += (int)row_least_from(key, lo);      // the border is a key: the smallest taken one
     unsigned taken = 0;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) taken |= key[j] != kShut && key[j] >= lo ? 1u << j : 0u;
+    for (int j = VPL - 1; j >= 0; --j) taken = taken + taken + (unsigned)(key[j] >= lo);      // lo is above kShut, INT_MAX without open keys
     const int have = row_sum(__popc(taken));
-    if (have > want) fine = false;
-    if (!(plain && sizeof(T) == 2)) {
-        // a border with open keys below it: exactly `want` above it, by more than their errors
-        const float t = plain ? 0.f : __int_as_float(lo);
-        const float e = 2.f * fminf(most, 0x1p-15f * t);
-        int open = 0;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) open += key[j] != kShut;
-        open = row_sum(open);
-        const int reach = plain ? have : row_count(key, max(kShut + 1, __float_as_int(t - e)));
-        if (open > want && (have != want || reach != want)) fine = false;
+    if (have != n) fine = false;                 // equal keys at the border
+    if (!plain) {
+        // no other key within the errors of two keys below the smallest taken one
+        const float t = __int_as_float(lo), e = 2.f * fminf(most, 0x1p-15f * t);
+        if (row_count(key, max(kShut + 1, __float_as_int(t - e))) != have) fine = false;
     }
     return taken;
 }
@@ -654,7 +662,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
 #pragma unroll
     for (int j = 0; j < VPL; ++j) bias[j] += bmax;
     const bool sums = a.kind == 0 && (a.bias != nullptr || a.ngroups > 1 || !a.renorm);
-    const int odd_class = a.kind == 0 ? 0x203 : 0x003;
+    const bool full = __ballot(own != VPL) == 0;      // every lane has VPL experts
     const long long end = (a.ncols - 1LL) * a.ldz + a.nexperts;
     const long long step = (long long)gridDim.x * WAVES * d.batch;
     for (long long c0 = ((long long)blockIdx.x * WAVES + wave) * d.batch; c0 < a.ncols; c0 += step) {
@@ -664,7 +672,12 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
             const long long c = c0 + (b < cols ? b : cols - 1);      // rows past the end repeat the last column
             const long long at = c * a.ldz + first;
             float z[VPL];
-            if (VPL >= 2 && at + VPL <= end) {
+            if (VPL >= 2 && full) {
+                T raw[VPL];
+                __builtin_memcpy(raw, (const T*)a.Z + at, sizeof(raw));
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) z[j] = (float)raw[j];
+            } else if (VPL >= 2 && at + VPL <= end) {          // wide loads may run into the next column, not out of the matrix
                 T raw[VPL];
                 __builtin_memcpy(raw, (const T*)a.Z + at, sizeof(raw));
 #pragma unroll
@@ -673,24 +686,29 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) z[j] = j < own ? (float)((const T*)a.Z)[at + j] : -INFINITY;
             }
-            int odd = 0;
+            // a NaN anywhere, or +inf where the softmax has no value
+            unsigned size = 0;
+            float high = z[0], low = z[0];
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) odd |= __builtin_amdgcn_classf(z[j], odd_class);
-            const bool bad = row_sum(odd) != 0;
+            for (int j = 0; j < VPL; ++j) {
+                size = max(size, (unsigned)__float_as_int(z[j]) & 0x7fffffffu);
+                low = fminf(low, z[j]);
+                high = fmaxf(high, z[j]);
+            }
+            const bool bad = row_sum(size > 0x7f800000u || (a.kind == 0 && high == INFINITY)) != 0;
+            const bool shut = __ballot(low == -INFINITY) != 0;
             float top = 0.f, by = 1.f;
             if (sums) {
-                top = z[0];
-#pragma unroll
-                for (int j = 1; j < VPL; ++j) top = fmaxf(top, z[j]);
-                top = group_allmax<16>(top);
+                top = group_allmax<16>(high);
+                const float from = top > -INFINITY ? top : 0.f;
                 float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < VPL; ++j) sum += z[j] > -INFINITY ? __builtin_amdgcn_exp2f((z[j] - top) * kLog2e) : 0.f;
+                for (int j = 0; j < VPL; ++j) sum += __builtin_amdgcn_exp2f((z[j] - from) * kLog2e);
                 sum = group_allsum<16>(sum);
                 by = sum > 0.f ? 1.f / sum : 0.f;
             }
             bool fine;
-            unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, fine);
+            unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, shut, fine);
             if (bad) { taken = 0; fine = true; }
             // fewer than topk open: the lowest others fill the column
             const unsigned valid = taken;
@@ -781,6 +799,7 @@ __global__ __launch_bounds__(1024) void k_add_counts(int n, int nshares, const i
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, e = blockIdx.x * 16 + x;
     int c = 0;
     if (e < n)
+#pragma unroll 8
         for (int p = y; p < nshares; p += 64) c += shares[(size_t)p * n + e];
     sh[y][x] = c;
     for (int step = 32; step > 0; step >>= 1) {
