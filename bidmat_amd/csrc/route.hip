@@ -751,44 +751,68 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
 //   softmax, renormalised    dz_i = w_i * (dg_i - mean / scale)                taken entries, 0 elsewhere
 //   sigmoid                  dz_i = w_i * (1 - p_i) * dg_i                     likewise
 //   sigmoid, renormalised    dz_i = w_i * (1 - p_i) * (dg_i - mean / scale)    likewise
-// One wave per column: it writes the column (the softmax form from its scores), then its own entries over it.
-template <class T>
+// LPC lanes share a column, eight experts to a lane and turn. The entries' values meet the experts in LDS, so that the
+// column is written once.
+template <class T, int LPC, int NV>
 __global__ __launch_bounds__(BM_BLOCK) void k_route_grad(RouteGradArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long long c = (long long)blockIdx.x * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6);
+    constexpr int CPW = 64 / LPC;
+    __shared__ float at_expert[BM_BLOCK / LPC][LPC * NV * 8];
+    const int lane = threadIdx.x & 63, t = lane & (LPC - 1);
+    const long long c = ((long long)blockIdx.x * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6)) * CPW + lane / LPC;
     if (c >= a.ncols) return;
+    float* up = at_expert[threadIdx.x / LPC];
     const T* z = (const T*)a.Z + c * a.ldz;
-    T* dz = (T*)a.dZ + c * a.lddz;
-    const bool mine = lane < a.topk;
-    const long long q = c * a.topk + lane;
-    const int r = mine ? a.ir[q] : -1;
-    const bool ok = mine && (unsigned)r < (unsigned)a.nexperts;
-    const float w = ok ? a.data[q] : 0.f, dg = ok ? a.ddata[q] : 0.f;
-    const float mean = group_allsum<64>(w == 0.f ? 0.f : w * dg);
+    const int n = a.nexperts;
     const bool dense = a.kind == 0 && !a.renorm;
-    float top = -INFINITY, sum = 0.f, zr = 0.f;
-    if (ok && (dense || a.kind == 1)) zr = (float)z[r];
-    if (dense) {
-        for (int i = lane; i < a.nexperts; i += 64) top = fmaxf(top, (float)z[i]);
-        top = group_allmax<64>(top);
-        if (top == -INFINITY) top = 0.f;
-        for (int i = lane; i < a.nexperts; i += 64) sum += expf((float)z[i] - top);
-        sum = group_allsum<64>(sum);
+    const long long q0 = c * a.topk;
+    float mean = 0.f;
+    for (int s = t; s < a.topk; s += LPC) {
+        const float w = (unsigned)a.ir[q0 + s] < (unsigned)n ? a.data[q0 + s] : 0.f;
+        if (w != 0.f) mean += w * a.ddata[q0 + s];
     }
-    const float by = sum == 0.f ? 0.f : 1.f / sum;      // a column without open experts; a NaN stays one
-    for (int i = lane; i < a.nexperts; i += 64) dz[i] = (T)(dense ? -(expf((float)z[i] - top) * by) * mean : 0.f);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    if (ok) {
-        float d = 0.f;
-        if (w != 0.f) {
-            if (dense) d = expf(zr - top) * by * (a.scale * dg - mean);
-            else d = w * (a.renorm ? dg - mean / a.scale : dg) * (a.kind == 1 ? 1.f / (1.f + expf(zr)) : 1.f);
-        } else if (dense) {
-            d = -(expf(zr - top) * by) * mean;
+    mean = group_allsum<LPC>(mean);
+    float8_t x[NV];
+    float by = 0.f, top = -INFINITY;
+    if (dense) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            x[v] = load_col8(z, (v * LPC + t) * 8, n, (T)(-INFINITY)).wide();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, x[v][j]);
         }
-        dz[r] = (T)d;
+        top = group_allmax<LPC>(top);
+        if (top == -INFINITY) top = 0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[v][j] = __builtin_amdgcn_exp2f((x[v][j] - top) * kLog2e);
+                sum += x[v][j];
+            }
+        sum = group_allsum<LPC>(sum);
+        by = sum == 0.f ? 0.f : 1.f / sum;              // a column without open experts; a NaN stays one
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) *(float8_t*)(up + (v * LPC + t) * 8) = (float8_t)(0.f);
+    __builtin_amdgcn_wave_barrier();                    // a wave's LDS operations take effect in order
+    for (int s = t; s < a.topk; s += LPC) {
+        const int r = a.ir[q0 + s];
+        if ((unsigned)r >= (unsigned)n) continue;
+        const float w = a.data[q0 + s], dg = a.ddata[q0 + s];
+        if (w == 0.f) continue;
+        float d = dense ? a.scale * dg : w * (a.renorm ? dg - mean / a.scale : dg);
+        if (a.kind == 1) d *= 1.f / (1.f + expf((float)z[r]));
+        if (w != w) d = w;
+        up[r] = d;
+    }
+    __builtin_amdgcn_wave_barrier();
+    T* dz = (T*)a.dZ + c * a.lddz;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        float8_t d = *(const float8_t*)(up + (v * LPC + t) * 8);
+        if (dense) d = x[v] * by * (d - mean);
+        store_col8(dz, (v * LPC + t) * 8, n, d);
     }
 }
 
@@ -893,12 +917,25 @@ hipError_t route(const RouteArgs& a, hipStream_t s) {
     return a.type == ELEM_F32 ? route_typed<float>(a, s) : a.type == ELEM_F16 ? route_typed<f16_t>(a, s) : route_typed<bf16_t>(a, s);
 }
 
-hipError_t route_grad(const RouteGradArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)((a.ncols + BM_WAVES_PER_BLOCK - 1LL) / BM_WAVES_PER_BLOCK)), block(BM_BLOCK);
-    if (a.type == ELEM_F32) hipLaunchKernelGGL((k_route_grad<float>), grid, block, 0, s, a);
-    else if (a.type == ELEM_F16) hipLaunchKernelGGL((k_route_grad<f16_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_route_grad<bf16_t>), grid, block, 0, s, a);
+namespace {
+template <class T, int LPC, int NV>
+hipError_t launch_route_grad(const RouteGradArgs& a, hipStream_t s) {
+    constexpr int CPB = BM_BLOCK / LPC;
+    hipLaunchKernelGGL((k_route_grad<T, LPC, NV>), dim3((unsigned)((a.ncols + CPB - 1LL) / CPB)), dim3(BM_BLOCK), 0, s, a);
     return hipGetLastError();
+}
+template <class T>
+hipError_t route_grad_typed(const RouteGradArgs& a, hipStream_t s) {
+    if (a.nexperts <= 64) return launch_route_grad<T, 8, 1>(a, s);
+    if (a.nexperts <= 128) return launch_route_grad<T, 16, 1>(a, s);
+    if (a.nexperts <= 256) return launch_route_grad<T, 32, 1>(a, s);
+    if (a.nexperts <= 512) return launch_route_grad<T, 64, 1>(a, s);
+    return launch_route_grad<T, 64, 2>(a, s);
+}
+}  // namespace
+
+hipError_t route_grad(const RouteGradArgs& a, hipStream_t s) {
+    return a.type == ELEM_F32 ? route_grad_typed<float>(a, s) : a.type == ELEM_F16 ? route_grad_typed<f16_t>(a, s) : route_grad_typed<bf16_t>(a, s);
 }
 
 }  // namespace bm
