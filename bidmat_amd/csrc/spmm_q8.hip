@@ -49,6 +49,35 @@ __device__ __forceinline__ void fma_codes(float (&acc)[16], uint4 x, float by) {
     }
 }
 
+// Nonzeros it0 .. it0 + U - 1 of every group (slot it * NG + g of the wave's chunk of 64, held one per lane): U gathers in
+// flight per lane before their sums are taken. FULL: all of them exist.
+template <int LPN, int U, bool FULL>
+__device__ __forceinline__ void gather_codes(const Q8Args& a, int row, float val, int rem, int it0, int g, int i, int left, int sg, float (&acc)[16]) {
+    constexpr int NG = 64 / LPN;
+    uint4 x[U];
+    float by[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int src = (it0 + u) * NG + g;
+        long long r;
+        if constexpr (LPN == 64) {
+            r = __builtin_amdgcn_readlane(row, it0 + u);
+            v[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(val), it0 + u));
+        } else {
+            r = lane_read(row, src);
+            v[u] = lane_read(val, src);
+        }
+        by[u] = 0.f;
+        x[u] = make_uint4(0, 0, 0, 0);
+        if (left > 0 && (FULL || src < rem)) {
+            x[u] = load_codes(a.Q + r * a.ldq + i, left);
+            by[u] = a.scales[r * a.nscales + sg];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) fma_codes(acc, x[u], FULL || (it0 + u) * NG + g < rem ? v[u] * by[u] : 0.f);
+}
+
 template <int LPN>
 __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     constexpr int NG = 64 / LPN;
@@ -79,24 +108,44 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     }
     for (int k0 = 0; k0 < a.k; k0 += 16 * LPN) {
         const int i = k0 + 16 * l, left = a.k - i;
-        const int sg = a.shift < 31 ? i >> a.shift : 0;
+        const int sg = a.shift < 31 && left > 0 ? i >> a.shift : 0;
         float acc[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-        if (left > 0)
-            for (int j = lo + g; j < hi; j += NG) {
-                const long long r = a.ir[j];
-                const float by = a.vals[j] * a.scales[r * a.nscales + sg];
-                fma_codes(acc, load_codes(a.Q + r * a.ldq + i, left), by);
+        constexpr int U = LPN < 8 ? LPN : 8;
+        for (int j0 = lo; j0 < hi; j0 += 64) {
+            const int rem = hi - j0 < 64 ? hi - j0 : 64;
+            int row = 0;
+            float val = 0.f;
+            if (lane < rem) {
+                row = a.ir[j0 + lane];
+                val = a.vals[j0 + lane];
             }
+            const int turns = (rem + NG - 1) / NG;         // per group
+            int it = 0;
+            for (; (it + U) * NG <= rem; it += U) gather_codes<LPN, U, true>(a, row, val, rem, it, g, i, left, sg, acc);
+            for (; it < turns; it += (U > 4 ? 4 : U)) gather_codes<LPN, (U > 4 ? 4 : U), false>(a, row, val, rem, it, g, i, left, sg, acc);
+        }
 #pragma unroll
         for (int m = LPN; m < 64; m <<= 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[j] += __shfl_xor(acc[j], m, 64);
-        if (g == 0)
+        if (g == 0) {
+            if (left >= 16) {
+                float4 o[4];
+                if (add) __builtin_memcpy(o, out + i, 64);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < left) out[i + j] = add ? out[i + j] + acc[j] : acc[j];
+                for (int j = 0; j < 4; ++j) {
+                    const float4 s = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+                    o[j] = add ? make_float4(o[j].x + s.x, o[j].y + s.y, o[j].z + s.z, o[j].w + s.w) : s;
+                }
+                __builtin_memcpy(out + i, o, 64);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < left) out[i + j] = add ? out[i + j] + acc[j] : acc[j];
+            }
+        }
     }
 }
 
