@@ -73,8 +73,6 @@ hipError_t build_overflow_table(int ncols, int nnz, const int* jc, int seglen, i
 size_t overflow_table_ints(int ncols);
 hipError_t build_overflow_table_in(int ncols, int nnz, const int* jc, int seglen, int* buf, int** d_ovf,
                                    hipStream_t s);
-// C[:,c] += the partial sums of column c's overflow segments, in segment order (C is k x ncols)
-hipError_t overflow_reduce(int k, int ncols, const int* ovf, const float* partial, float* C, hipStream_t s);
 // A column overflow table that the caller already holds (a plan builds it once per pattern):
 // seglen it was built with, table (ncols+1 ints; unused when novf == 0), number of overflow
 // segments. (A*S keeps the novf*k partial sums of those segments in the stream's scratch.)

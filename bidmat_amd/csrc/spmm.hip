@@ -814,12 +814,6 @@ hipError_t dsmult_csc_ex(int k, int lda, int ldc, int ncols, int nnz, const floa
     return err;
 }
 
-hipError_t overflow_reduce(int k, int ncols, const int* ovf, const float* partial, float* C, hipStream_t s) {
-    const unsigned nblk = (unsigned)(((long long)ncols + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK);
-    hipLaunchKernelGGL(k_overflow_reduce, dim3(nblk), dim3(BM_BLOCK), 0, s, k, k, ncols, ovf, partial, C);
-    return hipGetLastError();
-}
-
 // A*S over a class-ordered pattern in `nphase` passes, one launch each: pass p only gathers the rows
 // of classes [8*p/nphase, 8*(p+1)/nphase), and the passes follow each other on the stream. While
 // a pass runs, every L2 of the device only sees that pass's share of the rows, so it holds

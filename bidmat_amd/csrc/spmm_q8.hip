@@ -1,9 +1,16 @@
 // C = beta*C + A*S with A in 8 bits (e4m3) and fp32 scales: A[i, r] = scales[i / group, r] * q[i, r].
 //
-// The gathers of A's columns bound A*S; codes are a quarter of the fp32 bytes. One wavefront owns a column of S, like in
-// the fp32 product (spmm.hip), with its rule for long columns: a column longer than "seglen" nonzeros is cut, extra waves
-// take the other segments and leave partial sums that are added in order. Sums are fp32.
+// The gathers of A's columns bound A*S; codes are a quarter of the fp32 bytes. One wavefront owns a column of S. A column
+// longer than a segment (a quarter of "seglen" nonzeros: with a quarter of the bytes per nonzero, a wave that walks more
+// of them alone is still running when the others are done) is cut at the multiples of the segment length in the array of
+// nonzeros: its own wave goes up to the first of them, the wave of every multiple inside it takes the segment that begins
+// there, found by a search in jc, and leaves a partial sum; these are added in order. Sums are fp32.
 // LPN lanes cover 16 * LPN rows with one 16-byte load each; a wave works on 64 / LPN nonzeros at a time.
+//
+// What bounds it: lines of A that miss L2, which the fabric passes at 7.0 to 7.7 TB/s whatever lies behind it. k = 1024,
+// 200000 columns of A, 2 M nonzeros in 50000 columns of 40: 350 us, 5.8 TB/s of gathers and 0.6 TB/s of C (one gather at a
+// time 746 us; four in flight per lane as good as eight or sixteen, which cost occupancy where k is small: 140 us instead
+// of 175 at k = 100).
 #include "columns.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -13,25 +20,37 @@ namespace bm {
 namespace {
 
 struct Q8Args {
-    int k, ncols, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
+    int k, ncols, nnz, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
+    int nsegs;                                            // waves in front of the columns', one per multiple of seglen
     long long ldq;
     const unsigned char* Q;
     const float *scales, *vals;
-    const int *ir, *jc, *ovf;
+    const int *ir, *jc;
     float *C, *partial;
 };
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ uint4 load_codes(const unsigned char* p, int left) {
+// Rows i .. i+15 of a column of k codes, those past its end as zeros. A short last part is loaded as the column's last 16
+// codes and shifted down.
+__device__ __forceinline__ uint4 load_codes(const unsigned char* col, int i, int k) {
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (left >= 16) {
-        __builtin_memcpy(&x, p, 16);
+    if ((k & 15) == 0) {
+        __builtin_memcpy(&x, col + i, 16);
+    } else if (k >= 16) {
+        const int s = i + 16 - k > 0 ? i + 16 - k : 0;          // codes in front of row i
+        __builtin_memcpy(&x, col + i - s, 16);
+        if (s & 8) x = make_uint4(x.z, x.w, 0, 0);
+        if (s & 4) x = make_uint4(x.y, x.z, x.w, 0);
+        x.x = __builtin_amdgcn_alignbyte(x.y, x.x, s & 3);
+        x.y = __builtin_amdgcn_alignbyte(x.z, x.y, s & 3);
+        x.z = __builtin_amdgcn_alignbyte(x.w, x.z, s & 3);
+        x.w = __builtin_amdgcn_alignbyte(0u, x.w, s & 3);
     } else {
         unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < left) w[j >> 2] |= (unsigned)p[j] << (8 * (j & 3));
+        for (int j = 0; j < 15; ++j)
+            if (i + j < k) w[j >> 2] |= (unsigned)col[i + j] << (8 * (j & 3));
         x = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return x;
@@ -70,13 +89,17 @@ __device__ __forceinline__ void gather_codes(const Q8Args& a, int row, float val
         by[u] = 0.f;
         x[u] = make_uint4(0, 0, 0, 0);
         if (left > 0 && (FULL || src < rem)) {
-            x[u] = load_codes(a.Q + r * a.ldq + i, left);
+            x[u] = load_codes(a.Q + r * a.ldq, i, a.k);
             by[u] = a.scales[r * a.nscales + sg];
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) fma_codes(acc, x[u], FULL || (it0 + u) * NG + g < rem ? v[u] * by[u] : 0.f);
 }
+
+// Segments begin at the multiples of seglen counted from the first nonzero, jc[0] (a range of columns may be passed with the
+// whole matrix's arrays). The first one that begins at or after position x:
+__device__ __forceinline__ int segment_from(const Q8Args& a, int x) { return (int)(((long long)x - a.jc[0] + a.seglen - 1) / a.seglen); }
 
 template <int LPN>
 __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
@@ -86,25 +109,27 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     int lo, hi;
     float* out;
     bool add = false;
-    if (w < a.ncols) {
-        lo = a.jc[w];
-        hi = a.jc[w + 1];
-        if (hi - lo > a.seglen) hi = lo + a.seglen;
-        out = a.C + w * a.k;
+    if (w >= a.nsegs) {
+        const long long c = w - a.nsegs;
+        if (c >= a.ncols) return;
+        lo = a.jc[c];
+        hi = a.jc[c + 1];
+        if (hi - lo > a.seglen) hi = a.jc[0] + segment_from(a, lo) * a.seglen;
+        out = a.C + c * a.k;
         add = a.beta != 0;
     } else {
-        if (a.ovf == nullptr) return;
-        const long long x = w - a.ncols;
-        if (x >= a.ovf[a.ncols]) return;
-        int c0 = 0, c1 = a.ncols;                    // ovf[c0] <= x < ovf[c1]
+        const long long from = a.jc[0] + w * a.seglen;
+        if (from >= a.jc[a.ncols]) return;
+        lo = (int)from;
+        int c0 = 0, c1 = a.ncols;                    // jc[c0] <= lo < jc[c1]
         while (c1 - c0 > 1) {
             const int mid = (int)(((long long)c0 + c1) >> 1);
-            if (a.ovf[mid] <= x) c0 = mid; else c1 = mid;
+            if (a.jc[mid] <= lo) c0 = mid; else c1 = mid;
         }
-        const long long from = (long long)a.jc[c0] + (x - a.ovf[c0] + 1) * a.seglen, end = a.jc[c0 + 1];
-        lo = (int)from;
-        hi = (int)(end < from + a.seglen ? end : from + a.seglen);
-        out = a.partial + x * a.k;
+        const int end = a.jc[c1];
+        if (end - a.jc[c0] <= a.seglen) return;      // its column's own wave takes all of it
+        hi = end - lo > a.seglen ? lo + a.seglen : end;
+        out = a.partial + w * a.k;
     }
     for (int k0 = 0; k0 < a.k; k0 += 16 * LPN) {
         const int i = k0 + 16 * l, left = a.k - i;
@@ -112,7 +137,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
         float acc[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-        constexpr int U = LPN < 8 ? LPN : 8;
+        constexpr int U = LPN < 4 ? LPN : 4;
         for (int j0 = lo; j0 < hi; j0 += 64) {
             const int rem = hi - j0 < 64 ? hi - j0 : 64;
             int row = 0;
@@ -124,7 +149,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
             const int turns = (rem + NG - 1) / NG;         // per group
             int it = 0;
             for (; (it + U) * NG <= rem; it += U) gather_codes<LPN, U, true>(a, row, val, rem, it, g, i, left, sg, acc);
-            for (; it < turns; it += (U > 4 ? 4 : U)) gather_codes<LPN, (U > 4 ? 4 : U), false>(a, row, val, rem, it, g, i, left, sg, acc);
+            for (; it < turns; it += U) gather_codes<LPN, U, false>(a, row, val, rem, it, g, i, left, sg, acc);
         }
 #pragma unroll
         for (int m = LPN; m < 64; m <<= 1)
@@ -149,6 +174,27 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     }
 }
 
+// C[:,c] += the partial sums of column c's segments, in order. A workgroup looks at kLook columns and adds those that were
+// cut with all of its threads.
+constexpr int kLook = 16;
+__global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
+    const int lane = threadIdx.x & 63;
+    const long long first = (long long)blockIdx.x * kLook;
+    bool long_ = false;
+    if (lane < kLook && first + lane < a.ncols) long_ = a.jc[first + lane + 1] - a.jc[first + lane] > a.seglen;
+    for (unsigned long long cut = __ballot(long_); cut != 0; cut &= cut - 1) {
+        const long long c = first + __builtin_ctzll(cut);
+        const int s0 = segment_from(a, a.jc[c]);
+        const int s1 = min(segment_from(a, a.jc[c + 1]), a.nsegs);
+        for (int el = threadIdx.x; el < a.k; el += BM_BLOCK) {
+            float acc = a.C[c * a.k + el];
+#pragma unroll 8
+            for (int s = s0; s < s1; ++s) acc += a.partial[(long long)s * a.k + el];
+            a.C[c * a.k + el] = acc;
+        }
+    }
+}
+
 template <int LPN>
 hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
     hipLaunchKernelGGL((k_dsmult_q8<LPN>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK)), dim3(BM_BLOCK), 0, s, a);
@@ -160,22 +206,20 @@ hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
 hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long long ldq, const float* scales, int group,
                          const float* vals, const int* ir, const int* jc, float* C, int beta, hipStream_t s) {
     Q8Args a;
-    a.k = k; a.ncols = ncols; a.seglen = opt_seglen(); a.beta = beta;
+    a.k = k; a.ncols = ncols; a.nnz = nnz; a.beta = beta;
+    a.seglen = opt_seglen() / 4;
     a.nscales = group == 0 ? 1 : (k + group - 1) / group;
     a.shift = group == 0 ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7;
     a.ldq = ldq; a.Q = Q; a.scales = scales; a.vals = vals; a.ir = ir; a.jc = jc; a.C = C;
-    a.ovf = nullptr; a.partial = nullptr;
-    int* ovf = nullptr;
-    hipError_t err = build_overflow_table(ncols, nnz, jc, a.seglen, &ovf, s);
-    if (err != hipSuccess) return err;
-    long long extra = 0;
-    if (ovf != nullptr) {
-        extra = nnz / a.seglen;
-        a.ovf = ovf;
-        a.partial = (float*)ws_get(WS_PARTIAL, sizeof(float) * (size_t)extra * (size_t)k, &err, s);
+    a.partial = nullptr;
+    a.nsegs = 0;
+    hipError_t err;
+    if (nnz > a.seglen) {
+        a.nsegs = (nnz + a.seglen - 1) / a.seglen;
+        a.partial = (float*)ws_get(WS_PARTIAL, sizeof(float) * (size_t)a.nsegs * (size_t)k, &err, s);
         if (!a.partial) return err;
     }
-    const long long nwaves = (long long)ncols + extra;
+    const long long nwaves = (long long)ncols + a.nsegs;
     const int lanes = pow2ceil((k + 15) / 16);
     if (lanes <= 1) err = launch_q8<1>(a, nwaves, s);
     else if (lanes <= 2) err = launch_q8<2>(a, nwaves, s);
@@ -184,7 +228,10 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     else if (lanes <= 16) err = launch_q8<16>(a, nwaves, s);
     else if (lanes <= 32) err = launch_q8<32>(a, nwaves, s);
     else err = launch_q8<64>(a, nwaves, s);
-    if (err == hipSuccess && ovf != nullptr) err = overflow_reduce(k, ncols, ovf, a.partial, C, s);
+    if (err == hipSuccess && a.nsegs > 0) {
+        hipLaunchKernelGGL(k_add_segments, dim3((unsigned)(((long long)ncols + kLook - 1) / kLook)), dim3(BM_BLOCK), 0, s, a);
+        err = hipGetLastError();
+    }
     return err;
 }
 
