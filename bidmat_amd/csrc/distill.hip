@@ -17,9 +17,11 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+constexpr int kColumnsMin = 64;
+
 // What a column's teacher entries come to. at0: the largest student logit x among them, subtracted before the sum so
 // that loss = tau^2 * weight * (part + mass * (lse - at0)) cancels nothing large.
-struct Teacher { float lse, part, mass, at0; };      // lse = -inf: no entries
+struct Teacher { float lse, part, mass, at0; int repeats; };      // lse = -inf: no entries; repeats: a row is stored twice
 
 // A running log-sum in base 2: sum of 2^(v - top).
 struct LogSum { float top, sum; };
@@ -54,6 +56,26 @@ __device__ __forceinline__ void column_entries(const DistillArgs& a, long long c
     hi = min(max(a.tjc[c + 1], lo), a.nnz);
 }
 __device__ __forceinline__ float column_scale(const DistillArgs& a, long long c) { return a.weight != nullptr ? a.weight[c] : 1.f; }
+
+// One wave: whether a row is stored twice among n. Ascending rows show that they are not in one pass; others are compared
+// in pairs, 64 at a time.
+__device__ int rows_repeat(const int* rows, int n) {
+    const int lane = threadIdx.x & 63;
+    bool ascend = true;
+    for (int j = lane; j + 1 < n; j += 64) ascend = ascend && rows[j] < rows[j + 1];
+    if (__ballot(!ascend) == 0) return 0;
+    unsigned long long met = 0;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int mine = j0 + lane < n ? rows[j0 + lane] : -1 - lane;
+        for (int q0 = j0; q0 < n; q0 += 64) {
+            const int other = q0 + lane < n ? rows[q0 + lane] : -1;
+            const int count = n - q0 < 64 ? n - q0 : 64;
+#pragma unroll 8
+            for (int q = 0; q < count; ++q) met |= __ballot(mine == __builtin_amdgcn_readlane(other, q) && (j0 != q0 || lane != q));
+        }
+    }
+    return met != 0;
+}
 
 // One wave: statistics of a column's teacher entries; at[] receives the student's x at each of them.
 template <class T>
@@ -99,6 +121,7 @@ __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, f
     r.part = group_allsum<64>(part);
     r.mass = group_allsum<64>(mass);
     r.at0 = xtop;
+    r.repeats = rows_repeat(a.tir + lo, hi - lo);
     return r;
 }
 
@@ -160,6 +183,17 @@ __global__ __launch_bounds__(BM_BLOCK) void k_distill_loss(DistillArgs a, int nc
     if ((threadIdx.x & 63) == 0) write_loss(a, c, natural_lse(x), stats[c]);
 }
 
+// The gradient at teacher entry j of [e0, e1), whose student logit was x, over its scale.
+__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& t, int e0, int e1, int j, int r, float x, float it, float from) {
+    float p = expf(a.tdata[j] * it - t.lse);
+    if (t.repeats) {
+        p = 0.f;
+        for (int q = e0; q < e1; ++q)
+            if (a.tir[q] == r) p += expf(a.tdata[q] * it - t.lse);
+    }
+    return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -from)) - p;
+}
+
 // The gradient of rows [lo, hi) of column c, once every student logit at a teacher entry has been saved in at[].
 template <class T>
 __device__ void grad_chunk(const DistillArgs& a, long long c, int lo, int hi, float it, float lse, const Teacher& t, const float* at) {
@@ -168,14 +202,26 @@ __device__ void grad_chunk(const DistillArgs& a, long long c, int lo, int hi, fl
     const float w = column_scale(a, c) * a.temperature;
     const bool none = t.lse == -INFINITY || w == 0.f;
     const float k = it * kLog2e, from = lse * kLog2e;
-    for (int i = lo + (int)threadIdx.x * 8; i < hi; i += (int)blockDim.x * 8) {
-        float8_t v = (float8_t)(0.f);
+    constexpr int U = 4;                    // loads in flight per thread
+    const int step = (int)blockDim.x * 8;
+    for (int i0 = lo + (int)threadIdx.x * 8; i0 < hi; i0 += U * step) {
+        Raw8<T> x[U];
         if (!none) {
-            const float8_t x = load_col8(z, i, hi).wide();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(x[j], k, -from));
+            for (int u = 0; u < U; ++u)
+                if (i0 + u * step < hi) x[u] = load_col8(z, i0 + u * step, hi);
         }
-        store_col8(dz, i, hi, v);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * step >= hi) break;
+            float8_t v = (float8_t)(0.f);
+            if (!none) {
+                const float8_t y = x[u].wide();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+            }
+            store_col8(dz, i0 + u * step, hi, v);
+        }
     }
     if (none) return;
     __syncthreads();          // the entries' values go over what other threads of the workgroup wrote
@@ -183,11 +229,7 @@ __device__ void grad_chunk(const DistillArgs& a, long long c, int lo, int hi, fl
     column_entries(a, c, e0, e1);
     for (int j = e0 + (int)threadIdx.x; j < e1; j += (int)blockDim.x) {
         const int r = a.tir[j];
-        if (r < lo || r >= hi) continue;
-        float p = 0.f;
-        for (int q = e0; q < e1; ++q)
-            if (a.tir[q] == r) p += expf(a.tdata[q] * it - t.lse);
-        dz[r] = (T)(w * (__builtin_amdgcn_exp2f(fmaf(at[j], kLog2e, -from)) - p));
+        if (r >= lo && r < hi) dz[r] = (T)(w * entry_grad(a, t, e0, e1, j, r, at[j], it, from));
     }
 }
 
@@ -209,18 +251,106 @@ __global__ __launch_bounds__(BM_BLOCK) void k_distill_grad(DistillArgs a, int nc
     grad_chunk<T>(a, c, lo, min(a.nrows, lo + chunk), 1.f / a.temperature, lse, t, at);
 }
 
+// A whole column in the registers of one workgroup of BLOCK threads, NV vectors of eight logits each: read once, written
+// once. The last wave takes the teacher's entries before its share of the column. Log-sums run along with the loads;
+// afterwards the logits are still there as they were read.
+// An entry's gradient goes over the one written for its row by the wave that wrote that one, whose stores take effect
+// in order: no barrier has to wait for the column's stores.
+template <class T, int BLOCK, int NV>
+__global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* at) {
+    constexpr int WAVES = BLOCK / 64;
+    __shared__ LogSum sh[WAVES];
+    __shared__ Teacher teacher;
+    const long long c = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = wave_uniform(t >> 6), n = a.nrows;
+    const float it = 1.f / a.temperature, k = it * kLog2e;
+    const T* z = (const T*)a.Z + c * a.ldz;
+    if (wave == WAVES - 1) {
+        const Teacher r = teacher_column<T>(a, c, it, at);
+        if (lane == 0) teacher = r;
+    }
+    Raw8<T> x[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v] = load_col8(z, (v * BLOCK + t) * 8, n, (T)(-INFINITY));
+    LogSum s = {-INFINITY, 0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const float8_t y = x[v].wide() * k;
+        float top = s.top;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
+        const float from = top == -INFINITY ? 0.f : top;
+        float sum = s.sum * __builtin_amdgcn_exp2f(s.top - from);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f(y[j] - from);
+        s = {top, sum};
+    }
+    const float lse = natural_lse(block_join(s, sh, WAVES));
+    const Teacher tc = teacher;
+    if (t == 0) write_loss(a, c, lse, tc);
+    if (a.dZ == nullptr) return;
+    T* dz = (T*)a.dZ + c * a.lddz;
+    const float w = column_scale(a, c) * a.temperature, from = lse * kLog2e;
+    const bool none = tc.lse == -INFINITY || w == 0.f;
+    int e0, e1;
+    column_entries(a, c, e0, e1);
+    const bool first = !none && e0 + lane < e1;
+    const int r0 = first ? a.tir[e0 + lane] : -1;
+    const float x0 = first ? at[e0 + lane] : 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        float8_t d = (float8_t)(0.f);
+        if (!none) {
+            const float8_t y = x[v].wide();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+        }
+        store_col8(dz, (v * BLOCK + t) * 8, n, d);
+    }
+    if (none) return;
+    for (int j = e0 + lane; j < e1; j += 64) {
+        const int r = j < e0 + 64 ? r0 : a.tir[j];
+        if ((unsigned)r >= (unsigned)n || ((r >> 3) & (BLOCK - 1)) >> 6 != wave) continue;
+        dz[r] = (T)(w * entry_grad(a, tc, e0, e1, j, r, j < e0 + 64 ? x0 : at[j], it, from));
+    }
+}
+
+template <class T, int BLOCK, int NV>
+hipError_t launch_column(const DistillArgs& a, float* at, hipStream_t s) {
+    hipLaunchKernelGGL((k_distill_column<T, BLOCK, NV>), dim3((unsigned)a.ncols), dim3(BLOCK), 0, s, a, at);
+    return hipGetLastError();
+}
+// Columns that fit the registers of a workgroup, where there are enough of them to fill the device.
+template <class T>
+bool by_column(const DistillArgs& a) {
+    return a.lse_in == nullptr && a.nrows <= (sizeof(T) == 2 ? 131072 : 65536) && a.ncols >= kColumnsMin;
+}
+template <class T>
+hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {
+    const int vecs = (a.nrows + 7) / 8;
+    if (vecs <= 256) return launch_column<T, 256, 1>(a, at, s);
+    if (vecs <= 512) return launch_column<T, 256, 2>(a, at, s);
+    if (vecs <= 1024) return launch_column<T, 256, 4>(a, at, s);
+    if (vecs <= 2048) return launch_column<T, 512, 4>(a, at, s);
+    if (vecs <= 4096) return launch_column<T, 1024, 4>(a, at, s);
+    if (vecs <= 8192) return launch_column<T, 1024, 8>(a, at, s);
+    if constexpr (sizeof(T) == 2) return launch_column<T, 1024, 16>(a, at, s);
+    return hipErrorInvalidValue;
+}
+
 template <class T>
 hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
+    hipError_t err;
+    float* at = (float*)ws_get(WS_DISTILL_AT, sizeof(float) * (size_t)a.nnz, &err, s);
+    if (!at) return err;
+    if (by_column<T>(a)) return distill_columns<T>(a, at, s);
     // a chunk is a multiple of what a workgroup takes at once; smaller ones where there are few columns
     int chunk = 4 * BM_BLOCK * 8;
     while (chunk > BM_BLOCK * 8 && (long long)a.ncols * ((a.nrows + chunk - 1) / chunk) < 1024) chunk >>= 1;
     const int nchunks = (a.nrows + chunk - 1) / chunk;
     const long long nparts = (long long)nchunks * a.ncols;
-    hipError_t err;
     char* buf = (char*)ws_get(WS_DISTILL, sizeof(Teacher) * (size_t)a.ncols + sizeof(LogSum) * (size_t)nparts, &err, s);
     if (!buf) return err;
-    float* at = (float*)ws_get(WS_DISTILL_AT, sizeof(float) * (size_t)a.nnz, &err, s);
-    if (!at) return err;
     Teacher* stats = (Teacher*)buf;
     LogSum* parts = (LogSum*)(buf + sizeof(Teacher) * (size_t)a.ncols);
     const int waves = (a.ncols + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK;
