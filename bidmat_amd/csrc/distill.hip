@@ -18,6 +18,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 constexpr int kColumnsMin = 64;
+constexpr int kRowsKept = 512;         // teacher rows of a column that a workgroup keeps in LDS
 
 // What a column's teacher entries come to. at0: the largest student logit x among them, subtracted before the sum so
 // that loss = tau^2 * weight * (part + mass * (lse - at0)) cancels nothing large.
@@ -70,7 +71,6 @@ __device__ int rows_repeat(const int* rows, int n) {
         for (int q0 = j0; q0 < n; q0 += 64) {
             const int other = q0 + lane < n ? rows[q0 + lane] : -1;
             const int count = n - q0 < 64 ? n - q0 : 64;
-#pragma unroll 8
             for (int q = 0; q < count; ++q) met |= __ballot(mine == __builtin_amdgcn_readlane(other, q) && (j0 != q0 || lane != q));
         }
     }
@@ -194,61 +194,102 @@ __device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher&
     return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -from)) - p;
 }
 
-// The gradient of rows [lo, hi) of column c, once every student logit at a teacher entry has been saved in at[].
-template <class T>
-__device__ void grad_chunk(const DistillArgs& a, long long c, int lo, int hi, float it, float lse, const Teacher& t, const float* at) {
+// The gradient of rows [lo, hi) of column c. ALONE: nothing was prepared and dZ is not Z: the log-sum is an earlier call's, and
+// a fifth wave takes the teacher's entries while the others are at the column. Otherwise stats and at[] hold the
+// teacher's statistics and the student's logits at its entries, parts the log-sums of the column's chunks (or lse_in).
+template <class T, bool ALONE>
+__global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_grad(DistillArgs a, int nchunks, int chunk, const LogSum* parts, const Teacher* stats,
+                                                           const float* at) {
+    __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
+    __shared__ Teacher own;
+    __shared__ int rows[ALONE ? kRowsKept : 1];
+    constexpr int U = 4, STEP = BM_BLOCK * 8;            // loads in flight per thread
+    const long long c = blockIdx.x / nchunks;
+    const int b = (int)(blockIdx.x % nchunks), lo = b * chunk, hi = min(a.nrows, lo + chunk);
     const T* z = (const T*)a.Z + c * a.ldz;
     T* dz = (T*)a.dZ + c * a.lddz;
+    int e0, e1;
+    column_entries(a, c, e0, e1);
     const float w = column_scale(a, c) * a.temperature;
-    const bool none = t.lse == -INFINITY || w == 0.f;
+    bool none = e0 == e1 || w == 0.f;
+    const bool extra = ALONE && threadIdx.x >= BM_BLOCK;
+    const int i0 = extra ? hi : lo + (int)threadIdx.x * 8;
+    Raw8<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (!none && i0 + u * STEP < hi) x[u] = load_col8(z, i0 + u * STEP, hi);
+    const float it = 1.f / a.temperature;
+    float lse;
+    Teacher t;
+    if constexpr (ALONE) {
+        lse = a.lse_in[c];
+        if (extra && !none) {
+            const int lane = threadIdx.x & 63;
+            float top = -INFINITY, sum = 0.f;
+            bool any = false;
+            for (int j = e0 + lane; j < e1; j += 64)
+                if ((unsigned)a.tir[j] < (unsigned)a.nrows) top = fmaxf(top, a.tdata[j] * it);
+            top = group_allmax<64>(top);
+            for (int j = e0 + lane; j < e1; j += 64)
+                if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
+                    const float v = a.tdata[j] * it;
+                    any = any || !(v == -INFINITY);
+                    sum += v == -INFINITY ? 0.f : expf(v - top);
+                }
+            sum = group_allsum<64>(sum);
+            t.lse = __ballot(any) != 0 ? top + logf(sum) : -INFINITY;
+            for (int j = lane; j < kRowsKept && e0 + j < e1; j += 64) rows[j] = a.tir[e0 + j];
+            if (lane == 0) own = t;
+        }
+    } else {
+        t = stats[c];
+        if (a.lse_in != nullptr) {
+            lse = a.lse_in[c];
+        } else {
+            lse = natural_lse(block_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x, BM_BLOCK), sh, BM_WAVES_PER_BLOCK));
+            if (b == 0 && threadIdx.x == 0) write_loss(a, c, lse, t);
+        }
+        none = none || t.lse == -INFINITY;
+    }
     const float k = it * kLog2e, from = lse * kLog2e;
-    constexpr int U = 4;                    // loads in flight per thread
-    const int step = (int)blockDim.x * 8;
-    for (int i0 = lo + (int)threadIdx.x * 8; i0 < hi; i0 += U * step) {
-        Raw8<T> x[U];
-        if (!none) {
+    for (int i = i0; i < hi;) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (i0 + u * step < hi) x[u] = load_col8(z, i0 + u * step, hi);
-        }
+        for (int u = 0; u < U; ++u)
+            if (i + u * STEP < hi) {
+                float8_t v = (float8_t)(0.f);
+                if (!none) {
+                    const float8_t y = x[u].wide();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u * step >= hi) break;
-            float8_t v = (float8_t)(0.f);
-            if (!none) {
-                const float8_t y = x[u].wide();
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+                    for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+                }
+                store_col8(dz, i + u * STEP, hi, v);
             }
-            store_col8(dz, i0 + u * step, hi, v);
-        }
+        i += U * STEP;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (!none && i + u * STEP < hi) x[u] = load_col8(z, i + u * STEP, hi);
     }
     if (none) return;
     __syncthreads();          // the entries' values go over what other threads of the workgroup wrote
-    int e0, e1;
-    column_entries(a, c, e0, e1);
+    if constexpr (ALONE) {
+        t = own;
+        if (t.lse == -INFINITY) {          // entries, but none that counts
+            for (int i = i0; i < hi; i += STEP) store_col8(dz, i, hi, (float8_t)(0.f));
+            return;
+        }
+    }
     for (int j = e0 + (int)threadIdx.x; j < e1; j += (int)blockDim.x) {
         const int r = a.tir[j];
-        if (r >= lo && r < hi) dz[r] = (T)(w * entry_grad(a, t, e0, e1, j, r, at[j], it, from));
+        if (r < lo || r >= hi) continue;
+        if constexpr (ALONE) {
+            int met = 0;
+            const int kept = min(e1 - e0, kRowsKept);
+            for (int q = 0; q < kept; ++q) met += rows[q] == r;
+            for (int q = e0 + kept; q < e1; ++q) met += a.tir[q] == r;
+            t.repeats = met > 1;
+        }
+        dz[r] = (T)(w * entry_grad(a, t, e0, e1, j, r, ALONE ? (float)z[r] * it : at[j], it, from));
     }
-}
-
-template <class T>
-__global__ __launch_bounds__(BM_BLOCK) void k_distill_grad(DistillArgs a, int nchunks, int chunk, int npart, const LogSum* parts,
-                                                           const Teacher* stats, const float* at) {
-    __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
-    const long long c = blockIdx.x / nchunks;
-    const int b = (int)(blockIdx.x % nchunks);
-    float lse;
-    const Teacher t = stats[c];
-    if (a.lse_in != nullptr) {
-        lse = a.lse_in[c];
-    } else {
-        lse = natural_lse(block_join(join_parts(parts + c * npart, npart, threadIdx.x, BM_BLOCK), sh, BM_WAVES_PER_BLOCK));
-        if (b == 0 && threadIdx.x == 0) write_loss(a, c, lse, t);
-    }
-    const int lo = b * chunk;
-    grad_chunk<T>(a, c, lo, min(a.nrows, lo + chunk), 1.f / a.temperature, lse, t, at);
 }
 
 // A whole column in the registers of one workgroup of BLOCK threads, NV vectors of eight logits each: read once, written
@@ -340,15 +381,20 @@ hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {
 
 template <class T>
 hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
-    hipError_t err;
-    float* at = (float*)ws_get(WS_DISTILL_AT, sizeof(float) * (size_t)a.nnz, &err, s);
-    if (!at) return err;
-    if (by_column<T>(a)) return distill_columns<T>(a, at, s);
     // a chunk is a multiple of what a workgroup takes at once; smaller ones where there are few columns
     int chunk = 4 * BM_BLOCK * 8;
     while (chunk > BM_BLOCK * 8 && (long long)a.ncols * ((a.nrows + chunk - 1) / chunk) < 1024) chunk >>= 1;
     const int nchunks = (a.nrows + chunk - 1) / chunk;
     const long long nparts = (long long)nchunks * a.ncols;
+    if (a.lse_in != nullptr && a.dZ != a.Z) {
+        if (nparts > 0x7fffffffLL) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((k_distill_grad<T, true>), dim3((unsigned)nparts), dim3(BM_BLOCK + 64), 0, s, a, nchunks, chunk, nullptr, nullptr, nullptr);
+        return hipGetLastError();
+    }
+    hipError_t err;
+    float* at = (float*)ws_get(WS_DISTILL_AT, sizeof(float) * (size_t)a.nnz, &err, s);
+    if (!at) return err;
+    if (by_column<T>(a)) return distill_columns<T>(a, at, s);
     char* buf = (char*)ws_get(WS_DISTILL, sizeof(Teacher) * (size_t)a.ncols + sizeof(LogSum) * (size_t)nparts, &err, s);
     if (!buf) return err;
     Teacher* stats = (Teacher*)buf;
@@ -359,7 +405,7 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_distill_parts<T>), dim3((unsigned)first), dim3(BM_BLOCK), 0, s, a, a.lse_in != nullptr ? 0 : nchunks, chunk, parts,
                        stats, at);
     if (a.dZ != nullptr)
-        hipLaunchKernelGGL((k_distill_grad<T>), dim3((unsigned)nparts), dim3(BM_BLOCK), 0, s, a, nchunks, chunk, nchunks, parts, stats, at);
+        hipLaunchKernelGGL((k_distill_grad<T, false>), dim3((unsigned)nparts), dim3(BM_BLOCK), 0, s, a, nchunks, chunk, parts, stats, at);
     else
         hipLaunchKernelGGL(k_distill_loss, dim3((unsigned)waves), dim3(BM_BLOCK), 0, s, a, nchunks, parts, stats);
     return hipGetLastError();
