@@ -77,22 +77,33 @@ __device__ int rows_repeat(const int* rows, int n) {
     return met != 0;
 }
 
-// One wave: statistics of a column's teacher entries; at[] receives the student's x at each of them.
+// One wave: statistics of a column's teacher entries; at[] receives the student's x at each of them. The first 64 entries
+// stay in registers, one per lane.
 template <class T>
 __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, float* at) {
     const int lane = threadIdx.x & 63;
     int lo, hi;
     column_entries(a, c, lo, hi);
     const T* z = (const T*)a.Z + c * a.ldz;
-    float top = -INFINITY, xtop = -INFINITY;
-    for (int j = lo + lane; j < hi; j += 64) {
+    struct Entry { bool in; float t, x; };
+    auto fetch = [&](int j) {
         const int r = a.tir[j];
+        const float t = a.tdata[j] * it;
         const bool in = (unsigned)r < (unsigned)a.nrows;
-        const float x = in ? (float)z[r] * it : 0.f;
-        at[j] = x;
-        if (in) {
-            top = fmaxf(top, a.tdata[j] * it);
-            xtop = fmaxf(xtop, x);
+        return Entry{in, t, in ? (float)z[r] * it : 0.f};
+    };
+    Entry e0 = {false, 0.f, 0.f};
+    if (lo + lane < hi) {
+        e0 = fetch(lo + lane);
+        at[lo + lane] = e0.x;
+    }
+    float top = e0.in ? e0.t : -INFINITY, xtop = e0.in ? e0.x : -INFINITY;
+    for (int j = lo + 64 + lane; j < hi; j += 64) {
+        const Entry e = fetch(j);
+        at[j] = e.x;
+        if (e.in) {
+            top = fmaxf(top, e.t);
+            xtop = fmaxf(xtop, e.x);
         }
     }
     top = group_allmax<64>(top);
@@ -100,24 +111,25 @@ __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, f
     if (xtop == -INFINITY || xtop == INFINITY) xtop = 0.f;
     float sum = 0.f;
     bool any = false;
-    for (int j = lo + lane; j < hi; j += 64)
-        if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
-            const float t = a.tdata[j] * it;
-            any = any || !(t == -INFINITY);
-            sum += t == -INFINITY ? 0.f : expf(t - top);
-        }
+    auto add = [&](const Entry& e) {
+        if (!e.in || e.t == -INFINITY) return;
+        any = true;
+        sum += expf(e.t - top);
+    };
+    add(e0);
+    for (int j = lo + 64 + lane; j < hi; j += 64) add(fetch(j));
     sum = group_allsum<64>(sum);
     Teacher r;
     r.lse = __ballot(any) != 0 ? top + logf(sum) : -INFINITY;
     float part = 0.f, mass = 0.f;
-    for (int j = lo + lane; j < hi; j += 64)
-        if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
-            const float logp = a.tdata[j] * it - r.lse, p = expf(logp);
-            if (p != 0.f) {
-                part += p * (logp - (at[j] - xtop));
-                mass += p;
-            }
-        }
+    auto weigh = [&](const Entry& e) {
+        const float logp = e.t - r.lse, p = expf(logp);
+        if (!e.in || p == 0.f) return;
+        part += p * (logp - (e.x - xtop));
+        mass += p;
+    };
+    weigh(e0);
+    for (int j = lo + 64 + lane; j < hi; j += 64) weigh(fetch(j));
     r.part = group_allsum<64>(part);
     r.mass = group_allsum<64>(mass);
     r.at0 = xtop;
@@ -183,9 +195,10 @@ __global__ __launch_bounds__(BM_BLOCK) void k_distill_loss(DistillArgs a, int nc
     if ((threadIdx.x & 63) == 0) write_loss(a, c, natural_lse(x), stats[c]);
 }
 
-// The gradient at teacher entry j of [e0, e1), whose student logit was x, over its scale.
-__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& t, int e0, int e1, int j, int r, float x, float it, float from) {
-    float p = expf(a.tdata[j] * it - t.lse);
+// The gradient at an entry of [e0, e1) in row r with the teacher's logit `value`, whose student logit was x, over its scale.
+__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& t, int e0, int e1, int r, float value, float x, float it,
+                                            float from) {
+    float p = expf(value * it - t.lse);
     if (t.repeats) {
         p = 0.f;
         for (int q = e0; q < e1; ++q)
@@ -219,6 +232,11 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     for (int u = 0; u < U; ++u)
         if (!none && i0 + u * STEP < hi) x[u] = load_col8(z, i0 + u * STEP, hi);
     const float it = 1.f / a.temperature;
+    // the first entries are on their way while the column is
+    const int j0 = e0 + (int)threadIdx.x;
+    const bool early = !none && j0 < e1;
+    const int r0 = early ? a.tir[j0] : -1;
+    const float t0 = early ? a.tdata[j0] : 0.f, x0 = ALONE || !early ? 0.f : at[j0];
     float lse;
     Teacher t;
     if constexpr (ALONE) {
@@ -278,8 +296,8 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
             return;
         }
     }
-    for (int j = e0 + (int)threadIdx.x; j < e1; j += (int)blockDim.x) {
-        const int r = a.tir[j];
+    for (int j = j0; j < e1; j += (int)blockDim.x) {
+        const int r = j == j0 ? r0 : a.tir[j];
         if (r < lo || r >= hi) continue;
         if constexpr (ALONE) {
             int met = 0;
@@ -288,7 +306,8 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
             for (int q = e0 + kept; q < e1; ++q) met += a.tir[q] == r;
             t.repeats = met > 1;
         }
-        dz[r] = (T)(w * entry_grad(a, t, e0, e1, j, r, ALONE ? (float)z[r] * it : at[j], it, from));
+        const float x = ALONE ? (float)z[r] * it : j == j0 ? x0 : at[j];
+        dz[r] = (T)(w * entry_grad(a, t, e0, e1, r, j == j0 ? t0 : a.tdata[j], x, it, from));
     }
 }
 
@@ -352,7 +371,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     for (int j = e0 + lane; j < e1; j += 64) {
         const int r = j < e0 + 64 ? r0 : a.tir[j];
         if ((unsigned)r >= (unsigned)n || ((r >> 3) & (BLOCK - 1)) >> 6 != wave) continue;
-        dz[r] = (T)(w * entry_grad(a, tc, e0, e1, j, r, j < e0 + 64 ? x0 : at[j], it, from));
+        dz[r] = (T)(w * entry_grad(a, tc, e0, e1, r, a.tdata[j], j < e0 + 64 ? x0 : at[j], it, from));
     }
 }
 
