@@ -17,7 +17,11 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-constexpr int kColumnsMin = 64;
+// Columns in registers (k_distill_column) or cut into chunks (two launches): up to 128 KiB a column in one workgroup is
+// faster however few there are (32768 bf16 rows: 8 columns 9.7 us against 12.7, 2048 columns 65 against 83); above, a
+// workgroup of its own takes about 20 us, and below this many columns the chunks win (131072 bf16 rows: 64 columns 22 us
+// against 17, 128 columns 24 against 22, 256 columns 33 against 45).
+constexpr int kColumnsMin = 160;
 constexpr int kRowsKept = 512;         // teacher rows of a column that a workgroup keeps in LDS
 
 // What a column's teacher entries come to. at0: the largest student logit x among them, subtracted before the sum so
@@ -380,10 +384,10 @@ hipError_t launch_column(const DistillArgs& a, float* at, hipStream_t s) {
     hipLaunchKernelGGL((k_distill_column<T, BLOCK, NV>), dim3((unsigned)a.ncols), dim3(BLOCK), 0, s, a, at);
     return hipGetLastError();
 }
-// Columns that fit the registers of a workgroup, where there are enough of them to fill the device.
 template <class T>
 bool by_column(const DistillArgs& a) {
-    return a.lse_in == nullptr && a.nrows <= (sizeof(T) == 2 ? 131072 : 65536) && a.ncols >= kColumnsMin;
+    const size_t bytes = sizeof(T) * (size_t)a.nrows;
+    return a.lse_in == nullptr && (bytes <= (128 << 10) || (bytes <= (256 << 10) && a.ncols >= kColumnsMin));
 }
 template <class T>
 hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {

@@ -137,19 +137,30 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
 #pragma unroll
     for (int v = 0; v < NV; ++v) dw[v] = (float8_t)(0.f);
     int turn = 0;
-    for (long long c = (long long)blockIdx.x * CPB + threadIdx.x / TPC; c < a.ncols; c += (long long)gridDim.x * CPB) {
-        const T* hp = (const T*)a.H + c * a.ldh;
-        const T* gp = (const T*)a.dY + c * a.lddy;
-        Raw8<T> h[NV], g[NV];
+    // A column's data are requested while the one before is worked on, where a thread's registers hold both.
+    constexpr bool AHEAD = TPC < 1024 || NV == 1;
+    const long long step = (long long)gridDim.x * CPB;
+    long long c = (long long)blockIdx.x * CPB + threadIdx.x / TPC;
+    Raw8<T> h[NV], g[NV], r[NV];
+    auto fetch = [&](long long col) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            h[v] = load_col8(hp, (v * TPC + t) * 8, n);
-            g[v] = load_col8(gp, (v * TPC + t) * 8, n);
+            h[v] = load_col8((const T*)a.H + col * a.ldh, (v * TPC + t) * 8, n);
+            g[v] = load_col8((const T*)a.dY + col * a.lddy, (v * TPC + t) * 8, n);
+            if (a.dH != nullptr) r[v] = load_col8((const T*)a.dH + col * a.lddh, (v * TPC + t) * 8, n);
         }
+    };
+    if (AHEAD && c < a.ncols) fetch(c);
+    for (; c < a.ncols; c += step) {
+        if (!AHEAD) fetch(c);
+        Raw8<T> hc[NV], gc[NV], rc[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) { hc[v] = h[v]; gc[v] = g[v]; rc[v] = r[v]; }
+        if (AHEAD && c + step < a.ncols) fetch(c + step);
         float hh = 0.f, gh = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const float8_t x = h[v].wide(), y = g[v].wide() * load_col8(a.w, (v * TPC + t) * 8, n).wide();
+            const float8_t x = hc[v].wide(), y = gc[v].wide() * load_col8(a.w, (v * TPC + t) * 8, n).wide();
             hh += square_sum(x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) gh = fmaf(x[j], y[j], gh);
@@ -163,10 +174,10 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int i = (v * TPC + t) * 8;
-            const float8_t x = h[v].wide(), y = g[v].wide();
+            const float8_t x = hc[v].wide(), y = gc[v].wide();
             float8_t d = rs * (y * load_col8(a.w, i, n).wide() - x * k);
             dw[v] += y * x * rs;
-            if (a.dH != nullptr) d += load_col8((const T*)a.dH + c * a.lddh, i, n).wide();
+            if (a.dH != nullptr) d += rc[v].wide();
             store_col8(o, i, n, d);
         }
     }
@@ -250,6 +261,20 @@ hipError_t by_height(int n, F&& f) {
     if (vecs <= 2048) return f.template go<T, 1024, 2>();
     return f.template go<T, 1024, 4>();
 }
+template <class T, class F>
+hipError_t by_height_grad(int n, F&& f) {
+    const int vecs = (n + 7) / 8;
+    if (vecs <= 8) return f.template go<T, 8, 1>();
+    if (vecs <= 16) return f.template go<T, 16, 1>();
+    if (vecs <= 32) return f.template go<T, 32, 1>();
+    if (vecs <= 64) return f.template go<T, 64, 1>();
+    if (vecs <= 128) return f.template go<T, 128, 1>();
+    if (vecs <= 256) return f.template go<T, 256, 1>();
+    if (vecs <= 512) return f.template go<T, 512, 1>();
+    if (vecs <= 1024) return f.template go<T, 1024, 1>();
+    if (vecs <= 2048) return f.template go<T, 1024, 2>();
+    return f.template go<T, 1024, 4>();
+}
 struct Norm {
     const NormArgs& a;
     hipStream_t s;
@@ -269,6 +294,10 @@ hipError_t by_type(int type, int n, F f) {
 
 hipError_t rmsnorm(const NormArgs& a, hipStream_t s) { return by_type(a.type, a.nrows, Norm{a, s}); }
 
-hipError_t rmsnorm_grad(const NormGradArgs& a, hipStream_t s) { return by_type(a.type, a.nrows, NormGrad{a, s}); }
+hipError_t rmsnorm_grad(const NormGradArgs& a, hipStream_t s) {
+    const int n = a.nrows;
+    NormGrad f{a, s};
+    return a.type == ELEM_F32 ? by_height_grad<float>(n, f) : a.type == ELEM_F16 ? by_height_grad<f16_t>(n, f) : by_height_grad<bf16_t>(n, f);
+}
 
 }  // namespace bm
