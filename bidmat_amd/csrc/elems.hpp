@@ -25,22 +25,59 @@ struct Raw8 {
     __device__ __forceinline__ static Raw8 narrow(float8_t x) { return {__builtin_convertvector(x, typename Eight<T>::type)}; }
 };
 
-// Elements i .. i+7 of a column of n; those past its end are neither read nor written and count as `fill`.
+// Elements i .. i+7 of a column of n; those past its end are neither read nor written and count as `fill`. A short last
+// part is read (and written) in pieces of four, two and one.
 template <class T>
 __device__ __forceinline__ Raw8<T> load_col8(const T* col, int i, int n, T fill = T(0.f)) {
     if (i + 8 <= n) return Raw8<T>::load(col + i);
     Raw8<T> r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.v[j] = i + j < n ? col[i + j] : fill;
+    for (int j = 0; j < 8; ++j) r.v[j] = fill;
+    const int rem = n - i;
+    if (rem <= 0) return r;
+    typedef T Two __attribute__((ext_vector_type(2)));
+    typedef T Four __attribute__((ext_vector_type(4)));
+    const T* p = col + i;
+    Two two;
+    if (rem & 4) {
+        Four four;
+        __builtin_memcpy(&four, p, sizeof(four));
+        r.v[0] = four[0]; r.v[1] = four[1]; r.v[2] = four[2]; r.v[3] = four[3];
+        if (rem & 2) {
+            __builtin_memcpy(&two, p + 4, sizeof(two));
+            r.v[4] = two[0]; r.v[5] = two[1];
+            if (rem & 1) r.v[6] = p[6];
+        } else if (rem & 1) {
+            r.v[4] = p[4];
+        }
+    } else if (rem & 2) {
+        __builtin_memcpy(&two, p, sizeof(two));
+        r.v[0] = two[0]; r.v[1] = two[1];
+        if (rem & 1) r.v[2] = p[2];
+    } else {
+        r.v[0] = p[0];
+    }
     return r;
 }
 template <class T>
 __device__ __forceinline__ void store_col8(T* col, int i, int n, float8_t x) {
-    const Raw8<T> r = Raw8<T>::narrow(x);
+    Raw8<T> r = Raw8<T>::narrow(x);
     if (i + 8 <= n) { r.store(col + i); return; }
+    const int rem = n - i;
+    if (rem <= 0) return;
+    T* p = col + i;
+    if (rem & 4) {
+        __builtin_memcpy(p, &r.v, 4 * sizeof(T));
+        p += 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (i + j < n) col[i + j] = r.v[j];
+        for (int j = 0; j < 4; ++j) r.v[j] = r.v[j + 4];
+    }
+    if (rem & 2) {
+        __builtin_memcpy(p, &r.v, 2 * sizeof(T));
+        p += 2;
+        r.v[0] = r.v[2];
+    }
+    if (rem & 1) *p = r.v[0];
 }
 
 // Largest value over aligned groups of N lanes (the steps of group_allsum); a NaN loses against any number.

@@ -147,9 +147,14 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         for (int v = 0; v < NV; ++v) {
             h[v] = load_col8((const T*)a.H + col * a.ldh, (v * TPC + t) * 8, n);
             g[v] = load_col8((const T*)a.dY + col * a.lddy, (v * TPC + t) * 8, n);
-            if (a.dH != nullptr) r[v] = load_col8((const T*)a.dH + col * a.lddh, (v * TPC + t) * 8, n);
+            if (AHEAD && a.dH != nullptr) r[v] = load_col8((const T*)a.dH + col * a.lddh, (v * TPC + t) * 8, n);
         }
     };
+    float8_t w[NV];
+    if (AHEAD) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) w[v] = load_col8(a.w, (v * TPC + t) * 8, n).wide();
+    }
     if (AHEAD && c < a.ncols) fetch(c);
     for (; c < a.ncols; c += step) {
         if (!AHEAD) fetch(c);
@@ -160,7 +165,7 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         float hh = 0.f, gh = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const float8_t x = hc[v].wide(), y = gc[v].wide() * load_col8(a.w, (v * TPC + t) * 8, n).wide();
+            const float8_t x = hc[v].wide(), y = gc[v].wide() * (AHEAD ? w[v] : load_col8(a.w, (v * TPC + t) * 8, n).wide());
             hh += square_sum(x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) gh = fmaf(x[j], y[j], gh);
@@ -175,46 +180,50 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         for (int v = 0; v < NV; ++v) {
             const int i = (v * TPC + t) * 8;
             const float8_t x = hc[v].wide(), y = gc[v].wide();
-            float8_t d = rs * (y * load_col8(a.w, i, n).wide() - x * k);
+            float8_t d = rs * (y * (AHEAD ? w[v] : load_col8(a.w, i, n).wide()) - x * k);
             dw[v] += y * x * rs;
-            if (a.dH != nullptr) d += rc[v].wide();
+            if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : load_col8((const T*)a.dH + c * a.lddh, i, n).wide();
             store_col8(o, i, n, d);
         }
     }
     if (a.dw == nullptr) return;
     float* share = partial + (size_t)blockIdx.x * n;
     if constexpr (CPB > 1) {
-        __shared__ float sum[TPC * 8 * NV];
-        for (int i = threadIdx.x; i < TPC * 8 * NV; i += BM_BLOCK) sum[i] = 0.f;
-        for (int p = 0; p < CPB; ++p) {
-            __syncthreads();
-            if ((int)threadIdx.x / TPC == p) {
+        // the columns of a wave first, then the workgroup's four waves
+        __shared__ float sum[BM_WAVES_PER_BLOCK][TPC * 8 * NV];
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[(v * TPC + t) * 8 + j] += dw[v][j];
+            for (int j = 0; j < 8; ++j) {
+                float d = dw[v][j];
+#pragma unroll
+                for (int m = TPC; m < 64; m <<= 1) d += __shfl_xor(d, m, 64);
+                if ((threadIdx.x & 63) < TPC) sum[threadIdx.x >> 6][(v * TPC + t) * 8 + j] = d;
             }
-        }
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += BM_BLOCK) share[i] = sum[i];
+        for (int i = threadIdx.x; i < n; i += BM_BLOCK) share[i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
     } else {
 #pragma unroll
         for (int v = 0; v < NV; ++v) store_col8(share, (v * TPC + t) * 8, n, dw[v]);
     }
 }
 
-// dw[i] = beta * dw[i] + sum over shares of partial[share][i]: 16 rows x 64 threads per workgroup, thread (x, y) adds
-// shares y, y + 64, ... of row x, then the 64 sums of a row are added by halves.
+// dw[i] = beta * dw[i] + sum over shares of partial[share][i]: ROWS rows x 1024 / ROWS threads per workgroup; thread (x, y)
+// adds every so many-th share of row x, then the sums of a row are added by halves.
+template <int ROWS>
 __global__ __launch_bounds__(1024) void k_add_shares(int n, int nshares, const float* __restrict__ partial, float* __restrict__ dw,
                                                      int beta) {
-    __shared__ float sh[64][17];
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    const int i = blockIdx.x * 16 + x;
+    constexpr int Y = 1024 / ROWS;
+    __shared__ float sh[Y][ROWS + 1];
+    const int x = threadIdx.x % ROWS, y = threadIdx.x / ROWS;
+    const int i = blockIdx.x * ROWS + x;
     float s = 0.f;
-    if (i < n)
-        for (int p = y; p < nshares; p += 64) s += partial[(size_t)p * n + i];
+    if (i < n) {
+#pragma unroll 8
+        for (int p = y; p < nshares; p += Y) s += partial[(size_t)p * n + i];
+    }
     sh[y][x] = s;
-    for (int step = 32; step > 0; step >>= 1) {
+    for (int step = Y / 2; step > 0; step >>= 1) {
         __syncthreads();
         if (y < step) sh[y][x] += sh[y + step][x];
     }
@@ -228,21 +237,24 @@ hipError_t launch_norm(const NormArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_rmsnorm<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a);
     return hipGetLastError();
 }
-constexpr int kShares = 512;      // workgroups of the gradient, at most
+// Workgroups of the gradient, at most: 16 waves per CU. More of them hide more latency but leave more shares of dw (4096
+// rows x 16384 columns bf16: 256 workgroups of 512 threads 134 us, 512 113 us, 1024 116 us).
+constexpr int norm_shares(int block) { return 262144 / block; }
 template <class T, int TPC, int NV>
 hipError_t launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
     constexpr int CPB = norm_block(TPC) / TPC;
-    const long long want = (a.ncols + CPB - 1LL) / CPB;
-    const unsigned grid = (unsigned)(want < kShares ? want : kShares);
+    const long long want = (a.ncols + CPB - 1LL) / CPB, most = norm_shares(norm_block(TPC));
+    const unsigned grid = (unsigned)(want < most ? want : most);
     float* partial = nullptr;
     if (a.dw != nullptr) {
         hipError_t err;
-        partial = (float*)ws_get(WS_NORM_SHARES, sizeof(float) * (size_t)kShares * (size_t)a.nrows, &err, s);
+        partial = (float*)ws_get(WS_NORM_SHARES, sizeof(float) * (size_t)grid * (size_t)a.nrows, &err, s);
         if (!partial) return err;
     }
     hipLaunchKernelGGL((k_rmsnorm_grad<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a, partial);
     if (a.dw != nullptr)
-        hipLaunchKernelGGL(k_add_shares, dim3((a.nrows + 15) / 16), dim3(1024), 0, s, a.nrows, (int)grid, partial, a.dw, a.beta);
+        hipLaunchKernelGGL((a.nrows >= 1024 ? k_add_shares<16> : k_add_shares<4>), dim3(a.nrows >= 1024 ? (a.nrows + 15) / 16 : (a.nrows + 3) / 4),
+                           dim3(1024), 0, s, a.nrows, (int)grid, partial, a.dw, a.beta);
     return hipGetLastError();
 }
 
