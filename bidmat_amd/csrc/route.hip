@@ -514,6 +514,15 @@ __device__ __forceinline__ void row_rank(float score, float lo, float hi, int& r
     }
 }
 
+// How many of the other lanes of the column hold a larger key.
+template <int N>
+__device__ __forceinline__ void row_before(int key, int& before) {
+    if constexpr (N < 16) {
+        before += row_move<0x120 + N>(key) > key;      // row_ror N
+        row_before<N + 1>(key, before);
+    }
+}
+
 // Exact keys (scores of 16 bits, no bias, no groups) get the expert's number into their lower bits, so that no two are
 // equal and the lower expert stands higher. Other keys are p + bias + bmax: never negative, so that their bits are in
 // order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
@@ -584,16 +593,26 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     int lo, hi = row_max(best), n;
     hi = hi == kShut ? kShut + 2 : hi + 1;
     {
-        const int two[2] = {best, second};
-        int end = hi;
-        lo = row_min(second == kShut ? (best == kShut ? INT_MAX : best) : second);
-        n = row_count(two, lo);
-        const bool enough = n >= want;
-        while (__ballot(enough && n != want && (unsigned)end - (unsigned)lo > 1u) != 0) {
-            const int mid = lo + (int)(((unsigned)end - (unsigned)lo) >> 1);
-            const int m = row_count(two, mid);
-            if (enough) {
-                if (m >= want) { lo = mid; n = m; } else end = mid;
+        bool enough;
+        if (__ballot(row_sum(best != kShut) < 2 * want) == 0) {
+            // open keys in twice as many lanes as keys are wanted: few lanes hold two of them, so that the want-th of the lanes'
+            // largest keys is close to the border, and on its far side
+            int before = 0;
+            row_before<1>(best, before);
+            lo = row_min(before < want && best != kShut ? best : INT_MAX);
+            enough = true;
+        } else {
+            const int two[2] = {best, second};
+            int end = hi;
+            lo = row_min(second == kShut ? (best == kShut ? INT_MAX : best) : second);
+            n = row_count(two, lo);
+            enough = n >= want;
+            while (__ballot(enough && n != want && (unsigned)end - (unsigned)lo > 1u) != 0) {
+                const int mid = lo + (int)(((unsigned)end - (unsigned)lo) >> 1);
+                const int m = row_count(two, mid);
+                if (enough) {
+                    if (m >= want) { lo = mid; n = m; } else end = mid;
+                }
             }
         }
         if (__ballot(!enough) != 0) {
@@ -871,8 +890,8 @@ hipError_t launch_route(const RouteArgs& a, Deal d, hipStream_t s) {
 
 template <class T, int VPL>
 hipError_t launch_route_rows(const RouteArgs& a, Deal d, const Deal& d64, hipStream_t s) {
-    const long long all = 8192;
-    d.batch = a.ncols >= all * 8 ? 8 : 4;
+    const long long all = 4096;
+    d.batch = a.ncols >= all * 4 ? 8 : 4;
     const long long want = (a.ncols + BM_WAVES_PER_BLOCK * (long long)d.batch - 1) / (BM_WAVES_PER_BLOCK * d.batch);
     const unsigned grid = (unsigned)(want < all / BM_WAVES_PER_BLOCK ? want : all / BM_WAVES_PER_BLOCK);
     int* shares;
