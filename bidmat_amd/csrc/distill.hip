@@ -24,37 +24,61 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kColumnsMin = 160;
 constexpr int kRowsKept = 512;         // teacher rows of a column that a workgroup keeps in LDS
 
-// What a column's teacher entries come to. at0: the largest student logit x among them, subtracted before the sum so
-// that loss = tau^2 * weight * (part + mass * (lse - at0)) cancels nothing large.
-struct Teacher { float lse, part, mass, at0; int repeats; };      // lse = -inf: no entries; repeats: a row is stored twice
+// Differences of logits are taken before they are scaled: a mask of the type's lowest value stays finite, and large
+// common offsets cost no digits.
+//
+// What a column's teacher entries come to: p_j = exp((T_j - top) / tau - lsum). at0: the largest student logit among them,
+// so that loss = tau^2 * weight * (part + mass * (lse - at0 / tau)) cancels nothing large.
+struct Teacher {
+    float top, lsum, part, mass, at0;
+    int some, repeats;                   // whether an entry counts; whether a row is stored twice
+};
 
-// A running log-sum in base 2: sum of 2^(v - top).
+// A running sum of 2^((z - top) * k), k = log2(e) / tau.
 struct LogSum { float top, sum; };
-__device__ __forceinline__ LogSum join(LogSum a, LogSum b) {
+__device__ __forceinline__ LogSum join(LogSum a, LogSum b, float k) {
     const float top = fmaxf(a.top, b.top);
     if (top == -INFINITY) return {top, a.sum + b.sum};          // both empty; a NaN in a sum stays
-    return {top, a.sum * __builtin_amdgcn_exp2f(a.top - top) + b.sum * __builtin_amdgcn_exp2f(b.top - top)};
+    return {top, a.sum * __builtin_amdgcn_exp2f((a.top - top) * k) + b.sum * __builtin_amdgcn_exp2f((b.top - top) * k)};
 }
-__device__ __forceinline__ LogSum wave_join(LogSum x) {
+__device__ __forceinline__ LogSum wave_join(LogSum x, float k) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         LogSum y;
         y.top = __shfl_xor(x.top, m, 64);
         y.sum = __shfl_xor(x.sum, m, 64);
-        x = join(x, y);
+        x = join(x, y, k);
     }
     return x;
 }
 // All threads of a workgroup of 64 * waves get the joined log-sum.
-__device__ __forceinline__ LogSum block_join(LogSum x, LogSum* sh, int waves) {
-    x = wave_join(x);
+__device__ __forceinline__ LogSum block_join(LogSum x, float k, LogSum* sh, int waves) {
+    x = wave_join(x, k);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
     __syncthreads();
     x = sh[0];
-    for (int w = 1; w < waves; ++w) x = join(x, sh[w]);
+    for (int w = 1; w < waves; ++w) x = join(x, sh[w], k);
     return x;
 }
-__device__ __forceinline__ float natural_lse(LogSum x) { return (x.top + __log2f(x.sum)) * kLn2; }
+// Eight more logits.
+__device__ __forceinline__ LogSum add_eight(LogSum s, float8_t z, float k) {
+    float top = s.top;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, z[j]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = s.sum * __builtin_amdgcn_exp2f((s.top - from) * k);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f((z[j] - from) * k);
+    return {top, sum};
+}
+
+// q = exp(z / tau - lse) = 2^((z - base) * k - off), from a column's log-sum or from a kept lse.
+struct Share {
+    float k, base, off;
+    __device__ __forceinline__ float operator()(float z) const { return __builtin_amdgcn_exp2f(fmaf(z - base, k, -off)); }
+};
+__device__ __forceinline__ Share share_of(LogSum s, float k) { return {k, s.top, __log2f(s.sum)}; }
+__device__ __forceinline__ Share share_of_lse(float lse, float k) { return {k, 0.f, lse * kLog2e}; }
 
 __device__ __forceinline__ void column_entries(const DistillArgs& a, long long c, int& lo, int& hi) {
     lo = min(max(a.tjc[c], 0), a.nnz);
@@ -81,62 +105,62 @@ __device__ int rows_repeat(const int* rows, int n) {
     return met != 0;
 }
 
-// One wave: statistics of a column's teacher entries; at[] receives the student's x at each of them. The first 64 entries
-// stay in registers, one per lane.
+// One wave: statistics of a column's teacher entries; at[] receives the student's logit at each of them. The first 64
+// entries stay in registers, one per lane.
 template <class T>
 __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, float* at) {
     const int lane = threadIdx.x & 63;
     int lo, hi;
     column_entries(a, c, lo, hi);
     const T* z = (const T*)a.Z + c * a.ldz;
-    struct Entry { bool in; float t, x; };
+    struct Entry { bool in; float t, z; };
     auto fetch = [&](int j) {
         const int r = a.tir[j];
-        const float t = a.tdata[j] * it;
+        const float t = a.tdata[j];
         const bool in = (unsigned)r < (unsigned)a.nrows;
-        return Entry{in, t, in ? (float)z[r] * it : 0.f};
+        return Entry{in, t, in ? (float)z[r] : 0.f};
     };
     Entry e0 = {false, 0.f, 0.f};
     if (lo + lane < hi) {
         e0 = fetch(lo + lane);
-        at[lo + lane] = e0.x;
+        at[lo + lane] = e0.z;
     }
-    float top = e0.in ? e0.t : -INFINITY, xtop = e0.in ? e0.x : -INFINITY;
+    Teacher r;
+    r.top = e0.in ? e0.t : -INFINITY;
+    r.at0 = e0.in ? e0.z : -INFINITY;
     for (int j = lo + 64 + lane; j < hi; j += 64) {
         const Entry e = fetch(j);
-        at[j] = e.x;
+        at[j] = e.z;
         if (e.in) {
-            top = fmaxf(top, e.t);
-            xtop = fmaxf(xtop, e.x);
+            r.top = fmaxf(r.top, e.t);
+            r.at0 = fmaxf(r.at0, e.z);
         }
     }
-    top = group_allmax<64>(top);
-    xtop = group_allmax<64>(xtop);
-    if (xtop == -INFINITY || xtop == INFINITY) xtop = 0.f;
+    r.top = group_allmax<64>(r.top);
+    r.at0 = group_allmax<64>(r.at0);
+    if (r.at0 == -INFINITY || r.at0 == INFINITY) r.at0 = 0.f;
     float sum = 0.f;
-    bool any = false;
+    bool some = false;
     auto add = [&](const Entry& e) {
         if (!e.in || e.t == -INFINITY) return;
-        any = true;
-        sum += expf(e.t - top);
+        some = true;
+        sum += expf((e.t - r.top) * it);
     };
     add(e0);
     for (int j = lo + 64 + lane; j < hi; j += 64) add(fetch(j));
-    sum = group_allsum<64>(sum);
-    Teacher r;
-    r.lse = __ballot(any) != 0 ? top + logf(sum) : -INFINITY;
-    float part = 0.f, mass = 0.f;
+    r.some = __ballot(some) != 0;
+    r.lsum = logf(group_allsum<64>(sum));
+    r.part = r.mass = 0.f;
     auto weigh = [&](const Entry& e) {
-        const float logp = e.t - r.lse, p = expf(logp);
+        const float logp = (e.t - r.top) * it - r.lsum, p = expf(logp);
         if (!e.in || p == 0.f) return;
-        part += p * (logp - (e.x - xtop));
-        mass += p;
+        r.part += p * (logp - (e.z - r.at0) * it);
+        r.mass += p;
     };
     weigh(e0);
     for (int j = lo + 64 + lane; j < hi; j += 64) weigh(fetch(j));
-    r.part = group_allsum<64>(part);
-    r.mass = group_allsum<64>(mass);
-    r.at0 = xtop;
+    r.part = group_allsum<64>(r.part);
+    r.mass = group_allsum<64>(r.mass);
     r.repeats = rows_repeat(a.tir + lo, hi - lo);
     return r;
 }
@@ -160,34 +184,24 @@ __global__ __launch_bounds__(BM_BLOCK) void k_distill_parts(DistillArgs a, int n
     const int lo = b * chunk, hi = min(a.nrows, lo + chunk);
     const float k = it * kLog2e;
     LogSum x = {-INFINITY, 0.f};
-    for (int i = lo + (int)threadIdx.x * 8; i < hi; i += BM_BLOCK * 8) {
-        const float8_t v = load_col8(z, i, hi, (T)(-INFINITY)).wide() * k;
-        float top = v[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, v[j]);
-        top = fmaxf(top, x.top);
-        const float from = top == -INFINITY ? 0.f : top;
-        float sum = x.sum * __builtin_amdgcn_exp2f(x.top - from);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f(v[j] - from);
-        x = {top, sum};
-    }
-    x = block_join(x, sh, BM_WAVES_PER_BLOCK);
+    for (int i = lo + (int)threadIdx.x * 8; i < hi; i += BM_BLOCK * 8) x = add_eight(x, load_col8(z, i, hi, (T)(-INFINITY)).wide(), k);
+    x = block_join(x, k, sh, BM_WAVES_PER_BLOCK);
     if (threadIdx.x == 0) parts[blockIdx.x] = x;
 }
 
-__device__ __forceinline__ LogSum join_parts(const LogSum* parts, int nchunks, int t, int step) {
+__device__ __forceinline__ LogSum join_parts(const LogSum* parts, int nchunks, int t, int step, float k) {
     LogSum x = {-INFINITY, 0.f};
-    for (int b = t; b < nchunks; b += step) x = join(x, parts[b]);
+    for (int b = t; b < nchunks; b += step) x = join(x, parts[b], k);
     return x;
 }
 
-__device__ __forceinline__ void write_loss(const DistillArgs& a, long long c, float lse, const Teacher& t) {
-    if (a.lse != nullptr) a.lse[c] = lse;
+__device__ __forceinline__ void write_loss(const DistillArgs& a, long long c, LogSum s, float it, const Teacher& t) {
+    const float l = __log2f(s.sum) * kLn2;
+    if (a.lse != nullptr) a.lse[c] = fmaf(s.top, it, l);
     if (a.loss != nullptr) {
         const float w = column_scale(a, c);
-        const float v = w * a.temperature * a.temperature * (t.part + t.mass * (lse - t.at0));
-        a.loss[c] = t.lse == -INFINITY || w == 0.f ? 0.f : v;
+        const float v = w * a.temperature * a.temperature * (t.part + t.mass * ((s.top - t.at0) * it + l));
+        a.loss[c] = !t.some || w == 0.f ? 0.f : v;
     }
 }
 
@@ -195,20 +209,21 @@ __device__ __forceinline__ void write_loss(const DistillArgs& a, long long c, fl
 __global__ __launch_bounds__(BM_BLOCK) void k_distill_loss(DistillArgs a, int nchunks, const LogSum* parts, const Teacher* stats) {
     const long long c = (long long)blockIdx.x * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6);
     if (c >= a.ncols) return;
-    const LogSum x = wave_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x & 63, 64));
-    if ((threadIdx.x & 63) == 0) write_loss(a, c, natural_lse(x), stats[c]);
+    const float it = 1.f / a.temperature, k = it * kLog2e;
+    const LogSum x = wave_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x & 63, 64, k), k);
+    if ((threadIdx.x & 63) == 0) write_loss(a, c, x, it, stats[c]);
 }
 
-// The gradient at an entry of [e0, e1) in row r with the teacher's logit `value`, whose student logit was x, over its scale.
-__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& t, int e0, int e1, int r, float value, float x, float it,
-                                            float from) {
-    float p = expf(value * it - t.lse);
+// The gradient at an entry of [e0, e1) in row r with the teacher's logit `value`, whose student logit was z, over its scale.
+__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& t, int e0, int e1, int r, float value, float z, float it,
+                                            const Share& q) {
+    float p = expf((value - t.top) * it - t.lsum);
     if (t.repeats) {
         p = 0.f;
-        for (int q = e0; q < e1; ++q)
-            if (a.tir[q] == r) p += expf(a.tdata[q] * it - t.lse);
+        for (int i = e0; i < e1; ++i)
+            if (a.tir[i] == r) p += expf((a.tdata[i] - t.top) * it - t.lsum);
     }
-    return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -from)) - p;
+    return q(z) - p;
 }
 
 // The gradient of rows [lo, hi) of column c. ALONE: nothing was prepared and dZ is not Z: the log-sum is an earlier call's, and
@@ -241,39 +256,40 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     const bool early = !none && j0 < e1;
     const int r0 = early ? a.tir[j0] : -1;
     const float t0 = early ? a.tdata[j0] : 0.f, x0 = ALONE || !early ? 0.f : at[j0];
-    float lse;
+    const float k = it * kLog2e;
+    Share q;
     Teacher t;
     if constexpr (ALONE) {
-        lse = a.lse_in[c];
+        q = share_of_lse(a.lse_in[c], k);
         if (extra && !none) {
             const int lane = threadIdx.x & 63;
-            float top = -INFINITY, sum = 0.f;
-            bool any = false;
+            float sum = 0.f;
+            bool some = false;
+            t.top = -INFINITY;
             for (int j = e0 + lane; j < e1; j += 64)
-                if ((unsigned)a.tir[j] < (unsigned)a.nrows) top = fmaxf(top, a.tdata[j] * it);
-            top = group_allmax<64>(top);
+                if ((unsigned)a.tir[j] < (unsigned)a.nrows) t.top = fmaxf(t.top, a.tdata[j]);
+            t.top = group_allmax<64>(t.top);
             for (int j = e0 + lane; j < e1; j += 64)
-                if ((unsigned)a.tir[j] < (unsigned)a.nrows) {
-                    const float v = a.tdata[j] * it;
-                    any = any || !(v == -INFINITY);
-                    sum += v == -INFINITY ? 0.f : expf(v - top);
+                if ((unsigned)a.tir[j] < (unsigned)a.nrows && a.tdata[j] != -INFINITY) {
+                    some = true;
+                    sum += expf((a.tdata[j] - t.top) * it);
                 }
-            sum = group_allsum<64>(sum);
-            t.lse = __ballot(any) != 0 ? top + logf(sum) : -INFINITY;
+            t.lsum = logf(group_allsum<64>(sum));
+            t.some = __ballot(some) != 0;
             for (int j = lane; j < kRowsKept && e0 + j < e1; j += 64) rows[j] = a.tir[e0 + j];
             if (lane == 0) own = t;
         }
     } else {
         t = stats[c];
         if (a.lse_in != nullptr) {
-            lse = a.lse_in[c];
+            q = share_of_lse(a.lse_in[c], k);
         } else {
-            lse = natural_lse(block_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x, BM_BLOCK), sh, BM_WAVES_PER_BLOCK));
-            if (b == 0 && threadIdx.x == 0) write_loss(a, c, lse, t);
+            const LogSum s = block_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x, BM_BLOCK, k), k, sh, BM_WAVES_PER_BLOCK);
+            q = share_of(s, k);
+            if (b == 0 && threadIdx.x == 0) write_loss(a, c, s, it, t);
         }
-        none = none || t.lse == -INFINITY;
+        none = none || !t.some;
     }
-    const float k = it * kLog2e, from = lse * kLog2e;
     for (int i = i0; i < hi;) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -282,7 +298,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
                 if (!none) {
                     const float8_t y = x[u].wide();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+                    for (int j = 0; j < 8; ++j) v[j] = w * q(y[j]);
                 }
                 store_col8(dz, i + u * STEP, hi, v);
             }
@@ -295,7 +311,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     __syncthreads();          // the entries' values go over what other threads of the workgroup wrote
     if constexpr (ALONE) {
         t = own;
-        if (t.lse == -INFINITY) {          // entries, but none that counts
+        if (!t.some) {          // entries, but none that counts
             for (int i = i0; i < hi; i += STEP) store_col8(dz, i, hi, (float8_t)(0.f));
             return;
         }
@@ -310,8 +326,8 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
             for (int q = e0 + kept; q < e1; ++q) met += a.tir[q] == r;
             t.repeats = met > 1;
         }
-        const float x = ALONE ? (float)z[r] * it : j == j0 ? x0 : at[j];
-        dz[r] = (T)(w * entry_grad(a, t, e0, e1, r, j == j0 ? t0 : a.tdata[j], x, it, from));
+        const float zr = ALONE ? (float)z[r] : j == j0 ? x0 : at[j];
+        dz[r] = (T)(w * entry_grad(a, t, e0, e1, r, j == j0 ? t0 : a.tdata[j], zr, it, q));
     }
 }
 
@@ -338,24 +354,20 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     for (int v = 0; v < NV; ++v) x[v] = load_col8(z, (v * BLOCK + t) * 8, n, (T)(-INFINITY));
     LogSum s = {-INFINITY, 0.f};
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const float8_t y = x[v].wide() * k;
-        float top = s.top;
+    for (int v = 0; v < NV; ++v) s = add_eight(s, x[v].wide(), k);
+    s = block_join(s, k, sh, WAVES);
+    // 16-bit logits are widened again below: kept from above as floats they would take twice the registers
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
-        const float from = top == -INFINITY ? 0.f : top;
-        float sum = s.sum * __builtin_amdgcn_exp2f(s.top - from);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f(y[j] - from);
-        s = {top, sum};
+        for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(x[v].v));
     }
-    const float lse = natural_lse(block_join(s, sh, WAVES));
     const Teacher tc = teacher;
-    if (t == 0) write_loss(a, c, lse, tc);
+    if (t == 0) write_loss(a, c, s, it, tc);
     if (a.dZ == nullptr) return;
     T* dz = (T*)a.dZ + c * a.lddz;
-    const float w = column_scale(a, c) * a.temperature, from = lse * kLog2e;
-    const bool none = tc.lse == -INFINITY || w == 0.f;
+    const float w = column_scale(a, c) * a.temperature;
+    const Share q = share_of(s, k);
+    const bool none = !tc.some || w == 0.f;
     int e0, e1;
     column_entries(a, c, e0, e1);
     const bool first = !none && e0 + lane < e1;
@@ -367,7 +379,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
         if (!none) {
             const float8_t y = x[v].wide();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] = w * __builtin_amdgcn_exp2f(fmaf(y[j], k, -from));
+            for (int j = 0; j < 8; ++j) d[j] = w * q(y[j]);
         }
         store_col8(dz, (v * BLOCK + t) * 8, n, d);
     }
@@ -375,7 +387,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     for (int j = e0 + lane; j < e1; j += 64) {
         const int r = j < e0 + 64 ? r0 : a.tir[j];
         if ((unsigned)r >= (unsigned)n || ((r >> 3) & (BLOCK - 1)) >> 6 != wave) continue;
-        dz[r] = (T)(w * entry_grad(a, tc, e0, e1, r, a.tdata[j], j < e0 + 64 ? x0 : at[j], it, from));
+        dz[r] = (T)(w * entry_grad(a, tc, e0, e1, r, a.tdata[j], j < e0 + 64 ? x0 : at[j], it, q));
     }
 }
 
