@@ -7,6 +7,7 @@
 #include "kernels.hpp"
 #include "workspace.hpp"
 #include <climits>
+#include <initializer_list>
 #include <cmath>
 
 #define API extern "C" __attribute__((visibility("default")))
@@ -17,25 +18,37 @@ constexpr int kInvalid = (int)hipErrorInvalidValue;
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-// A dense operand: nrows x ncols elements of `size` bytes, column stride ld.
-struct Block {
-    const void* p;
-    long long ld;
-    size_t size;
-};
 bool type_ok(int type) { return type == BIDMAT_F32 || type == BIDMAT_F16 || type == BIDMAT_BF16; }
-bool block_ok(const Block& b, int nrows) { return b.ld >= nrows && (uintptr_t)b.p % b.size == 0; }
-// Two operands of the same shape share memory in another way than element by element.
-bool clash(const Block& x, const Block& y, int nrows, int ncols) {
-    if (x.p == nullptr || y.p == nullptr) return false;
-    if (x.p == y.p && x.ld == y.ld && x.size == y.size) return false;
-    const uintptr_t x0 = (uintptr_t)x.p, x1 = x0 + ((size_t)(ncols - 1) * x.ld + nrows) * x.size;
-    const uintptr_t y0 = (uintptr_t)y.p, y1 = y0 + ((size_t)(ncols - 1) * y.ld + nrows) * y.size;
-    return x0 < y1 && y0 < x1;
+
+// An operand of a call: a vector of n elements of `size` bytes, or a dense matrix of nrows x ncols with column stride ld.
+struct Operand {
+    const void* p;
+    size_t size, n;
+    long long ld;            // 0: a vector
+    bool out, aligned;
+};
+template <class T>
+Operand vec(const T* p, long long n, bool out = false) {
+    return {p, sizeof(T), (size_t)n, 0, out, (uintptr_t)p % sizeof(T) == 0};
 }
-// Two outputs share memory at all.
-bool meet(const Block& x, const Block& y, int nrows, int ncols) {
-    return x.p != nullptr && (x.p == y.p || clash(x, y, nrows, ncols));
+Operand dense(const void* p, size_t size, int nrows, int ncols, long long ld, bool out = false) {
+    return {p, size, (size_t)(ncols - 1) * (size_t)ld + nrows, ld, out, (uintptr_t)p % size == 0 && ld >= nrows};
+}
+// Every operand given (p not null) lies at a multiple of its element, with columns apart; and no output shares memory with
+// another operand, except a dense one that is a dense input, element by element.
+bool operands_ok(std::initializer_list<Operand> all) {
+    for (const Operand* x = all.begin(); x != all.end(); ++x) {
+        if (!x->p) continue;
+        if (!x->aligned) return false;
+        for (const Operand* y = all.begin(); y != x; ++y) {
+            if (!y->p || (!x->out && !y->out)) continue;
+            const uintptr_t x0 = (uintptr_t)x->p, x1 = x0 + x->n * x->size, y0 = (uintptr_t)y->p, y1 = y0 + y->n * y->size;
+            if (x0 >= y1 || y0 >= x1) continue;
+            const bool same = x->ld != 0 && x0 == y0 && x->ld == y->ld && x->size == y->size;
+            if (!same || (x->out && y->out)) return false;
+        }
+    }
+    return true;
 }
 bool group_ok(int group) { return group == 0 || group == 32 || group == 64 || group == 128; }
 
@@ -48,18 +61,10 @@ API int bidmat_rmsnorm(int nrows, int ncols, int type, const void* X, int ldx, c
     if (nrows == 0 || ncols == 0) return 0;
     if (!X || !w || (!H && !Y && !Q)) return kInvalid;
     const size_t size = bm::elem_size(type);
-    const Block in[2] = {{X, ldx, size}, {R, ldr, size}};
-    const Block out[3] = {{H, ldh, size}, {Y, ldy, size}, {Q, ldq, 1}};
-    for (const Block& b : in)
-        if (b.p && !block_ok(b, nrows)) return kInvalid;
-    for (int i = 0; i < 3; ++i) {
-        if (!out[i].p) continue;
-        if (!block_ok(out[i], nrows)) return kInvalid;
-        for (const Block& b : in)
-            if (clash(out[i], b, nrows, ncols)) return kInvalid;
-        for (int j = 0; j < i; ++j)
-            if (meet(out[i], out[j], nrows, ncols)) return kInvalid;
-    }
+    const long long ng = group == 0 ? 1 : (nrows + group - 1) / group;
+    if (!operands_ok({dense(X, size, nrows, ncols, ldx), dense(R, size, nrows, ncols, ldr), vec(w, nrows), dense(H, size, nrows, ncols, ldh, true),
+                      dense(Y, size, nrows, ncols, ldy, true), dense(Q, 1, nrows, ncols, ldq, true), vec(scales, ng * ncols, true)}))
+        return kInvalid;
     bm::NormArgs a{nrows, ncols, type, X, R, ldx, ldr, w, eps, H, Y, ldh, ldy, Q, ldq, scales, group};
     return (int)bm::rmsnorm(a, as_stream(stream));
 }
@@ -73,10 +78,9 @@ API int bidmat_rmsnorm_grad(int nrows, int ncols, int type, const void* H, int l
     if (ncols == 0) return dw && beta == 0 ? (int)bm::fill_f32(dw, nrows, 0.f, as_stream(stream)) : 0;
     if (!H || !w || !dY || !dX) return kInvalid;
     const size_t size = bm::elem_size(type);
-    const Block in[3] = {{H, ldh, size}, {dY, lddy, size}, {dH, lddh, size}}, out = {dX, lddx, size};
-    if (!block_ok(out, nrows)) return kInvalid;
-    for (const Block& b : in)
-        if (b.p && (!block_ok(b, nrows) || clash(out, b, nrows, ncols))) return kInvalid;
+    if (!operands_ok({dense(H, size, nrows, ncols, ldh), vec(w, nrows), dense(dY, size, nrows, ncols, lddy), dense(dH, size, nrows, ncols, lddh),
+                      dense(dX, size, nrows, ncols, lddx, true), vec(dw, nrows, true)}))
+        return kInvalid;
     bm::NormGradArgs a{nrows, ncols, type, H, dY, dH, ldh, lddy, lddh, w, eps, dX, lddx, dw, beta};
     return (int)bm::rmsnorm_grad(a, as_stream(stream));
 }
@@ -94,7 +98,11 @@ API int bidmat_route(int nexperts, int ncols, int type, const void* Z, int ldz, 
         if (e == hipSuccess && counts) e = bm::fill_i32(counts, nexperts, 0, as_stream(stream));
         return (int)e;
     }
-    if (!Z || !Gdata || !Gir || !block_ok({Z, ldz, bm::elem_size(type)}, nexperts)) return kInvalid;
+    const long long nnz = (long long)ncols * topk;
+    if (!Z || !Gdata || !Gir) return kInvalid;
+    if (!operands_ok({dense(Z, bm::elem_size(type), nexperts, ncols, ldz), vec(bias, nexperts), vec(Gdata, nnz, true), vec(Gir, nnz, true),
+                      vec(Gic, nnz, true), vec(Gjc, ncols + 1LL, true), vec(counts, nexperts, true)}))
+        return kInvalid;
     bm::RouteArgs a{nexperts, ncols, type, Z, ldz, bias, kind, ngroups, topgroups, topk, renorm, scale, Gdata, Gir, Gic, Gjc, counts};
     return (int)bm::route(a, as_stream(stream));
 }
@@ -107,8 +115,11 @@ API int bidmat_route_grad(int nexperts, int ncols, int type, const void* Z, int 
     if ((long long)ncols * topk > INT_MAX) return kInvalid;
     if (ncols == 0) return 0;
     if (!Z || !Gdata || !Gir || !dG || !dZ) return kInvalid;
-    const Block z = {Z, ldz, bm::elem_size(type)}, dz = {dZ, lddz, bm::elem_size(type)};
-    if (!block_ok(z, nexperts) || !block_ok(dz, nexperts) || clash(z, dz, nexperts, ncols)) return kInvalid;
+    const long long nnz = (long long)ncols * topk;
+    const size_t size = bm::elem_size(type);
+    if (!operands_ok({dense(Z, size, nexperts, ncols, ldz), vec(Gdata, nnz), vec(Gir, nnz), vec(dG, nnz),
+                      dense(dZ, size, nexperts, ncols, lddz, true)}))
+        return kInvalid;
     bm::RouteGradArgs a{nexperts, ncols, type, Z, ldz, kind, topk, renorm, scale, Gdata, Gir, dG, dZ, lddz};
     return (int)bm::route_grad(a, as_stream(stream));
 }
@@ -119,9 +130,11 @@ int distill_call(const bm::DistillArgs& a, hipStream_t s) {
     if (!(a.temperature > 0.f) || std::isinf(a.temperature) || std::isinf(1.f / a.temperature)) return kInvalid;
     if (a.nrows == 0 || a.ncols == 0) return a.nnz > 0 ? kInvalid : 0;
     if (!a.Z || !a.tjc || (a.nnz > 0 && (!a.tdata || !a.tir))) return kInvalid;
-    const Block z = {a.Z, a.ldz, bm::elem_size(a.type)}, dz = {a.dZ, a.lddz, bm::elem_size(a.type)};
-    if (!block_ok(z, a.nrows)) return kInvalid;
-    if (a.dZ && (!block_ok(dz, a.nrows) || clash(z, dz, a.nrows, a.ncols))) return kInvalid;
+    const size_t size = bm::elem_size(a.type);
+    if (!operands_ok({dense(a.Z, size, a.nrows, a.ncols, a.ldz), vec(a.tdata, a.nnz), vec(a.tir, a.nnz), vec(a.tjc, a.ncols + 1LL),
+                      vec(a.weight, a.ncols), vec(a.lse_in, a.ncols), vec(a.loss, a.ncols, true), vec(a.lse, a.ncols, true),
+                      dense(a.dZ, size, a.nrows, a.ncols, a.lddz, true)}))
+        return kInvalid;
     return (int)bm::distill(a, s);
 }
 }  // namespace
@@ -146,5 +159,9 @@ API int bidmat_dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, 
     if (k < 0 || ncols < 0 || nnz < 0 || !group_ok(group) || (beta != 0 && beta != 1)) return kInvalid;
     if (k == 0 || ncols == 0) return 0;
     if (ldq < k || !Sjc || !C || (nnz > 0 && (!Q || !scales || !Sdata || !Sir))) return kInvalid;
+    // (the columns of A are not counted in the call: only its first one is known to be there)
+    if (!operands_ok({dense(Q, 1, k, 1, ldq), vec(scales, 1), vec(Sdata, nnz), vec(Sir, nnz), vec(Sjc, ncols + 1LL),
+                      dense(C, sizeof(float), k, ncols, k, true)}))
+        return kInvalid;
     return (int)bm::dsmult_q8_csc(k, ncols, nnz, Q, ldq, scales, group, Sdata, Sir, Sjc, C, beta, as_stream(stream));
 }

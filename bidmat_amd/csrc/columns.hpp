@@ -10,6 +10,9 @@ constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTop = 64;
 constexpr int kRouteMaxGroups = 64;
 
+// A launch may not hold 2^32 threads: kernels with a grid over the columns take at most so many columns at once.
+constexpr int kSlabColumns = 1 << 21;
+
 struct NormArgs {
     int nrows, ncols, type;
     const void *X, *R;                   // R nullable

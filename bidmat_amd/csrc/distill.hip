@@ -22,6 +22,7 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // workgroup of its own takes about 20 us, and below this many columns the chunks win (131072 bf16 rows: 64 columns 22 us
 // against 17, 128 columns 24 against 22, 256 columns 33 against 45).
 constexpr int kColumnsMin = 160;
+constexpr long long kSlabParts = 1 << 22;      // workgroups of one launch, at most
 constexpr int kRowsKept = 512;         // teacher rows of a column that a workgroup keeps in LDS
 
 // Differences of logits are taken before they are scaled: a mask of the type's lowest value stays finite, and large
@@ -421,8 +422,22 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
     while (chunk > BM_BLOCK * 8 && (long long)a.ncols * ((a.nrows + chunk - 1) / chunk) < 1024) chunk >>= 1;
     const int nchunks = (a.nrows + chunk - 1) / chunk;
     const long long nparts = (long long)nchunks * a.ncols;
+    if (a.ncols > 1 && nparts + a.ncols > kSlabParts) {          // halves, until a launch holds them
+        DistillArgs x = a, y = a;
+        const long long half = a.ncols / 2, size = sizeof(T);
+        x.ncols = (int)half;
+        y.ncols = a.ncols - (int)half;
+        y.Z = (const char*)a.Z + half * a.ldz * size;
+        y.tjc += half;
+        if (a.weight) y.weight += half;
+        if (a.lse_in) y.lse_in += half;
+        if (a.loss) y.loss += half;
+        if (a.lse) y.lse += half;
+        if (a.dZ) y.dZ = (char*)a.dZ + half * a.lddz * size;
+        const hipError_t e = distill_typed<T>(x, s);
+        return e != hipSuccess ? e : distill_typed<T>(y, s);
+    }
     if (a.lse_in != nullptr && a.dZ != a.Z) {
-        if (nparts > 0x7fffffffLL) return hipErrorInvalidValue;
         hipLaunchKernelGGL((k_distill_grad<T, true>), dim3((unsigned)nparts), dim3(BM_BLOCK + 64), 0, s, a, nchunks, chunk, nullptr, nullptr, nullptr);
         return hipGetLastError();
     }
@@ -436,7 +451,6 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
     LogSum* parts = (LogSum*)(buf + sizeof(Teacher) * (size_t)a.ncols);
     const int waves = (a.ncols + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK;
     const long long first = a.lse_in != nullptr ? waves : nparts + waves;
-    if (first > 0x7fffffffLL || nparts > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_distill_parts<T>), dim3((unsigned)first), dim3(BM_BLOCK), 0, s, a, a.lse_in != nullptr ? 0 : nchunks, chunk, parts,
                        stats, at);
     if (a.dZ != nullptr)

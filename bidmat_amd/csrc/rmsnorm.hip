@@ -63,7 +63,7 @@ __device__ __forceinline__ float lanes_allmax(float x, int lanes) {
 template <class T, int TPC, int NV>
 __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
     constexpr int CPB = norm_block(TPC) / TPC;
-    __shared__ float sh[2][TPC > 64 ? TPC / 64 : 1];
+    __shared__ float sh[3][TPC > 64 ? TPC / 64 : 1];
     const long long c = (long long)blockIdx.x * CPB + threadIdx.x / TPC;
     if (c >= a.ncols) return;
     const int t = threadIdx.x % TPC, n = a.nrows;
@@ -86,7 +86,14 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
     }
     if (a.Y == nullptr && a.Q == nullptr) return;
     ss = column_allsum<TPC>(ss, sh[0]);
-    const float rs = 1.f / sqrtf(ss / (float)n + a.eps);
+    float rs = 1.f / sqrtf(ss / (float)n + a.eps);
+    if (ss == INFINITY) {
+        // squares beyond fp32: the same from h * 2^-64, where eps is nothing (an infinite h leaves rs = 0)
+        float small = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) small += square_sum(h[v] * 0x1p-64f);
+        rs = 0x1p-64f / sqrtf(column_allsum<TPC>(small, sh[2]) / (float)n);
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const float8_t w = load_col8(a.w, (v * TPC + t) * 8, n).wide();
@@ -131,7 +138,7 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 template <class T, int TPC, int NV>
 __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
     constexpr int CPB = norm_block(TPC) / TPC;
-    __shared__ float sh[2][2][TPC > 64 ? TPC / 64 : 1];
+    __shared__ float sh[2][3][TPC > 64 ? TPC / 64 : 1];
     const int t = threadIdx.x % TPC, n = a.nrows;
     float8_t dw[NV];
 #pragma unroll
@@ -172,9 +179,15 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         }
         hh = column_allsum<TPC>(hh, sh[turn][0]);
         gh = column_allsum<TPC>(gh, sh[turn][1]);
+        float rs = 1.f / sqrtf(hh / (float)n + a.eps);
+        if (hh == INFINITY) {          // as in k_rmsnorm
+            float small = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) small += square_sum(hc[v].wide() * 0x1p-64f);
+            rs = 0x1p-64f / sqrtf(column_allsum<TPC>(small, sh[turn][2]) / (float)n);
+        }
         turn ^= 1;
-        const float rs = 1.f / sqrtf(hh / (float)n + a.eps);
-        const float k = rs * rs * (gh / (float)n);
+        const float k = gh / (float)n * rs * rs;
         T* o = (T*)a.dX + c * a.lddx;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -304,7 +317,24 @@ hipError_t by_type(int type, int n, F f) {
 
 }  // namespace
 
-hipError_t rmsnorm(const NormArgs& a, hipStream_t s) { return by_type(a.type, a.nrows, Norm{a, s}); }
+hipError_t rmsnorm(const NormArgs& all, hipStream_t s) {
+    const long long size = (long long)elem_size(all.type), ng = all.group == 0 ? 1 : (all.nrows + all.group - 1) / all.group;
+    for (long long c = 0; c < all.ncols; c += kSlabColumns) {
+        NormArgs a = all;
+        a.ncols = (int)(all.ncols - c < kSlabColumns ? all.ncols - c : kSlabColumns);
+        a.X = (const char*)all.X + c * all.ldx * size;
+        if (all.R) a.R = (const char*)all.R + c * all.ldr * size;
+        if (all.H) a.H = (char*)all.H + c * all.ldh * size;
+        if (all.Y) a.Y = (char*)all.Y + c * all.ldy * size;
+        if (all.Q) {
+            a.Q = all.Q + c * all.ldq;
+            a.scales = all.scales + c * ng;
+        }
+        const hipError_t e = by_type(a.type, a.nrows, Norm{a, s});
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
 
 hipError_t rmsnorm_grad(const NormGradArgs& a, hipStream_t s) {
     const int n = a.nrows;

@@ -953,8 +953,20 @@ hipError_t route_grad_typed(const RouteGradArgs& a, hipStream_t s) {
 }
 }  // namespace
 
-hipError_t route_grad(const RouteGradArgs& a, hipStream_t s) {
-    return a.type == ELEM_F32 ? route_grad_typed<float>(a, s) : a.type == ELEM_F16 ? route_grad_typed<f16_t>(a, s) : route_grad_typed<bf16_t>(a, s);
+hipError_t route_grad(const RouteGradArgs& all, hipStream_t s) {
+    const long long size = (long long)elem_size(all.type);
+    for (long long c = 0; c < all.ncols; c += kSlabColumns) {
+        RouteGradArgs a = all;
+        a.ncols = (int)(all.ncols - c < kSlabColumns ? all.ncols - c : kSlabColumns);
+        a.Z = (const char*)all.Z + c * all.ldz * size;
+        a.dZ = (char*)all.dZ + c * all.lddz * size;
+        a.data = all.data + c * all.topk;
+        a.ir = all.ir + c * all.topk;
+        a.ddata = all.ddata + c * all.topk;
+        const hipError_t e = a.type == ELEM_F32 ? route_grad_typed<float>(a, s) : a.type == ELEM_F16 ? route_grad_typed<f16_t>(a, s) : route_grad_typed<bf16_t>(a, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace bm

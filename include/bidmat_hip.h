@@ -367,8 +367,9 @@ int bidmat_applyop_flat(const float *A, const float *B, float *C, long long n, i
  *    example, a row a feature, an expert or a word.  Dense matrices are column-major with a leading dimension of their
  *    own (in elements, >= the rows) and hold fp32, fp16 or bf16 elements (`type`); addresses need the alignment of one
  *    element.  Everything is computed and summed in fp32 and rounded to nearest even once, when it is written.  Weights,
- *    scales and values of sparse matrices are fp32.  They only enqueue work on `stream`.  An output may be one of the
- *    call's dense inputs (same address and leading dimension); any other overlap returns hipErrorInvalidValue.
+ *    scales and values of sparse matrices are fp32.  They only enqueue work on `stream`.  A dense output may
+ *    be one of the call's dense inputs of its type (same address and leading dimension); any other overlap of an output
+ *    returns hipErrorInvalidValue.
  * ------------------------------------------------------------------------------------ */
 enum { BIDMAT_F32 = 0, BIDMAT_F16 = 1, BIDMAT_BF16 = 2 };
 enum { BIDMAT_SOFTMAX = 0, BIDMAT_SIGMOID = 1 };
@@ -378,7 +379,8 @@ enum { BIDMAT_SOFTMAX = 0, BIDMAT_SIGMOID = 1 };
  * H (nullable) receives h, Y (nullable) y.  Q and scales (both or neither) receive y in 8 bits: e4m3 codes (OCP, nrows x
  * ncols, leading dimension ldq) and one scale per `group` rows (0 = the column; 32, 64 or 128; the last group of a column
  * may be short; scales is ceil(nrows / group) x ncols): scale = max(largest |y| / 448, 2^-126), code = e4m3(y / scale).
- * y is formed from the unrounded sum.  A NaN or an infinity in a column of h makes its y and codes NaN.
+ * y is formed from the unrounded sum.  In a column of h with a NaN every y and code is NaN,
+ * with an infinity that row's y and code is NaN and the others are 0.
  * nrows <= 32768 (a column stays in the registers of one workgroup). */
 int bidmat_rmsnorm(int nrows, int ncols, int type, const void *X, int ldx, const void *R, int ldr, const float *w,
                    float eps, void *H, int ldh, void *Y, int ldy, unsigned char *Q, int ldq, float *scales, int group,
@@ -463,7 +465,8 @@ int bidmat_host_free(void *hptr);
  * recorded pointers and sizes are fixed; the data they point to may change between replays.
  * A recording also holds the addresses of the stream's scratch buffers and of any plan it used:
  * destroy it (and record again) before a larger problem is run on that stream (scratch grows by
- * reallocation), before the plan is destroyed and before bidmat_release_caches. */
+ * reallocation), before the plan is destroyed and before bidmat_release_caches.  Graphs recorded on one
+ * stream share its scratch: replay them one after the other, not at the same time on two streams. */
 int bidmat_graph_begin_capture(void *stream);
 int bidmat_graph_end_capture(void *stream, void **graph_exec);
 int bidmat_graph_launch(void *graph_exec, void *stream);

@@ -133,6 +133,18 @@ def test_rmsnorm_small_and_large_values(hip):
         norm_case(hip, rng, 300, 6, 0, False, True, True, group, x=x, eps=1e-6)
 
 
+@pytest.mark.parametrize("n", [40, 300, 3000, 9000])
+@pytest.mark.parametrize("t", [0, 2])
+def test_rmsnorm_squares_beyond_single_precision(hip, n, t):
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((5, n))
+    x[1] *= 1e21
+    x[2, 0] = 3e37
+    x[4] *= 1e35
+    norm_case(hip, rng, n, 5, t, False, True, True, 32, x=x)
+    norm_grad_case(hip, rng, n, 5, t, True, H=x)
+
+
 def test_rmsnorm_nan_and_infinity_stay_in_their_columns(hip):
     rng = np.random.default_rng(6)
     n = 200
@@ -163,8 +175,8 @@ def test_rmsnorm_in_place(hip, t, n):
     assert np.array_equal(r.get(), h) and np.array_equal(x.get(), y)
 
 
-def norm_grad_case(hip, rng, n, m, t, with_dh, pad=0, shift=0, beta=0, in_place=False):
-    H, dY = encode(rng.standard_normal((m, n)) * 2, t), encode(rng.standard_normal((m, n)), t)
+def norm_grad_case(hip, rng, n, m, t, with_dh, pad=0, shift=0, beta=0, in_place=False, H=None):
+    H, dY = encode(rng.standard_normal((m, n)) * 2 if H is None else H, t), encode(rng.standard_normal((m, n)), t)
     dH = encode(rng.standard_normal((m, n)), t) if with_dh else None
     w = (1 + 0.1 * rng.standard_normal(n)).astype(F)
     dw0 = rng.standard_normal(n).astype(F)
@@ -482,6 +494,38 @@ def test_distill_large_offsets_cancel(hip):
     """Logits around 1000: the loss is a difference of large numbers that the kernels take before they sum."""
     rng = np.random.default_rng(70)
     distill_case(hip, rng, 3000, 4, 0, [10] * 4, Z=1000 + rng.standard_normal((4, 3000)))
+
+
+@pytest.mark.parametrize("V", [70, 5000, 140000])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
+def test_distill_masks_of_the_lowest_value(hip, V, t, tau):
+    """Masked logits hold the type's most negative number: some rows, a column but one row, the teacher's too. A column of
+    nothing else has the uniform softmax: its loss and gradient are finite, q is 1 / V."""
+    rng = np.random.default_rng(V)
+    low = {0: -3.4028234663852886e38, 1: -65504.0, 2: -3.3895313892515355e38}[t]
+    m, k = 5, 9
+    z = rng.standard_normal((m, V))
+    T, ir, jc = teacher(rng, V, [k] * m)
+    z[1, rng.choice(V, V // 2, replace=False)] = low
+    z[1, ir[k:2 * k]] = 1.0
+    z[2] = low
+    z[2, ir[2 * k]] = 0.5
+    T[2 * k + 1:3 * k] = np.float32(-3.4e38)
+    T[3 * k:4 * k - 1] = np.float32(-3.4e38)
+    z[4] = low
+    T[4 * k:5 * k] = np.float32(-3.4e38)
+    for in_place in (False, True):
+        loss, lse, dZ = distill_case_raw(hip, z, T, ir, jc, t, np.ones(m), in_place, tau)
+        want, _, wd, eloss, ez = ref.distill(decode(encode(z, t), t)[:4], T, ir, jc[:5], tau, np.ones(4))
+        within(loss[:4], want, eloss + 160 * EPS24 * np.abs(want), "loss")
+        within(dZ[:4], wd, HALF_STEP[t] * 1.01 * np.abs(wd) + TINY[t] + ez, "dz")
+        # the uniform column: q = 1 / V, p = 1 / k
+        share = np.zeros(V)
+        share[ir[4 * k:]] = 1 / k
+        u = tau * (1 / V - share)
+        within(dZ[4], u, HALF_STEP[t] * 1.01 * np.abs(u) + TINY[t] + 200 * EPS24 * tau * (1 / V + share), "uniform dz")
+        assert abs(loss[4] - tau * tau * np.log(V / k)) <= 200 * EPS24 * tau * tau * (np.log(V) + np.log(k) + 1)
 
 
 def test_distill_against_differences(hip):
