@@ -686,6 +686,82 @@ GSMatP GSMat::DDS(const GMatP& A, const GMatP& B, const GSMatP& C, GSMatP oldmat
     return out;
 }
 
+// ------------------------------------------------------------------ operators over a model's columns
+namespace {
+const float* devptr(const GMatP& a) { return a ? a->pdata : nullptr; }
+void sameShape(const GMat& a, const GMatP& b, const char* what) {
+    if (b && (b->nrows != a.nrows || b->ncols != a.ncols)) fail(fmt("%s dimensions mismatch (%d %d) (%d %d)", what, a.nrows, a.ncols, b->nrows, b->ncols));
+}
+void vectorOf(const GMatP& v, long long n, const char* what) {
+    if (v && v->length() != n) fail(fmt("%s: a vector of %lld is wanted, not %d x %d", what, n, v->nrows, v->ncols));
+}
+void finished(int err, const char* what) {
+    if (err == 0) err = bidmat_stream_synchronize(nullptr);
+    if (err != 0) fail(std::string("HIP error in ") + what + " " + bidmat_error_string(err));
+}
+}  // namespace
+
+GMatP GMat::rmsnorm(const GMatP& w, float eps, const GMatP& residual, GMatP oldmat, GMatP* h) {
+    if (!w) fail("GMat.rmsnorm: no weights");
+    vectorOf(w, nrows, "GMat.rmsnorm");
+    sameShape(*this, residual, "GMat.rmsnorm");
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, residual ? residual->GUID : 0, opHash("rmsnorm"));
+    if (h) *h = newOrCheckGMat(nrows, ncols, *h, GUID, residual ? residual->GUID : 0, opHash("rmsnorm sum"));
+    Mat::nflops += 4LL * length();
+    finished(bidmat_rmsnorm(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(residual), nrows, w->pdata, eps, h ? (*h)->pdata : nullptr, nrows,
+                            out->pdata, nrows, nullptr, nrows, nullptr, 0, nullptr), "GMat.rmsnorm");
+    return out;
+}
+
+GMatP GMat::rmsnormGrad(const GMatP& w, float eps, const GMatP& dy, const GMatP& dh, const GMatP& dw, GMatP oldmat) {
+    if (!w || !dy) fail("GMat.rmsnormGrad: no weights or no gradient");
+    vectorOf(w, nrows, "GMat.rmsnormGrad");
+    vectorOf(dw, nrows, "GMat.rmsnormGrad");
+    sameShape(*this, dy, "GMat.rmsnormGrad");
+    sameShape(*this, dh, "GMat.rmsnormGrad");
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dy->GUID, opHash("rmsnormGrad"));
+    Mat::nflops += 10LL * length();
+    finished(bidmat_rmsnorm_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, w->pdata, eps, dy->pdata, nrows, devptr(dh), nrows, out->pdata, nrows,
+                                 dw ? dw->pdata : nullptr, 1, nullptr), "GMat.rmsnormGrad");
+    return out;
+}
+
+GSMatP GMat::route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, int topk, bool renorm, float scale, GSMatP oldmat) {
+    vectorOf(bias, nrows, "GMat.route");
+    if (topk < 1 || (long long)ncols * topk > 0x7fffffffLL) fail(fmt("GMat.route: %d of %d experts for %d columns", topk, nrows, ncols));
+    const int nnz = ncols * topk;
+    GSMatP out = GSMat::newOrCheckGSMat(nrows, ncols, nnz, nnz, oldmat, GUID, bias ? bias->GUID : 0, topk,
+                                        opHash(fmt("route %d %d %d %d %g", sigmoid, ngroups, topgroups, renorm, scale).c_str()));
+    out->nnz0 = nnz;
+    out->ownPattern();                                     // new indices: nothing shared, any older plan is stale
+    Mat::nflops += 6LL * length();
+    finished(bidmat_route(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(bias), sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, ngroups, topgroups,
+                          topk, renorm, scale, out->pdata, out->pir, out->pic, out->pjc, nullptr, nullptr), "GMat.route");
+    return out;
+}
+
+GMatP GMat::routeGrad(const GSMatP& gate, const GSMatP& dgate, bool sigmoid, bool renorm, float scale, GMatP oldmat) {
+    if (!gate || !dgate || gate->nrows != nrows || gate->ncols != ncols || dgate->nnz() != gate->nnz())
+        fail("GMat.routeGrad dimensions mismatch");
+    if (ncols == 0 || gate->nnz() % ncols != 0) fail("GMat.routeGrad: the gate's columns differ in length");
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dgate->GUID, opHash("routeGrad"));
+    Mat::nflops += 6LL * length();
+    finished(bidmat_route_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, gate->nnz() / ncols, renorm,
+                               scale, gate->pdata, gate->pir, dgate->pdata, out->pdata, nrows, nullptr), "GMat.routeGrad");
+    return out;
+}
+
+GMatP GMat::distill(const GSMatP& teacher, float temperature, const GMatP& weight, const GMatP& grad, GMatP oldmat) {
+    if (!teacher || teacher->nrows != nrows || teacher->ncols != ncols) fail("GMat.distill dimensions mismatch");
+    vectorOf(weight, ncols, "GMat.distill");
+    sameShape(*this, grad, "GMat.distill");
+    GMatP out = newOrCheckGMat(1, ncols, oldmat, GUID, teacher->GUID, opHash("distill"));
+    Mat::nflops += 8LL * length();
+    finished(bidmat_distill(nrows, ncols, BIDMAT_F32, pdata, nrows, teacher->nnz(), teacher->pdata, teacher->pir, teacher->pjc, temperature,
+                            devptr(weight), out->pdata, nullptr, grad ? grad->pdata : nullptr, nrows, nullptr), "GMat.distill");
+    return out;
+}
+
 GSMatP GSMat::withValues(const GMatP& vals) const {
     if (vals->length() != nnz0) fail(fmt("withValues: %lld values for %d nonzeros", vals->length(), nnz0));
     GSMatP out = std::make_shared<GSMat>(nrows, ncols, nnz0, realnnz, *this);      // same index arrays, same plan

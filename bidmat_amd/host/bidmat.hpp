@@ -135,6 +135,19 @@ public:
     GMatP gOp(const GMatP& a, GMatP oldmat, int op);
     GMatP reduceOp(GMatP oldmat, int dir, float initval, int op);
 
+    // Operators over a model's columns (no counterpart in the reference); every optional matrix may be null.
+    // y = w * h / sqrt(mean(h^2) + eps) per column, h = this + residual; *h (optional) receives h
+    GMatP rmsnorm(const GMatP& w, float eps, const GMatP& residual, GMatP oldmat, GMatP* h = nullptr);
+    // this = h: the gradient with respect to this matrix (and the residual) from dy and, optional, dh; dw (optional, like w) += w's
+    GMatP rmsnormGrad(const GMatP& w, float eps, const GMatP& dy, const GMatP& dh, const GMatP& dw, GMatP oldmat);
+    // this = scores (experts x columns): a sparse matrix of weights, topk rows per column; sigmoid: kind of the scores
+    GSMatP route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, int topk, bool renorm, float scale, GSMatP oldmat);
+    // this = scores: their gradient from dgate, the gradient of gate's values (a GSMat with gate's pattern, as DDS returns it)
+    GMatP routeGrad(const GSMatP& gate, const GSMatP& dgate, bool sigmoid, bool renorm, float scale, GMatP oldmat);
+    // this = student logits: the loss of every column (1 x ncols) against the teacher's stored logits; grad (optional, like
+    // this) receives the gradient, weight (optional) holds one factor per column
+    GMatP distill(const GSMatP& teacher, float temperature, const GMatP& weight, const GMatP& grad, GMatP oldmat);
+
     static GMatP newOrCheckGMat(int nr, int nc, GMatP outmat);
     static GMatP newOrCheckGMat(int nr, int nc, GMatP outmat, long long g1, long long g2, long long opHash);
 };

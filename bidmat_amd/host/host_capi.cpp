@@ -110,6 +110,27 @@ API void* bmh_reduce(void* a, void* out, int dir, float initv, int op) {
     return guard_ptr([&] { return wrap(G(a)->reduceOp(G(out), dir, initv, op)); });
 }
 API void* bmh_gop(void* a, void* b, void* out, int op) { return guard_ptr([&] { return wrap(G(a)->gOp(G(b), G(out), op)); }); }
+// h_out (nullable): receives a handle of the sum h
+API void* bmh_rmsnorm(void* a, void* w, float eps, void* res, void* out, void** h_out) {
+    return guard_ptr([&] {
+        GMatP h;
+        GMatP y = G(a)->rmsnorm(G(w), eps, G(res), G(out), h_out ? &h : nullptr);
+        if (h_out) *h_out = wrap(h);
+        return wrap(y);
+    });
+}
+API void* bmh_rmsnorm_grad(void* h, void* w, float eps, void* dy, void* dh, void* dw, void* out) {
+    return guard_ptr([&] { return wrap(G(h)->rmsnormGrad(G(w), eps, G(dy), G(dh), G(dw), G(out))); });
+}
+API void* bmh_route(void* z, void* bias, int sigmoid, int ngroups, int topgroups, int topk, int renorm, float scale, void* out) {
+    return guard_ptr([&] { return wrap(G(z)->route(G(bias), sigmoid != 0, ngroups, topgroups, topk, renorm != 0, scale, S(out))); });
+}
+API void* bmh_route_grad(void* z, void* gate, void* dgate, int sigmoid, int renorm, float scale, void* out) {
+    return guard_ptr([&] { return wrap(G(z)->routeGrad(S(gate), S(dgate), sigmoid != 0, renorm != 0, scale, G(out))); });
+}
+API void* bmh_distill(void* z, void* teacher, float temperature, void* weight, void* grad, void* out) {
+    return guard_ptr([&] { return wrap(G(z)->distill(S(teacher), temperature, G(weight), G(grad), G(out))); });
+}
 API void* bmh_contents(void* s) { return guard_ptr([&] { return wrap(S(s)->contents()); }); }
 API void* bmh_with_values(void* s, void* vals) { return guard_ptr([&] { return wrap(S(s)->withValues(G(vals))); }); }
 

@@ -8,6 +8,7 @@ only moves handles around.
     sum(s, n), sum(a, n)                     (SFunctions.scala:10-15, GFunctions.scala:227)
     a / b            elementwise             (GMat.scala:1681)
     c.madd / c.maddT via out=...             (the `c ~ a * b` output-reuse form)
+    a.rmsnorm, a.route, a.distill            operators over a model's columns, with their gradients
 """
 import ctypes as C
 import os
@@ -31,8 +32,14 @@ def _load():
         L = C.CDLL(LIB_PATH)
         for name in ("bmh_gmat_from_host", "bmh_gmat_zeros", "bmh_gsmat_from_host", "bmh_mult", "bmh_madd",
                      "bmh_multT", "bmh_maddT", "bmh_dds", "bmh_sum_sparse", "bmh_sum_dense", "bmh_reduce",
-                     "bmh_gop", "bmh_contents", "bmh_with_values", "bmh_tile_mult", "bmh_sdmult", "bmh_gsdop", "bmh_load_gsmat", "bmh_colslice", "bmh_nhot", "bmh_full", "bmh_t"):
+                     "bmh_gop", "bmh_contents", "bmh_with_values", "bmh_tile_mult", "bmh_sdmult", "bmh_gsdop", "bmh_load_gsmat", "bmh_colslice", "bmh_nhot", "bmh_full", "bmh_t",
+                     "bmh_rmsnorm", "bmh_rmsnorm_grad", "bmh_route", "bmh_route_grad", "bmh_distill"):
             getattr(L, name).restype = vp
+        L.bmh_rmsnorm.argtypes = [vp, vp, C.c_float, vp, vp, C.POINTER(vp)]
+        L.bmh_rmsnorm_grad.argtypes = [vp, vp, C.c_float, vp, vp, vp, vp]
+        L.bmh_route.argtypes = [vp, vp] + [C.c_int] * 5 + [C.c_float, vp]
+        L.bmh_route_grad.argtypes = [vp, vp, vp, C.c_int, C.c_int, C.c_float, vp]
+        L.bmh_distill.argtypes = [vp, vp, C.c_float, vp, vp, vp]
         L.bmh_gmat_from_host.argtypes = [C.c_int, C.c_int, vp]
         L.bmh_gmat_zeros.argtypes = [C.c_int, C.c_int]
         L.bmh_gsmat_from_host.argtypes = [C.c_int, C.c_int, C.c_int, vp, vp, vp]
@@ -88,6 +95,10 @@ def _ok(h):
     if not h:
         raise RuntimeError(_load().bmh_last_error().decode())
     return h
+
+
+def _handle(m):
+    return m._h if m is not None else None
 
 
 class Mat:
@@ -203,6 +214,29 @@ class GMat(_Handle):
 
     def reduceOp(self, dir, initv, op, out=None):
         return GMat(_load().bmh_reduce(self._h, out._h if out else None, dir, initv, op))
+
+    # operators over a model's columns (the formulas stand with bidmat_rmsnorm, bidmat_route, bidmat_distill)
+    def rmsnorm(self, w, eps=1e-5, residual=None, out=None):
+        """(y, h): h = self + residual, y its normalised columns times w."""
+        h = vp()
+        y = GMat(_load().bmh_rmsnorm(self._h, w._h, eps, _handle(residual), _handle(out), C.byref(h)))
+        return y, GMat(h.value)
+
+    def rmsnormGrad(self, w, dy, eps=1e-5, dh=None, dw=None, out=None):
+        """self = h: the gradient with respect to what was added; dw (a GMat like w) receives += w's gradient."""
+        return GMat(_load().bmh_rmsnorm_grad(self._h, w._h, eps, dy._h, _handle(dh), _handle(dw), _handle(out)))
+
+    def route(self, topk, bias=None, sigmoid=False, ngroups=1, topgroups=1, renorm=True, scale=1.0, out=None):
+        """self = scores, experts x columns: the sparse matrix of weights, topk rows in every column."""
+        return GSMat(_load().bmh_route(self._h, _handle(bias), int(sigmoid), ngroups, topgroups, topk, int(renorm), scale, _handle(out)))
+
+    def routeGrad(self, gate, dgate, sigmoid=False, renorm=True, scale=1.0, out=None):
+        """self = scores: their gradient from dgate, the gradient of gate's values (DDS(a, b, gate), for one)."""
+        return GMat(_load().bmh_route_grad(self._h, gate._h, dgate._h, int(sigmoid), int(renorm), scale, _handle(out)))
+
+    def distill(self, teacher, temperature=1.0, weight=None, grad=None, out=None):
+        """self = student logits: the loss per column against a sparse teacher; grad (a GMat like self) receives the gradient."""
+        return GMat(_load().bmh_distill(self._h, teacher._h, temperature, _handle(weight), _handle(grad), _handle(out)))
 
 
 class GSMat(_Handle):

@@ -707,3 +707,82 @@ def test_two_threads_on_streams_of_their_own(hip):
     for t in threads:
         t.join()
     assert not failed, failed[0]
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+def _last(dev_ptr, first, count, dtype):
+    out = np.empty(count, dtype)
+    ok(hip_abi.load().bidmat_memcpy_d2h(out.ctypes.data, dev_ptr + first * out.itemsize, out.nbytes))
+    return out
+
+
+def _tail(dev_ptr, first, a):
+    ok(hip_abi.load().bidmat_memcpy_h2d(dev_ptr + first * a.itemsize, np.ascontiguousarray(a).ctypes.data, a.nbytes))
+
+
+def test_rmsnorm_offsets_past_32_bits(hip):
+    rng = np.random.default_rng(90)
+    n, m = 32768, 65600                                  # 2.15e9 elements
+    X, Y, Q, S, dw = DeviceArray.zeros(n * m, np.uint16), DeviceArray(n * m, np.uint16), DeviceArray(n * m, np.uint8), DeviceArray(m, F), DeviceArray(n, F)
+    last = encode(rng.standard_normal((2, n)), 2)
+    _tail(X.ptr, n * (m - 2), last)
+    w = dev(np.ones(n, F))
+    ok(hip.bidmat_rmsnorm(n, m, 2, X.ptr, n, None, n, w.ptr, 1e-5, None, n, Y.ptr, n, Q.ptr, n, S.ptr, 0, None))
+    h, y, s = ref.rmsnorm(decode(last, 2), None, np.ones(n), float(F(1e-5)), 0)
+    got = decode(_last(Y.ptr, n * (m - 2), 2 * n, np.uint16).reshape(2, n), 2)
+    within(got, y, (HALF_STEP[2] * 1.01 + NORM_DEPTH * EPS24) * np.abs(y) + TINY[2], "y")
+    q = ref.E4M3[_last(Q.ptr, n * (m - 2), 2 * n, np.uint8).reshape(2, n)] * _last(S.ptr, m - 2, 2, F)[:, None]
+    within(q, y, np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** -10 * s) * 1.01, "codes")
+    ok(hip.bidmat_rmsnorm_grad(n, m, 2, X.ptr, n, w.ptr, 1e-5, Y.ptr, n, None, n, Y.ptr, n, dw.ptr, 0, None))
+    want, wantw, size, sizew = ref.rmsnorm_grad(decode(last, 2), np.ones(n), float(F(1e-5)), got, None)
+    within(decode(_last(Y.ptr, n * (m - 2), 2 * n, np.uint16).reshape(2, n), 2), want,
+           HALF_STEP[2] * 1.01 * np.abs(want) + TINY[2] + 2 * NORM_DEPTH * EPS24 * size, "dx")
+    within(dw.numpy().astype(np.float64), wantw, 400 * EPS24 * sizew, "dw")         # the other columns are zeros
+
+
+def test_route_and_distill_offsets_past_32_bits(hip):
+    rng = np.random.default_rng(91)
+    V, m, k = 131072, 16500, 8                           # 2.16e9 elements
+    Z, loss = DeviceArray.zeros(V * m, np.uint16), DeviceArray(m, F)
+    last = encode(rng.standard_normal((2, V)) * 2, 2)
+    _tail(Z.ptr, V * (m - 2), last)
+    T, ir, jc = teacher(rng, V, [k, k])
+    full_jc = np.concatenate([np.zeros(m - 2, np.int32), jc]).astype(np.int32)
+    dT, di, dj = dev(T), dev(ir), dev(full_jc)
+    ok(hip.bidmat_distill(V, m, 2, Z.ptr, V, 2 * k, dT.ptr, di.ptr, dj.ptr, 1.0, None, loss.ptr, None, Z.ptr, V, None))
+    want, _, wd, eloss, ez = ref.distill(decode(last, 2), T, ir, jc, 1.0, None)
+    within(_last(loss.ptr, m - 2, 2, F).astype(np.float64), want, eloss + 160 * EPS24 * np.abs(want), "loss")
+    within(decode(_last(Z.ptr, V * (m - 2), 2 * V, np.uint16).reshape(2, V), 2), wd, HALF_STEP[2] * 1.01 * np.abs(wd) + TINY[2] + ez, "dz")
+    # the same memory as the scores of 1024 experts
+    E, m = 1024, V * m // 1024
+    ok(hip.bidmat_memset(Z.ptr, 0, V * 16500 * 2))
+    z = encode(rng.standard_normal((3, E)), 2)
+    _tail(Z.ptr, E * (m - 3), z)
+    G, ir_, cnt = DeviceArray(m * k, F), DeviceArray(m * k, np.int32), DeviceArray(E, np.int32)
+    ok(hip.bidmat_route(E, m, 2, Z.ptr, E, None, 0, 1, 1, k, 0, 1.0, G.ptr, ir_.ptr, None, None, cnt.ptr, None))
+    wi, ww, _ = ref.route(decode(z, 2), None, 0, 1, 1, k, False, 1.0)
+    assert np.array_equal(_last(ir_.ptr, k * (m - 3), 3 * k, np.int32).reshape(3, k), wi)
+    within(_last(G.ptr, k * (m - 3), 3 * k, F).astype(np.float64).reshape(3, k), ww, 80 * EPS24 * ww, "weights")
+    assert int(cnt.numpy().astype(np.int64).sum()) == m * k and np.array_equal(_last(ir_.ptr, 0, k, np.int32), np.arange(k))
+    dG = DeviceArray.zeros(m * k, F)
+    d = rng.standard_normal((3, k)).astype(F)
+    _tail(dG.ptr, k * (m - 3), d)
+    ok(hip.bidmat_route_grad(E, m, 2, Z.ptr, E, 0, k, 0, 1.0, G.ptr, ir_.ptr, dG.ptr, Z.ptr, E, None))
+    wd, size = ref.route_grad(decode(z, 2), 0, False, 1.0, ww, wi, d)
+    within(decode(_last(Z.ptr, E * (m - 3), 3 * E, np.uint16).reshape(3, E), 2), wd, HALF_STEP[2] * 1.01 * np.abs(wd) + TINY[2] + 200 * EPS24 * size, "dz")
+
+
+def test_dsmult_q8_offsets_past_32_bits(hip):
+    rng = np.random.default_rng(92)
+    k, rows = 1024, 2100500                              # 2.15e9 codes
+    Q, S = DeviceArray.zeros(k * rows, np.uint8), DeviceArray.zeros(8 * rows, F)
+    codes = rng.integers(0, 0x7F, (2, k)).astype(np.uint8)
+    sc = (0.01 + rng.random((2, 8))).astype(F)
+    _tail(Q.ptr, k * (rows - 2), codes)
+    _tail(S.ptr, 8 * (rows - 2), sc)
+    v, ir, jc = np.array([2, -1, 3], F), np.array([rows - 1, 0, rows - 2], np.int32), np.array([0, 2, 3], np.int32)
+    a, b, c, out = dev(v), dev(ir), dev(jc), empty(2, k, np.float32)
+    ok(hip.bidmat_dsmult_q8_csc(k, 2, 3, Q.ptr, k, S.ptr, 128, a.ptr, b.ptr, c.ptr, out.ptr, 0, None))
+    A = ref.E4M3[codes] * np.repeat(sc.astype(np.float64), 128, 1)
+    want = np.stack([2 * A[1], 3 * A[0]])
+    within(out.get().astype(np.float64), want, 4 * EPS24 * np.abs(want), "C")
