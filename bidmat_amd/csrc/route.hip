@@ -33,6 +33,7 @@ struct Deal {            // how a column's experts lie in the lanes
     int each;            // experts per lane
     int kp;              // topk rounded up to a power of two: lanes per column when the weights are written
     int batch;           // columns whose weights a wave writes together
+    bool halves;         // 16 lanes per column: the open groups take at most eight of them
 };
 
 template <class V>
@@ -280,15 +281,27 @@ __device__ __forceinline__ bool take_fast(const RouteArgs& a, const Deal& d, con
     return true;
 }
 
-// Sum / largest over aligned groups of n lanes, n a power of two known at run time.
+// Sum / largest over aligned groups of n lanes, n a power of two known at run time (steps of group_allsum).
 __device__ __forceinline__ float lanes_sum_rt(float x, int n) {
-    for (int m = 1; m < n; m <<= 1) x += __shfl_xor(x, m, 64);
+    if (n >= 2) x += dpp_mov<DPP_QUAD_XOR1>(x);
+    if (n >= 4) x += dpp_mov<DPP_QUAD_XOR2>(x);
+    if (n >= 8) x += dpp_mov<DPP_ROW_HALF_MIRROR>(x);
+    if (n >= 16) x += dpp_mov<DPP_ROW_MIRROR>(x);
+    if (n >= 32) x += __shfl_xor(x, 16, 64);
+    if (n >= 64) x += __shfl_xor(x, 32, 64);
     return x;
 }
 __device__ __forceinline__ float lanes_max_rt(float x, int n) {
-    for (int m = 1; m < n; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
+    if (n >= 2) x = fmaxf(x, dpp_mov<DPP_QUAD_XOR1>(x));
+    if (n >= 4) x = fmaxf(x, dpp_mov<DPP_QUAD_XOR2>(x));
+    if (n >= 8) x = fmaxf(x, dpp_mov<DPP_ROW_HALF_MIRROR>(x));
+    if (n >= 16) x = fmaxf(x, dpp_mov<DPP_ROW_MIRROR>(x));
+    if (n >= 32) x = fmaxf(x, __shfl_xor(x, 16, 64));
+    if (n >= 64) x = fmaxf(x, __shfl_xor(x, 32, 64));
     return x;
 }
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x)); }
 
 constexpr int kRouteBatch = 8;           // columns whose weights one wave writes together, at most
 struct Chosen {                          // of one wave
@@ -313,12 +326,12 @@ __device__ __forceinline__ void write_weights(const RouteArgs& a, const Deal& d,
             const float high = lanes_max_rt(z, d.kp);
             // Far below 0 sigmoid(z) is exp(z) to within a factor 1 + exp(z): with all taken scores below -30 their
             // shares are a softmax's, where the sigmoids themselves may have left the range of fp32.
-            p = a.kind == 0 || high < -30.f ? expf(z - high) : 1.f / (1.f + expf(-z));
+            p = a.kind == 0 || high < -30.f ? exp_of(z - high) : sigmoid_of(z);
             p = valid ? p : 0.f;
             const float sum = lanes_sum_rt(p, d.kp);
-            p = sum > 0.f ? p * (a.scale / sum) : 0.f;
+            p = sum > 0.f ? p * (a.scale * __builtin_amdgcn_rcpf(sum)) : 0.f;
         } else {
-            p = a.scale * (a.kind == 0 ? expf(z - top) * by : 1.f / (1.f + expf(-z)));
+            p = a.scale * (a.kind == 0 ? exp_of(z - top) * by : sigmoid_of(z));
             p = valid ? p : 0.f;
         }
         if (on) {
@@ -528,7 +541,7 @@ __device__ __forceinline__ void row_before(int key, int& before) {
 // order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
 template <class T, int VPL>
 __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, const float (&z)[VPL], const float (&bias)[VPL], float bmax,
-                                             float top, float by, int first, bool shut, bool& fine) {
+                                             float top, float by, int first, bool shut, int* sixteen, bool& fine) {
     const bool plain = a.bias == nullptr && a.ngroups == 1;
     int key[VPL];
     if (plain) {
@@ -582,7 +595,7 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
         }
         const bool in = reach < a.topgroups, out = pass >= a.topgroups;
         if (b1 != kShut && !in && !out) fine = false;
-        if (!in) {
+        if (!in || b1 == kShut) {
             best = second = kShut;
 #pragma unroll
             for (int j = 0; j < VPL; ++j) key[j] = kShut;
@@ -594,7 +607,23 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     hi = hi == kShut ? kShut + 2 : hi + 1;
     {
         bool enough;
-        if (__ballot(row_sum(best != kShut) < 2 * want) == 0) {
+        if (d.halves) {
+            // at most eight lanes are open: their two largest keys fit the sixteen lanes, one each
+            const bool mine = best != kShut;
+            const int i = threadIdx.x & 15, at = row_prefix(mine) - 1;
+            sixteen[i] = kShut;
+            __builtin_amdgcn_wave_barrier();          // a wave's LDS operations take effect in order
+            if (mine && at < 8) {
+                sixteen[at] = best;
+                sixteen[8 + at] = second;
+            }
+            __builtin_amdgcn_wave_barrier();
+            const int key16 = sixteen[i];
+            int before = 0;
+            row_before<1>(key16, before);
+            enough = row_sum(key16 != kShut) >= want;
+            lo = row_min(before < want && key16 != kShut ? key16 : INT_MAX);
+        } else if (__ballot(row_sum(best != kShut) < 2 * want) == 0) {
             // open keys in twice as many lanes as keys are wanted: few lanes hold two of them, so that the want-th of the lanes'
             // largest keys is close to the border, and on its far side
             int before = 0;
@@ -659,6 +688,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
     constexpr int WAVES = BM_WAVES_PER_BLOCK;
     __shared__ int hist[256];
     __shared__ Chosen chosen[WAVES];
+    __shared__ int two_largest[WAVES][4][16];
     extern __shared__ double exact_keys[];      // 64 * d64.each per wave
     if (a.counts != nullptr) {
         for (int e = threadIdx.x; e < a.nexperts; e += BM_BLOCK) hist[e] = 0;
@@ -707,18 +737,21 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
             }
             // a NaN anywhere, or +inf where the softmax has no value
             unsigned size = 0;
-            float high = z[0], low = z[0];
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                size = max(size, (unsigned)__float_as_int(z[j]) & 0x7fffffffu);
-                low = fminf(low, z[j]);
-                high = fmaxf(high, z[j]);
+            for (int j = 0; j < VPL; ++j) size = max(size, (unsigned)__float_as_int(z[j]) & 0x7fffffffu);
+            const bool shut = __ballot(size >= 0x7f800000u) != 0;          // some infinity: of -inf, where all is well
+            bool odd = size > 0x7f800000u;
+            if (shut && a.kind == 0) {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) odd = odd || z[j] == INFINITY;
             }
-            const bool bad = row_sum(size > 0x7f800000u || (a.kind == 0 && high == INFINITY)) != 0;
-            const bool shut = __ballot(low == -INFINITY) != 0;
+            const bool bad = shut && row_sum(odd) != 0;
             float top = 0.f, by = 1.f;
             if (sums) {
-                top = group_allmax<16>(high);
+                top = z[0];
+#pragma unroll
+                for (int j = 1; j < VPL; ++j) top = fmaxf(top, z[j]);
+                top = group_allmax<16>(top);
                 const float from = top > -INFINITY ? top : 0.f;
                 float sum = 0.f;
 #pragma unroll
@@ -727,7 +760,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
                 by = sum > 0.f ? 1.f / sum : 0.f;
             }
             bool fine;
-            unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, shut, fine);
+            unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, shut, two_largest[wave][row], fine);
             if (bad) { taken = 0; fine = true; }
             // fewer than topk open: the lowest others fill the column
             const unsigned valid = taken;
@@ -909,6 +942,7 @@ Deal deal(const RouteArgs& a, int lanes) {
     d.each = d.lanes > 0 ? (d.size + d.lanes - 1) / d.lanes : INT_MAX;
     d.kp = pow2ceil(a.topk);
     d.batch = 1;
+    d.halves = a.topgroups * d.lanes <= 8;
     return d;
 }
 
