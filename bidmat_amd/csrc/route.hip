@@ -365,13 +365,15 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d, int* share
     const int first = g * d.size + o;
     const int room = d.size - o < d.each ? d.size - o : d.each;
     const int own = g < a.ngroups && room > 0 ? room : 0;              // experts of this lane
-    float bias[VPL], bmax = 0.f;
+    float bias[VPL];
+    int most_bias = 0;          // a NaN stands above infinity here
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         bias[j] = a.bias != nullptr && j < own ? a.bias[first + j] : 0.f;
-        bmax = fmaxf(bmax, fabsf(bias[j]));
+        most_bias = max(most_bias, __float_as_int(bias[j]) & 0x7fffffff);
     }
-    bmax = number(wave_max(ordered(bmax)));
+    const float bmax = __int_as_float(wave_max(most_bias));
+    const bool exact_only = !(bmax < 0x1p100f);          // the error bounds below are for finite biases
     const bool sums = a.kind == 0 && (a.bias != nullptr || a.ngroups > 1 || !a.renorm);      // softmax over all is needed
     const long long end = (a.ncols - 1LL) * a.ldz + a.nexperts;                              // of the matrix, in elements
     const long long step = (long long)gridDim.x * WAVES * d.batch;
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(BLOCK) void k_route(RouteArgs a, Deal d, int* share
                 by = sum > 0.f ? 1.f / sum : 0.f;
             }
             unsigned taken = 0;
-            if (!bad && !take_fast<T, VPL>(a, d, z, bias, bmax, top, by, taken)) 
+            if (!bad && (exact_only || !take_fast<T, VPL>(a, d, z, bias, bmax, top, by, taken)))
                 taken = take_exact<T>((const T*)a.Z + at, a.bias != nullptr ? a.bias + first : nullptr, exact_keys + wave * 64 * d.each, own,
                                       d.each, a.kind, a.ngroups, a.topgroups, a.topk, d.lanes);
             // fewer than topk open: the lowest others fill the column
@@ -701,13 +703,15 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
     const int first = g * d.size + o;
     const int room = d.size - o < d.each ? d.size - o : d.each;
     const int own = g < a.ngroups && room > 0 ? room : 0;
-    float bias[VPL], bmax = 0.f;
+    float bias[VPL];
+    int most_bias = 0;          // a NaN stands above infinity here
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         bias[j] = a.bias != nullptr && j < own ? a.bias[first + j] : 0.f;
-        bmax = fmaxf(bmax, fabsf(bias[j]));
+        most_bias = max(most_bias, __float_as_int(bias[j]) & 0x7fffffff);
     }
-    bmax = number(wave_max(ordered(bmax)));
+    const float bmax = __int_as_float(wave_max(most_bias));
+    const bool exact_only = !(bmax < 0x1p100f);          // the error bounds below are for finite biases
 #pragma unroll
     for (int j = 0; j < VPL; ++j) bias[j] += bmax;
     const bool sums = a.kind == 0 && (a.bias != nullptr || a.ngroups > 1 || !a.renorm);
@@ -761,6 +765,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
             }
             bool fine;
             unsigned taken = take_row<T, VPL>(a, d, z, bias, bmax, top, by, first, shut, two_largest[wave][row], fine);
+            fine = fine && !exact_only;
             if (bad) { taken = 0; fine = true; }
             // fewer than topk open: the lowest others fill the column
             const unsigned valid = taken;

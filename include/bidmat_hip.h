@@ -397,7 +397,8 @@ int bidmat_rmsnorm_grad(int nrows, int ncols, int type, const void *H, int ldh, 
  *   the experts lie in ngroups equal groups in order; the topgroups groups with the largest sum of their two largest keys
  *   stay open, and of their experts the topk largest keys are taken; the lower index first among equals
  *   weight = scale * p, or with renorm scale * p / (sum of the taken p); the bias takes no part in it
- * Keys are compared as their values in 64 bits compare.  A score of -inf closes an expert to its column; where fewer than
+ * Keys are compared as their values in 64 bits compare.  A score of -inf closes an expert to its column (a bias of -inf or
+ * NaN closes it to all); where fewer than
  * topk are open, the remaining entries are the lowest other experts with weight 0 (a column of -inf is padding).  A NaN
  * among a column's scores (softmax: or +inf) makes its weights NaN, its experts 0 .. topk-1.
  * counts (nullable, nexperts ints): how many columns took each expert (entries of weight 0 by the rule above, and columns
@@ -419,7 +420,7 @@ int bidmat_route_grad(int nexperts, int ncols, int type, const void *Z, int ldz,
  * nullable, not all.  dZ may be Z.  A column without stored values (or only -inf), or of weight 0, has loss 0 and
  * gradient 0 whatever its logits are.  Rows need not be sorted; the shares of a row stored twice add.  Entries whose row lies outside
  * the matrix are left out.  A row whose student logit is -inf has q = 0 (with p > 0: loss +inf); a column of them has no
- * softmax: NaN.  nrows <= 2^30. */
+ * softmax: NaN.  temperature from 1e-30 to 1e30, nrows <= 2^30. */
 int bidmat_distill(int nrows, int ncols, int type, const void *Z, int ldz, int nnz, const float *Tdata, const int *Tir,
                    const int *Tjc, float temperature, const float *weight, float *loss, float *lse, void *dZ, int lddz,
                    void *stream);

@@ -98,7 +98,7 @@ def route(Z, bias, kind, ngroups, topgroups, topk, renorm, scale):
             continue
         p = _p(z, kind)
         key = z.copy() if bias is None and ngroups == 1 else p + (0 if bias is None else bias.astype(np.float64))
-        open_ = z > -np.inf
+        open_ = (z > -np.inf) & (key > -np.inf)
         if ngroups > 1:
             total = []
             for g in range(ngroups):

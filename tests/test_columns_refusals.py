@@ -95,7 +95,7 @@ def test_route_grad(bad):
 
 @pytest.mark.parametrize("bad", COMMON + [
     dict(V=-1), dict(V=2 ** 30 + 1, ldz=2 ** 30 + 1), dict(Z=None), dict(T=None), dict(ir=None), dict(jc=None), dict(nnz=-1), dict(tau=0.0),
-    dict(tau=-1.0), dict(tau=NAN), dict(tau=INF), dict(tau=1e-45), dict(ldz=99), dict(lddz=99), dict(dZ=P + 2), dict(dZ=P, lddz=101),
+    dict(tau=-1.0), dict(tau=NAN), dict(tau=INF), dict(tau=1e-45), dict(tau=1e-31), dict(tau=1e31), dict(ldz=99), dict(lddz=99), dict(dZ=P + 2), dict(dZ=P, lddz=101),
     dict(Z=P + 1)])
 def test_distill(bad):
     assert distill(**bad) == 1
@@ -113,6 +113,18 @@ def test_distill_needs_an_output():
     dict(ldq=63), dict(group=16), dict(group=256), dict(beta=2)])
 def test_dsmult_q8(bad):
     assert q8(**bad) == 1
+
+
+def test_overlapping_operands_are_refused():
+    n = 64 * 4                                           # elements of the dense operands above
+    assert norm(H=P + 2 * n - 2) == 1 and norm(H=FAR + 4) == 1 and norm(Y=FAR + 128) == 1
+    assert norm(Q=0x50000000, scales=0x50000000 + 3) == 1 and norm(Q=0x50000000, scales=P + 4) == 1
+    assert norm_grad(dw=FAR) == 1 and norm_grad(dw=0x40000000 + 8) == 1 and norm_grad(dw=FARTHER + 4) == 1
+    assert route(ir=FAR) == 1 and route(ic=FAR + 4) == 1 and route(jc=FARTHER + 8) == 1 and route(counts=P) == 1 and route(bias=FAR + 4) == 1
+    assert route_grad(dZ=FAR) == 1
+    assert distill(loss=FARTHER + 4) == 1 and distill(lse=FAR) == 1 and distill(loss=P) == 1 and distill(weight=FAR + 4, loss=FAR + 16) == 1
+    assert distill_grad(dZ=FAR) == 1
+    assert q8(C=FAR) == 1 and q8(C=P) == 1 and q8(C=FARTHER + 2) == 1 and q8(scales=FAR + 2) == 1
 
 
 def test_nothing_to_do_is_no_error():

@@ -321,6 +321,34 @@ def test_route_closed_experts_padding_and_nan(hip, kind, renorm):
                     route_case(hip, rng, E, m, t, kind, bias, groups, tg, k, renorm, Z=z)
 
 
+@pytest.mark.parametrize("kind", [0, 1])
+def test_route_biases_that_are_not_finite(hip, kind):
+    rng = np.random.default_rng(33)
+    E = 64
+    b = (0.05 * rng.standard_normal(E)).astype(F)
+    b[[3, 40]], b[17], b[[5, 63]] = -np.inf, np.inf, np.nan
+    for groups, tg, k in ((1, 1, 6), (8, 3, 6), (2, 2, 20)):
+        for m in (5, 200):
+            route_case(hip, rng, E, m, 0, kind, b, groups, tg, k, False)
+    b[:] = -np.inf
+    route_case(hip, rng, E, 70, 0, kind, b, 1, 1, 6, True)
+
+
+@pytest.mark.parametrize("E,groups,tg,k", [(16, 4, 2, 5), (48, 16, 3, 7), (256, 16, 16, 16), (250, 10, 4, 16), (240, 3, 1, 16), (17, 1, 1, 16),
+                                           (256, 2, 1, 2), (96, 12, 5, 1)])
+def test_route_sixteen_lanes(hip, E, groups, tg, k):
+    """More shapes of the kernel that takes four columns per wave: few and many groups, every column length, rows of few scores."""
+    rng = np.random.default_rng(E + k)
+    for t in TYPES:
+        for kind in (0, 1):
+            for bias in (None, True):
+                m = int(rng.integers(65, 300))
+                z = rng.standard_normal((m, E)) * 1.5
+                z[rng.random((m, E)) < 0.3] = -np.inf
+                z[::7] = np.round(z[::7])
+                route_case(hip, rng, E, m, t, kind, bias, groups, tg, k, bool(rng.integers(2)), Z=z, pad=int(rng.integers(3)))
+
+
 def route_grad_case(hip, rng, E, m, t, kind, k, renorm, pad=0, shift=0, in_place=False, Z=None):
     z = rng.standard_normal((m, E)) * 1.5 if Z is None else Z
     d, G, ir = route_case(hip, rng, E, m, t, kind, True, 1, 1, k, renorm, pad, shift, Z=z)
@@ -482,6 +510,39 @@ def distill_case_raw(hip, z, T, ir, jc, t, weight, in_place, tau=1.0):
     return loss.numpy().astype(np.float64), lse.numpy(), decode(dZ.get(), t)
 
 
+@pytest.mark.parametrize("V", [100, 9000, 140000])
+@pytest.mark.parametrize("t", TYPES)
+def test_distill_every_choice_of_outputs(hip, V, t):
+    """loss, lse and dZ alone and together, and the gradient alone in place of the logits."""
+    rng = np.random.default_rng(V + t)
+    m = 6
+    T, ir, jc = teacher(rng, V, [5, 0, 80, 1, 64, 65], sort=False)
+    z = encode(rng.standard_normal((m, V)), t)
+    a, dT, di, dj = Columns(z), dev(T), dev(ir), dev(jc)
+    base = (V, m, t, a.ptr, V, ir.size, dT.ptr, di.ptr, dj.ptr, 1.5, None)
+    zd = decode(z, t)
+    want, wlse, wd, eloss, ez = ref.distill(zd, T, ir, jc, 1.5, None)
+    elose = EPS24 * (8 * (np.abs(zd).max(1) + np.abs(wlse)) + 160)
+    for with_loss, with_lse, with_dz in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1), (1, 1, 0)):
+        loss, lse, dZ = dev(np.full(m, 7, F)), dev(np.full(m, 7, F)), empty(m, V, np_type(t))
+        untouched = dZ.get()
+        ok(hip.bidmat_distill(*base, loss.ptr if with_loss else None, lse.ptr if with_lse else None, dZ.ptr if with_dz else None, V, None))
+        if with_loss:
+            within(loss.numpy().astype(np.float64), want, eloss + 160 * EPS24 * np.abs(want), "loss")
+        if with_lse:
+            within(lse.numpy().astype(np.float64), wlse, elose, "lse")
+        if with_dz:
+            within(decode(dZ.get(), t), wd, HALF_STEP[t] * 1.01 * np.abs(wd) + TINY[t] + ez, "dz")
+        assert with_loss or (loss.numpy() == 7).all()
+        assert with_lse or (lse.numpy() == 7).all()
+        assert with_dz or np.array_equal(dZ.get(), untouched)
+    lse = dev(wlse.astype(F))
+    dZ = empty(m, V, np_type(t))
+    ok(hip.bidmat_distill_grad(*base, lse.ptr, dZ.ptr, V, None))
+    ok(hip.bidmat_distill_grad(*base, lse.ptr, a.ptr, V, None))
+    assert np.array_equal(a.get(), dZ.get())
+
+
 def test_distill_without_entries_at_all(hip):
     for V in (10, 5000):
         a, dZ = Columns(np.full((3, V), np.nan, F)), empty(3, V, np.float32)
@@ -594,6 +655,20 @@ def test_dsmult_q8_short_segments(hip):
         ok(hip.bidmat_set_option(b"seglen", old))
 
 
+def test_dsmult_q8_of_a_range_of_columns(hip):
+    """Columns [3, 8) of a matrix through Sjc + 3 and the whole matrix's arrays, columns among them that are cut."""
+    rng = np.random.default_rng(4)
+    lengths = [700, 3, 0, 900, 257, 2, 0, 1500, 40, 300]
+    k, rows = 80, 60
+    jc = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    ir, S = rng.integers(0, rows, int(jc[-1])).astype(np.int32), rng.standard_normal(int(jc[-1])).astype(F)
+    codes, scales = rng.integers(0, 0x7F, (rows, k)).astype(np.uint8), (0.01 + rng.random((rows, 1))).astype(F)
+    q, s, v, i, j, c = Columns(codes), dev(scales), dev(S), dev(ir), dev(jc), empty(5, k, np.float32)
+    ok(hip.bidmat_dsmult_q8_csc(k, 5, int(jc[8] - jc[3]), q.ptr, k, s.ptr, 0, v.ptr, i.ptr, j.ptr + 12, c.ptr, 0, None))
+    want, size = ref.q8_product(codes, scales, 0, S, ir, jc[3:9])
+    within(c.get().astype(np.float64), want, 300 * EPS24 * size, "C")
+
+
 def test_dsmult_q8_every_code(hip):
     """All 256 codes through a product with one nonzero of value 1 and scale 1: the decoded values themselves."""
     codes = np.arange(256, dtype=np.uint8)[None]
@@ -618,6 +693,35 @@ def test_rmsnorm_codes_round_to_nearest_even(hip):
     gap = np.abs(q[:, None] - want[:, None])
     nearest = np.abs(mags[None, :] - want[:, None]).min(1)
     assert (gap[:, 0] <= nearest + 4 * EPS24 * want).all()
+
+
+# ---------------------------------------------------------------- more columns than one launch takes
+def test_millions_of_columns(hip):
+    rng = np.random.default_rng(95)
+    n, m = 3, 4300000
+    x = encode(rng.standard_normal((m, n)), 2)
+    X, Y, w = dev(x), DeviceArray(n * m, np.uint16), dev(np.ones(n, F))
+    ok(hip.bidmat_rmsnorm(n, m, 2, X.ptr, n, None, n, w.ptr, 1e-5, None, n, Y.ptr, n, None, n, None, 0, None))
+    _, y, _ = ref.rmsnorm(decode(x, 2), None, np.ones(n), float(F(1e-5)))
+    within(decode(Y.numpy().reshape(m, n), 2), y, (HALF_STEP[2] * 1.01 + NORM_DEPTH * EPS24) * np.abs(y) + TINY[2], "y")
+    # one teacher entry per column: loss = lse - x at it, dz = q - 1 there
+    ir, jc = rng.integers(0, n, m).astype(np.int32), np.arange(m + 1, dtype=np.int32)
+    T, di, dj, loss = dev(np.ones(m, F)), dev(ir), dev(jc), DeviceArray(m, F)
+    ok(hip.bidmat_distill(n, m, 2, X.ptr, n, m, T.ptr, di.ptr, dj.ptr, 1.0, None, loss.ptr, None, Y.ptr, n, None))
+    xd = decode(x, 2)
+    q = np.exp(xd) / np.exp(xd).sum(1, keepdims=True)
+    within(loss.numpy().astype(np.float64), -np.log(q[np.arange(m), ir]), 200 * EPS24 * (1 + np.abs(xd).max(1)), "loss")
+    q[np.arange(m), ir] -= 1
+    within(decode(Y.numpy().reshape(m, n), 2), q, HALF_STEP[2] * 1.01 * np.abs(q) + 400 * EPS24, "dz")
+    G, ir1, dG = DeviceArray(m, F), DeviceArray(m, np.int32), dev(rng.standard_normal(m).astype(F))
+    ok(hip.bidmat_route(n, m, 2, X.ptr, n, None, 0, 1, 1, 1, 0, 1.0, G.ptr, ir1.ptr, None, None, None, None))
+    assert np.array_equal(ir1.numpy(), xd.argmax(1))
+    ok(hip.bidmat_route_grad(n, m, 2, X.ptr, n, 0, 1, 0, 1.0, G.ptr, ir1.ptr, dG.ptr, Y.ptr, n, None))
+    p = np.exp(xd) / np.exp(xd).sum(1, keepdims=True)
+    d = dG.numpy().astype(np.float64)[:, None]
+    top = xd.argmax(1)[:, None]
+    want = p * (np.where(np.arange(n) == top, d, 0) - np.take_along_axis(p, top, 1) * d)
+    within(decode(Y.numpy().reshape(m, n), 2), want, HALF_STEP[2] * 1.01 * np.abs(want) + 400 * EPS24 * np.abs(d), "route dz")
 
 
 # ---------------------------------------------------------------- streams, graphs, threads
