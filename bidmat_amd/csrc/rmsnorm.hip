@@ -200,7 +200,9 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         }
     }
     if (a.dw == nullptr) return;
-    float* share = partial + (size_t)blockIdx.x * n;
+    // a single workgroup's share is the gradient (partial == nullptr)
+    float* share = partial != nullptr ? partial + (size_t)blockIdx.x * n : a.dw;
+    const bool add = partial == nullptr && a.beta != 0;
     if constexpr (CPB > 1) {
         // the columns of a wave first, then the workgroup's four waves
         __shared__ float sum[BM_WAVES_PER_BLOCK][TPC * 8 * NV];
@@ -214,10 +216,16 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
                 if ((threadIdx.x & 63) < TPC) sum[threadIdx.x >> 6][(v * TPC + t) * 8 + j] = d;
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += BM_BLOCK) share[i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+        for (int i = threadIdx.x; i < n; i += BM_BLOCK) {
+            const float d = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+            share[i] = add ? share[i] + d : d;
+        }
     } else {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) store_col8(share, (v * TPC + t) * 8, n, dw[v]);
+        for (int v = 0; v < NV; ++v) {
+            const int i = (v * TPC + t) * 8;
+            store_col8(share, i, n, add ? load_col8(share, i, n).wide() + dw[v] : dw[v]);
+        }
     }
 }
 
@@ -257,15 +265,16 @@ template <class T, int TPC, int NV>
 hipError_t launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
     constexpr int CPB = norm_block(TPC) / TPC;
     const long long want = (a.ncols + CPB - 1LL) / CPB, most = norm_shares(norm_block(TPC));
-    const unsigned grid = (unsigned)(want < most ? want : most);
+    // up to four turns of one workgroup take less time than a second launch
+    const unsigned grid = (unsigned)(a.dw != nullptr && want <= 4 ? 1 : want < most ? want : most);
     float* partial = nullptr;
-    if (a.dw != nullptr) {
+    if (a.dw != nullptr && grid > 1) {
         hipError_t err;
         partial = (float*)ws_get(WS_NORM_SHARES, sizeof(float) * (size_t)grid * (size_t)a.nrows, &err, s);
         if (!partial) return err;
     }
     hipLaunchKernelGGL((k_rmsnorm_grad<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a, partial);
-    if (a.dw != nullptr)
+    if (a.dw != nullptr && grid > 1)
         hipLaunchKernelGGL((a.nrows >= 1024 ? k_add_shares<16> : k_add_shares<4>), dim3(a.nrows >= 1024 ? (a.nrows + 15) / 16 : (a.nrows + 3) / 4),
                            dim3(1024), 0, s, a.nrows, (int)grid, partial, a.dw, a.beta);
     return hipGetLastError();
