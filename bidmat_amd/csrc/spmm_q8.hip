@@ -31,21 +31,13 @@ struct Q8Args {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// Rows i .. i+15 of a column of k codes, those past its end as zeros. A short last part is loaded as the column's last 16
-// codes and shifted down.
+// Rows i .. i+15 of a column of k codes (i < k). A short last part is loaded as the column's last 16 codes, and shifted down
+// by settle_codes when its turn comes: nothing between the loads waits for one of them.
 __device__ __forceinline__ uint4 load_codes(const unsigned char* col, int i, int k) {
     uint4 x = make_uint4(0, 0, 0, 0);
-    if ((k & 15) == 0) {
-        __builtin_memcpy(&x, col + i, 16);
-    } else if (k >= 16) {
+    if (k >= 16) {
         const int s = i + 16 - k > 0 ? i + 16 - k : 0;          // codes in front of row i
         __builtin_memcpy(&x, col + i - s, 16);
-        if (s & 8) x = make_uint4(x.z, x.w, 0, 0);
-        if (s & 4) x = make_uint4(x.y, x.z, x.w, 0);
-        x.x = __builtin_amdgcn_alignbyte(x.y, x.x, s & 3);
-        x.y = __builtin_amdgcn_alignbyte(x.z, x.y, s & 3);
-        x.z = __builtin_amdgcn_alignbyte(x.w, x.z, s & 3);
-        x.w = __builtin_amdgcn_alignbyte(0u, x.w, s & 3);
     } else {
         unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -53,6 +45,17 @@ __device__ __forceinline__ uint4 load_codes(const unsigned char* col, int i, int
             if (i + j < k) w[j >> 2] |= (unsigned)col[i + j] << (8 * (j & 3));
         x = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    return x;
+}
+__device__ __forceinline__ uint4 settle_codes(uint4 x, int i, int k) {
+    if ((k & 15) == 0 || k < 16) return x;
+    const int s = i + 16 - k > 0 ? i + 16 - k : 0;
+    if (s & 8) x = make_uint4(x.z, x.w, 0, 0);
+    if (s & 4) x = make_uint4(x.y, x.z, x.w, 0);
+    x.x = __builtin_amdgcn_alignbyte(x.y, x.x, s & 3);
+    x.y = __builtin_amdgcn_alignbyte(x.z, x.y, s & 3);
+    x.z = __builtin_amdgcn_alignbyte(x.w, x.z, s & 3);
+    x.w = __builtin_amdgcn_alignbyte(0u, x.w, s & 3);
     return x;
 }
 __device__ __forceinline__ void fma_codes(float (&acc)[16], uint4 x, float by) {
@@ -94,12 +97,43 @@ __device__ __forceinline__ void gather_codes(const Q8Args& a, int row, float val
         }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) fma_codes(acc, x[u], FULL || (it0 + u) * NG + g < rem ? v[u] * by[u] : 0.f);
+    for (int u = 0; u < U; ++u) fma_codes(acc, settle_codes(x[u], i, a.k), FULL || (it0 + u) * NG + g < rem ? v[u] * by[u] : 0.f);
 }
 
 // Segments begin at the multiples of seglen counted from the first nonzero, jc[0] (a range of columns may be passed with the
 // whole matrix's arrays). The first one that begins at or after position x:
 __device__ __forceinline__ int segment_from(const Q8Args& a, int x) { return (int)(((long long)x - a.jc[0] + a.seglen - 1) / a.seglen); }
+
+// a summed over the two halves of the wave (HALVES) or over the two rows of 16 lanes of each half, in the lower of the two,
+// and b in the upper one.
+template <bool HALVES>
+__device__ __forceinline__ float split_sum(float a, float b) {
+    unsigned x = __float_as_uint(a), y = __float_as_uint(b);
+    if constexpr (HALVES) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        x = r[0]; y = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        x = r[0]; y = r[1];
+    }
+    return __uint_as_float(x) + __uint_as_float(y);
+}
+
+// Rows i .. i+W-1 of a column of k sums, those past its end left out.
+template <int W>
+__device__ __forceinline__ void store_rows(float* col, int i, int k, const float (&v)[16], bool add) {
+    if (i + W <= k) {
+        float o[W];
+        if (add) __builtin_memcpy(o, col + i, sizeof(o));
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[j] = add ? o[j] + v[j] : v[j];
+        __builtin_memcpy(col + i, o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (i + j < k) col[i + j] = add ? col[i + j] + v[j] : v[j];
+    }
+}
 
 template <int LPN>
 __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
@@ -151,26 +185,27 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
             for (; (it + U) * NG <= rem; it += U) gather_codes<LPN, U, true>(a, row, val, rem, it, g, i, left, sg, acc);
             for (; it < turns; it += U) gather_codes<LPN, U, false>(a, row, val, rem, it, g, i, left, sg, acc);
         }
+        // the groups' sums: the wave's halves, then rows of 16 lanes exchange half of their rows of C (one exchange and one
+        // addition give two sums), and what is left lies inside a row of lanes
+        int off = 0;
+        constexpr int W = NG == 1 ? 16 : NG == 2 ? 8 : 4;
+        if constexpr (NG >= 2) {
 #pragma unroll
-        for (int m = LPN; m < 64; m <<= 1)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[j] += __shfl_xor(acc[j], m, 64);
-        if (g == 0) {
-            if (left >= 16) {
-                float4 o[4];
-                if (add) __builtin_memcpy(o, out + i, 64);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 s = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-                    o[j] = add ? make_float4(o[j].x + s.x, o[j].y + s.y, o[j].z + s.z, o[j].w + s.w) : s;
-                }
-                __builtin_memcpy(out + i, o, 64);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (j < left) out[i + j] = add ? out[i + j] + acc[j] : acc[j];
-            }
+            for (int j = 0; j < 8; ++j) acc[j] = split_sum<true>(acc[j], acc[j + 8]);
+            off += lane & 32 ? 8 : 0;
         }
+        if constexpr (NG >= 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[j] = split_sum<false>(acc[j], acc[j + 4]);
+                if constexpr (LPN <= 8) acc[j] += dpp_mov<0x128>(acc[j]);      // row_ror 8, 4, 2, 1
+                if constexpr (LPN <= 4) acc[j] += dpp_mov<0x124>(acc[j]);
+                if constexpr (LPN <= 2) acc[j] += dpp_mov<0x122>(acc[j]);
+                if constexpr (LPN <= 1) acc[j] += dpp_mov<0x121>(acc[j]);
+            }
+            off += lane & 16 ? 4 : 0;
+        }
+        if (LPN >= 16 || (lane & 15) < LPN) store_rows<W>(out, i + off, a.k, acc, add);
     }
 }
 
