@@ -1,16 +1,18 @@
 // C = beta*C + A*S with A in 8 bits (e4m3) and fp32 scales: A[i, r] = scales[i / group, r] * q[i, r].
 //
 // The gathers of A's columns bound A*S; codes are a quarter of the fp32 bytes. One wavefront owns a column of S. A column
-// longer than a segment (a quarter of "seglen" nonzeros: with a quarter of the bytes per nonzero, a wave that walks more
-// of them alone is still running when the others are done) is cut at the multiples of the segment length in the array of
-// nonzeros: its own wave goes up to the first of them, the wave of every multiple inside it takes the segment that begins
-// there, found by a search in jc, and leaves a partial sum; these are added in order. Sums are fp32.
+// longer than a segment is cut at the multiples of the segment length in the array of nonzeros: its own wave goes up to the
+// first of them, the wave of every multiple inside it takes the segment that begins there, found by a search in jc, and
+// leaves a partial sum; these are added in order. Sums are fp32. A segment is an eighth of "seglen" nonzeros, so that no
+// wave is still walking when the others are done (k = 1024, columns of power-law lengths up to 2000: 364 us at 128 nonzeros,
+// 377 at 256, 483 at 1024), or a quarter where a wave takes eight nonzeros and more at a time (k = 64: 74 us at 256, 82 at 128).
 // LPN lanes cover 16 * LPN rows with one 16-byte load each; a wave works on 64 / LPN nonzeros at a time.
 //
-// What bounds it: lines of A that miss L2, which the fabric passes at 7.0 to 7.7 TB/s whatever lies behind it. k = 1024,
-// 200000 columns of A, 2 M nonzeros in 50000 columns of 40: 350 us, 5.8 TB/s of gathers and 0.6 TB/s of C (one gather at a
-// time 746 us; four in flight per lane as good as eight or sixteen, which cost occupancy where k is small: 140 us instead
-// of 175 at k = 100).
+// What bounds it: lines of A that miss L2, which come at 7.0 to 7.7 TB/s whatever lies behind it. k = 1024, 200000 columns
+// of A, 2 M nonzeros in 50000 columns of 40: 350 us, 5.8 TB/s of gathers and 0.6 TB/s of C (one gather at a time 746 us;
+// four in flight per lane as good as eight or sixteen, which cost occupancy where k is small). Rows of a column that
+// different groups of lanes hold are added by exchanging halves (k = 16, 4 M nonzeros in 100000 columns: 51 us; with all 16
+// sums shuffled through LDS 114 us).
 #include "columns.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -242,7 +244,7 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
                          const float* vals, const int* ir, const int* jc, float* C, int beta, hipStream_t s) {
     Q8Args a;
     a.k = k; a.ncols = ncols; a.nnz = nnz; a.beta = beta;
-    a.seglen = opt_seglen() / 4;
+    a.seglen = opt_seglen() / (k > 128 ? 8 : 4);
     a.nscales = group == 0 ? 1 : (k + group - 1) / group;
     a.shift = group == 0 ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7;
     a.ldq = ldq; a.Q = Q; a.scales = scales; a.vals = vals; a.ir = ir; a.jc = jc; a.C = C;
