@@ -137,9 +137,12 @@ __device__ __forceinline__ void store_rows(float* col, int i, int k, const float
     }
 }
 
-template <int LPN>
+// STAGED (LPN = 64): a lane's 16 rows go to C through LDS, so that a store covers one stretch of 1 KiB instead of 16 bytes of
+// every 64.
+template <int LPN, bool STAGED>
 __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     constexpr int NG = 64 / LPN;
+    __shared__ float stage[STAGED ? BM_WAVES_PER_BLOCK : 1][STAGED ? 16 * LPN : 1];
     const int lane = threadIdx.x & 63, l = lane % LPN, g = lane / LPN;
     const long long w = (long long)blockIdx.x * BM_WAVES_PER_BLOCK + wave_uniform(threadIdx.x >> 6);
     int lo, hi;
@@ -207,7 +210,22 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
             }
             off += lane & 16 ? 4 : 0;
         }
-        if (LPN >= 16 || (lane & 15) < LPN) store_rows<W>(out, i + off, a.k, acc, add);
+        if constexpr (STAGED) {
+            float* mine = stage[threadIdx.x >> 6];
+#pragma unroll
+            for (int j = 0; j < W; j += 4)
+                *(float4*)(mine + 16 * l + off + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            __builtin_amdgcn_wave_barrier();          // a wave's LDS operations take effect in order
+#pragma unroll
+            for (int j = 0; j < 16 * LPN; j += 256) {
+                float v[16];
+                *(float4*)v = *(const float4*)(mine + j + 4 * lane);
+                if (k0 + j + 4 * lane < a.k) store_rows<4>(out, k0 + j + 4 * lane, a.k, v, add);
+            }
+            __builtin_amdgcn_wave_barrier();
+        } else if (LPN >= 16 || (lane & 15) < LPN) {
+            store_rows<W>(out, i + off, a.k, acc, add);
+        }
     }
 }
 
@@ -232,9 +250,9 @@ __global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
     }
 }
 
-template <int LPN>
+template <int LPN, bool STAGED = false>
 hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
-    hipLaunchKernelGGL((k_dsmult_q8<LPN>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK)), dim3(BM_BLOCK), 0, s, a);
+    hipLaunchKernelGGL((k_dsmult_q8<LPN, STAGED>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK)), dim3(BM_BLOCK), 0, s, a);
     return hipGetLastError();
 }
 
@@ -264,6 +282,9 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     else if (lanes <= 8) err = launch_q8<8>(a, nwaves, s);
     else if (lanes <= 16) err = launch_q8<16>(a, nwaves, s);
     else if (lanes <= 32) err = launch_q8<32>(a, nwaves, s);
+    // Few nonzeros per column: C's stores are what counts (k = 1024, 100000 columns of 2: 123 us staged, 158 not; of 8: 204 and
+    // 223). With more, the gathers do, and they run faster beside the scattered stores (of 16: 329 and 319; 50000 of 32: 297 and 291).
+    else if (nnz < 12LL * ncols) err = launch_q8<64, true>(a, nwaves, s);
     else err = launch_q8<64>(a, nwaves, s);
     if (err == hipSuccess && a.nsegs > 0) {
         hipLaunchKernelGGL(k_add_segments, dim3((unsigned)(((long long)ncols + kLook - 1) / kLook)), dim3(BM_BLOCK), 0, s, a);
