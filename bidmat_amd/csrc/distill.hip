@@ -87,29 +87,35 @@ __device__ __forceinline__ void column_entries(const DistillArgs& a, long long c
 }
 __device__ __forceinline__ float column_scale(const DistillArgs& a, long long c) { return a.weight != nullptr ? a.weight[c] : 1.f; }
 
-// One wave: whether a row is stored twice among n. Ascending rows show that they are not in one pass; others are compared
-// in pairs, 64 at a time.
-__device__ int rows_repeat(const int* rows, int n) {
+// One wave: whether a row is stored twice among n. Ascending rows show that they are not in one pass. Others set a bit each in
+// a table in LDS, by a hash of the row; one that finds its bit set is compared with the rows before it.
+constexpr int kTableWords = 512;
+__device__ int rows_repeat(const int* rows, int n, unsigned* table) {
     const int lane = threadIdx.x & 63;
     bool ascend = true;
     for (int j = lane; j + 1 < n; j += 64) ascend = ascend && rows[j] < rows[j + 1];
     if (__ballot(!ascend) == 0) return 0;
-    unsigned long long met = 0;
+#pragma unroll
+    for (int i = 0; i < kTableWords; i += 64) table[i + lane] = 0;
     for (int j0 = 0; j0 < n; j0 += 64) {
-        const int mine = j0 + lane < n ? rows[j0 + lane] : -1 - lane;
-        for (int q0 = j0; q0 < n; q0 += 64) {
-            const int other = q0 + lane < n ? rows[q0 + lane] : -1;
-            const int count = n - q0 < 64 ? n - q0 : 64;
-            for (int q = 0; q < count; ++q) met |= __ballot(mine == __builtin_amdgcn_readlane(other, q) && (j0 != q0 || lane != q));
+        const bool on = j0 + lane < n;
+        const int r = on ? rows[j0 + lane] : 0;
+        const unsigned h = ((unsigned)r * 2654435761u) >> 18, bit = 1u << (h & 31);
+        const bool met = on && (atomicOr(&table[h >> 5], bit) & bit) != 0;
+        for (unsigned long long m = __ballot(met); m != 0; m &= m - 1) {
+            const int other = __builtin_amdgcn_readlane(r, __builtin_ctzll(m));
+            int count = 0;
+            for (int q = 0; q <= j0; q += 64) count += __popcll(__ballot(q + lane < n && rows[q + lane] == other));
+            if (count > 1) return 1;
         }
     }
-    return met != 0;
+    return 0;
 }
 
 // One wave: statistics of a column's teacher entries; at[] receives the student's logit at each of them. The first 64
 // entries stay in registers, one per lane.
 template <class T>
-__device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, float* at) {
+__device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, float* at, unsigned* table) {
     const int lane = threadIdx.x & 63;
     int lo, hi;
     column_entries(a, c, lo, hi);
@@ -162,7 +168,7 @@ __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, f
     for (int j = lo + 64 + lane; j < hi; j += 64) weigh(fetch(j));
     r.part = group_allsum<64>(r.part);
     r.mass = group_allsum<64>(r.mass);
-    r.repeats = rows_repeat(a.tir + lo, hi - lo);
+    r.repeats = rows_repeat(a.tir + lo, hi - lo, table);
     return r;
 }
 
@@ -170,12 +176,13 @@ __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, f
 template <class T>
 __global__ __launch_bounds__(BM_BLOCK) void k_distill_parts(DistillArgs a, int nchunks, int chunk, LogSum* parts, Teacher* stats, float* at) {
     __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
+    __shared__ unsigned table[BM_WAVES_PER_BLOCK][kTableWords];
     const float it = 1.f / a.temperature;
     const long long nparts = (long long)nchunks * a.ncols;
     if (blockIdx.x >= nparts) {
         const long long c = (blockIdx.x - nparts) * BM_WAVES_PER_BLOCK + (threadIdx.x >> 6);
         if (c >= a.ncols) return;
-        const Teacher r = teacher_column<T>(a, c, it, at);
+        const Teacher r = teacher_column<T>(a, c, it, at, table[threadIdx.x >> 6]);
         if ((threadIdx.x & 63) == 0) stats[c] = r;
         return;
     }
@@ -342,12 +349,13 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     constexpr int WAVES = BLOCK / 64;
     __shared__ LogSum sh[WAVES];
     __shared__ Teacher teacher;
+    __shared__ unsigned table[kTableWords];
     const long long c = blockIdx.x;
     const int t = threadIdx.x, lane = t & 63, wave = wave_uniform(t >> 6), n = a.nrows;
     const float it = 1.f / a.temperature, k = it * kLog2e;
     const T* z = (const T*)a.Z + c * a.ldz;
     if (wave == WAVES - 1) {
-        const Teacher r = teacher_column<T>(a, c, it, at);
+        const Teacher r = teacher_column<T>(a, c, it, at, table);
         if (lane == 0) teacher = r;
     }
     Raw8<T> x[NV];
