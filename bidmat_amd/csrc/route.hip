@@ -685,15 +685,15 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     return taken;
 }
 
-template <class T, int VPL>
-__global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, Deal d64, int* shares) {
-    constexpr int WAVES = BM_WAVES_PER_BLOCK;
+template <class T, int VPL, int BLOCK, bool ONE>
+__global__ __launch_bounds__(BLOCK) void k_route_rows(RouteArgs a, Deal d, Deal d64, int* shares) {
+    constexpr int WAVES = BLOCK / 64;
     __shared__ int hist[256];
     __shared__ Chosen chosen[WAVES];
     __shared__ int two_largest[WAVES][4][16];
     extern __shared__ double exact_keys[];      // 64 * d64.each per wave
     if (a.counts != nullptr) {
-        for (int e = threadIdx.x; e < a.nexperts; e += BM_BLOCK) hist[e] = 0;
+        for (int e = threadIdx.x; e < a.nexperts; e += BLOCK) hist[e] = 0;
         __syncthreads();
     }
     const int l = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
@@ -799,7 +799,10 @@ __global__ __launch_bounds__(BM_BLOCK) void k_route_rows(RouteArgs a, Deal d, De
     }
     if (a.counts != nullptr) {
         __syncthreads();
-        for (int e = threadIdx.x; e < a.nexperts; e += BM_BLOCK) shares[(size_t)blockIdx.x * a.nexperts + e] = hist[e];
+        for (int e = threadIdx.x; e < a.nexperts; e += BLOCK) {
+            if (ONE) a.counts[e] = hist[e];
+            else shares[(size_t)blockIdx.x * a.nexperts + e] = hist[e];
+        }
     }
 }
 
@@ -901,14 +904,18 @@ hipError_t add_counts(const RouteArgs& a, unsigned grid, const int* shares, hipS
     return hipGetLastError();
 }
 
-constexpr int kOneColumns = 64;          // up to so many columns one workgroup does it all, in one launch
+// Few columns are left to one workgroup, which writes the counts itself and saves the second launch (7.4 us a call instead of
+// 9.8): up to two columns per wave (384 experts: 16 columns 10.7 us, 32 17.2 us against 10.9 by many workgroups), or, with
+// 16 lanes to a column, kOneRows (128 experts: 32 columns 7.3 us, by one column per wave 9.3; 64 columns 9.1; 256 experts in 8
+// groups: 48 columns 13.2 us, by many workgroups 10.7, ungrouped 8.4 against 9.8).
+constexpr int kOneRows = 48, kOneColumns = 2;
 // Waves per workgroup: as many as leave the keys of take_exact 32 KiB of LDS.
 constexpr int route_waves(int vpl, bool one) { return vpl <= 4 ? (one ? 16 : 8) : 64 / vpl; }
 
 template <class T, int VPL>
 hipError_t launch_route(const RouteArgs& a, Deal d, hipStream_t s) {
     const size_t keys = 64 * sizeof(double) * d.each;      // of one wave
-    if (a.ncols <= kOneColumns) {
+    if (a.ncols <= kOneColumns * route_waves(VPL, true)) {
         constexpr int waves = route_waves(VPL, true);
         d.batch = (a.ncols + waves - 1) / waves < kRouteBatch ? (a.ncols + waves - 1) / waves : kRouteBatch;
         hipLaunchKernelGGL((k_route<T, VPL, 64 * waves, true>), dim3(1), dim3(64 * waves), waves * keys, s, a, d, (int*)nullptr);
@@ -928,6 +935,12 @@ hipError_t launch_route(const RouteArgs& a, Deal d, hipStream_t s) {
 
 template <class T, int VPL>
 hipError_t launch_route_rows(const RouteArgs& a, Deal d, const Deal& d64, hipStream_t s) {
+    const size_t keys = 64 * sizeof(double) * d64.each;      // of one wave
+    if (a.ncols <= kOneRows) {
+        d.batch = 4;
+        hipLaunchKernelGGL((k_route_rows<T, VPL, 1024, true>), dim3(1), dim3(1024), 16 * keys, s, a, d, d64, (int*)nullptr);
+        return hipGetLastError();
+    }
     const long long all = 4096;
     d.batch = a.ncols >= all * 4 ? 8 : 4;
     const long long want = (a.ncols + BM_WAVES_PER_BLOCK * (long long)d.batch - 1) / (BM_WAVES_PER_BLOCK * d.batch);
@@ -935,8 +948,7 @@ hipError_t launch_route_rows(const RouteArgs& a, Deal d, const Deal& d64, hipStr
     int* shares;
     const hipError_t e = count_shares(a, grid, &shares, s);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_route_rows<T, VPL>), dim3(grid), dim3(BM_BLOCK), BM_WAVES_PER_BLOCK * 64 * sizeof(double) * d64.each, s, a, d, d64,
-                       shares);
+    hipLaunchKernelGGL((k_route_rows<T, VPL, BM_BLOCK, false>), dim3(grid), dim3(BM_BLOCK), BM_WAVES_PER_BLOCK * keys, s, a, d, d64, shares);
     return add_counts(a, grid, shares, s);
 }
 
@@ -954,7 +966,8 @@ Deal deal(const RouteArgs& a, int lanes) {
 template <class T>
 hipError_t route_typed(const RouteArgs& a, hipStream_t s) {
     const Deal d = deal(a, 64), d16 = deal(a, 16);
-    if (a.ncols > kOneColumns && d16.each <= 16 && a.nexperts <= 256 && a.topk <= 16) {
+    // four columns per wave, once a workgroup's sixteen waves have a column each
+    if (a.ncols > 16 && d16.each <= 16 && a.nexperts <= 256 && a.topk <= 16) {
         if (d16.each <= 1) return launch_route_rows<T, 1>(a, d16, d, s);
         if (d16.each <= 2) return launch_route_rows<T, 2>(a, d16, d, s);
         if (d16.each <= 4) return launch_route_rows<T, 4>(a, d16, d, s);

@@ -349,6 +349,21 @@ def test_route_sixteen_lanes(hip, E, groups, tg, k):
                 route_case(hip, rng, E, m, t, kind, bias, groups, tg, k, bool(rng.integers(2)), Z=z, pad=int(rng.integers(3)))
 
 
+# Column counts on both sides of where one workgroup ends and where it takes several columns per wave; tied keys send columns
+# to the decision in 64 bits.
+@pytest.mark.parametrize("m", [2, 8, 9, 16, 17, 32, 33, 48, 49, 63])
+@pytest.mark.parametrize("E,groups,tg,k", [(16, 4, 2, 5), (60, 1, 1, 4), (256, 8, 4, 8), (256, 1, 1, 16), (100, 1, 1, 30), (384, 8, 4, 8),
+                                           (1000, 5, 2, 33)])
+def test_route_few_columns(hip, E, groups, tg, k, m):
+    rng = np.random.default_rng(E + m)
+    for t in TYPES:
+        route_case(hip, rng, E, m, t, 1, True, groups, tg, k, True)
+        route_case(hip, rng, E, m, t, 0, None, groups, tg, k, False, pad=2, shift=1)
+        steps = np.round(rng.standard_normal((m, E)) * 2) / 2
+        steps[m // 2, :] = -np.inf
+        route_case(hip, rng, E, m, t, 1, np.zeros(E, np.float32), groups, tg, k, True, Z=steps)
+
+
 def route_grad_case(hip, rng, E, m, t, kind, k, renorm, pad=0, shift=0, in_place=False, Z=None):
     z = rng.standard_normal((m, E)) * 1.5 if Z is None else Z
     d, G, ir = route_case(hip, rng, E, m, t, kind, True, 1, 1, k, renorm, pad, shift, Z=z)
