@@ -17,9 +17,13 @@
 #include "common.hpp"
 #include "kernels.hpp"
 #include "workspace.hpp"
+#include <algorithm>
 
 namespace bm {
 namespace {
+
+// Columns of S per launch, and segments at most: together they stay below 2^32 threads.
+constexpr int kSlab = 1 << 24, kSegsMax = 1 << 25;
 
 struct Q8Args {
     int k, ncols, nnz, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
@@ -260,9 +264,13 @@ hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
 
 hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long long ldq, const float* scales, int group,
                          const float* vals, const int* ir, const int* jc, float* C, int beta, hipStream_t s) {
+    for (; ncols > kSlab; ncols -= kSlab, jc += kSlab, C += (long long)kSlab * k) {
+        const hipError_t e = dsmult_q8_csc(k, kSlab, nnz, Q, ldq, scales, group, vals, ir, jc, C, beta, s);
+        if (e != hipSuccess) return e;
+    }
     Q8Args a;
     a.k = k; a.ncols = ncols; a.nnz = nnz; a.beta = beta;
-    a.seglen = opt_seglen() / (k > 128 ? 8 : 4);
+    a.seglen = std::max(opt_seglen() / (k > 128 ? 8 : 4), nnz / kSegsMax + 1);
     a.nscales = group == 0 ? 1 : (k + group - 1) / group;
     a.shift = group == 0 ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7;
     a.ldq = ldq; a.Q = Q; a.scales = scales; a.vals = vals; a.ir = ir; a.jc = jc; a.C = C;
