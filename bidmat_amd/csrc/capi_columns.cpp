@@ -127,7 +127,7 @@ API int bidmat_route_grad(int nexperts, int ncols, int type, const void* Z, int 
 namespace {
 int distill_call(const bm::DistillArgs& a, hipStream_t s) {
     if (a.nrows < 0 || a.nrows > (1 << 30) || a.ncols < 0 || a.nnz < 0 || !type_ok(a.type)) return kInvalid;
-    if (!(a.temperature >= 1e-30f) || !(a.temperature <= 1e30f)) return kInvalid;
+    if (!(a.temperature >= 1e-18f) || !(a.temperature <= 1e18f)) return kInvalid;      // its square stays in the range of fp32
     if (a.nrows == 0 || a.ncols == 0) return a.nnz > 0 ? kInvalid : 0;
     if (!a.Z || !a.tjc || (a.nnz > 0 && (!a.tdata || !a.tir))) return kInvalid;
     const size_t size = bm::elem_size(a.type);

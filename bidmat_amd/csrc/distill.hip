@@ -23,7 +23,6 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // against 17, 128 columns 24 against 22, 256 columns 33 against 45).
 constexpr int kColumnsMin = 160;
 constexpr long long kSlabParts = 1 << 22;      // workgroups of one launch, at most
-constexpr int kRowsKept = 512;         // teacher rows of a column that a workgroup keeps in LDS
 
 // Differences of logits are taken before they are scaled: a mask of the type's lowest value stays finite, and large
 // common offsets cost no digits.
@@ -88,26 +87,34 @@ __device__ __forceinline__ void column_entries(const DistillArgs& a, long long c
 __device__ __forceinline__ float column_scale(const DistillArgs& a, long long c) { return a.weight != nullptr ? a.weight[c] : 1.f; }
 
 // One wave: whether a row is stored twice among n. Ascending rows show that they are not in one pass. Others set a bit each in
-// a table in LDS, by a hash of the row; one that finds its bit set is compared with the rows before it.
-constexpr int kTableWords = 512;
-__device__ int rows_repeat(const int* rows, int n, unsigned* table) {
+// a table in LDS. A few entries do so by a hash of the row, and one that finds its bit set is compared with the entries before
+// it; with n^2 over four times the matrix's rows those comparisons would cost more than a pass over the entries for every
+// 16384 rows, in which a bit is a row.
+constexpr int kTableWords = 512, kTableBits = 32 * kTableWords;
+__device__ int rows_repeat(const int* rows, int n, int nrows, unsigned* table) {
     const int lane = threadIdx.x & 63;
     bool ascend = true;
     for (int j = lane; j + 1 < n; j += 64) ascend = ascend && rows[j] < rows[j + 1];
     if (__ballot(!ascend) == 0) return 0;
+    const bool hashed = (long long)n * n < 4LL * nrows;
+    for (int base = 0, left = nrows; left > 0; base += kTableBits, left -= kTableBits) {
 #pragma unroll
-    for (int i = 0; i < kTableWords; i += 64) table[i + lane] = 0;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const bool on = j0 + lane < n;
-        const int r = on ? rows[j0 + lane] : 0;
-        const unsigned h = ((unsigned)r * 2654435761u) >> 18, bit = 1u << (h & 31);
-        const bool met = on && (atomicOr(&table[h >> 5], bit) & bit) != 0;
-        for (unsigned long long m = __ballot(met); m != 0; m &= m - 1) {
-            const int other = __builtin_amdgcn_readlane(r, __builtin_ctzll(m));
-            int count = 0;
-            for (int q = 0; q <= j0; q += 64) count += __popcll(__ballot(q + lane < n && rows[q + lane] == other));
-            if (count > 1) return 1;
+        for (int i = 0; i < kTableWords; i += 64) table[i + lane] = 0;
+        for (int j0 = 0; j0 < n; j0 += 64) {
+            const int r = j0 + lane < n ? rows[j0 + lane] : -1;
+            const unsigned h = hashed ? ((unsigned)r * 2654435761u) >> 18 : (unsigned)r - (unsigned)base;
+            const unsigned bit = 1u << (h & 31);
+            const bool met = r >= 0 && h < kTableBits && (atomicOr(&table[h >> 5], bit) & bit) != 0;
+            unsigned long long m = __ballot(met);
+            if (!hashed && m != 0) return 1;
+            for (; m != 0; m &= m - 1) {
+                const int other = __builtin_amdgcn_readlane(r, __builtin_ctzll(m));
+                int count = 0;
+                for (int q = 0; q <= j0; q += 64) count += __popcll(__ballot(q + lane < n && rows[q + lane] == other));
+                if (count > 1) return 1;
+            }
         }
+        if (hashed) return 0;
     }
     return 0;
 }
@@ -168,7 +175,7 @@ __device__ Teacher teacher_column(const DistillArgs& a, long long c, float it, f
     for (int j = lo + 64 + lane; j < hi; j += 64) weigh(fetch(j));
     r.part = group_allsum<64>(r.part);
     r.mass = group_allsum<64>(r.mass);
-    r.repeats = rows_repeat(a.tir + lo, hi - lo, table);
+    r.repeats = rows_repeat(a.tir + lo, hi - lo, a.nrows, table);
     return r;
 }
 
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
                                                            const float* at) {
     __shared__ LogSum sh[BM_WAVES_PER_BLOCK];
     __shared__ Teacher own;
-    __shared__ int rows[ALONE ? kRowsKept : 1];
+    __shared__ unsigned table[ALONE ? kTableWords : 1];
     constexpr int U = 4, STEP = BM_BLOCK * 8;            // loads in flight per thread
     const long long c = blockIdx.x / nchunks;
     const int b = (int)(blockIdx.x % nchunks), lo = b * chunk, hi = min(a.nrows, lo + chunk);
@@ -284,7 +291,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
                 }
             t.lsum = logf(group_allsum<64>(sum));
             t.some = __ballot(some) != 0;
-            for (int j = lane; j < kRowsKept && e0 + j < e1; j += 64) rows[j] = a.tir[e0 + j];
+            t.repeats = rows_repeat(a.tir + e0, e1 - e0, a.nrows, table);
             if (lane == 0) own = t;
         }
     } else {
@@ -327,13 +334,6 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     for (int j = j0; j < e1; j += (int)blockDim.x) {
         const int r = j == j0 ? r0 : a.tir[j];
         if (r < lo || r >= hi) continue;
-        if constexpr (ALONE) {
-            int met = 0;
-            const int kept = min(e1 - e0, kRowsKept);
-            for (int q = 0; q < kept; ++q) met += rows[q] == r;
-            for (int q = e0 + kept; q < e1; ++q) met += a.tir[q] == r;
-            t.repeats = met > 1;
-        }
         const float zr = ALONE ? (float)z[r] : j == j0 ? x0 : at[j];
         dz[r] = (T)(w * entry_grad(a, t, e0, e1, r, j == j0 ? t0 : a.tdata[j], zr, it, q));
     }

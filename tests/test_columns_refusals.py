@@ -95,7 +95,7 @@ def test_route_grad(bad):
 
 @pytest.mark.parametrize("bad", COMMON + [
     dict(V=-1), dict(V=2 ** 30 + 1, ldz=2 ** 30 + 1), dict(Z=None), dict(T=None), dict(ir=None), dict(jc=None), dict(nnz=-1), dict(tau=0.0),
-    dict(tau=-1.0), dict(tau=NAN), dict(tau=INF), dict(tau=1e-45), dict(tau=1e-31), dict(tau=1e31), dict(ldz=99), dict(lddz=99), dict(dZ=P + 2), dict(dZ=P, lddz=101),
+    dict(tau=-1.0), dict(tau=NAN), dict(tau=INF), dict(tau=1e-45), dict(tau=1e-31), dict(tau=1e31), dict(tau=9e-19), dict(tau=1.1e18), dict(ldz=99), dict(lddz=99), dict(dZ=P + 2), dict(dZ=P, lddz=101),
     dict(Z=P + 1)])
 def test_distill(bad):
     assert distill(**bad) == 1

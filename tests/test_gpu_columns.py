@@ -490,6 +490,22 @@ def test_distill_long_teacher_columns(hip):
     distill_case(hip, rng, 9000, 3, 2, [6000, 0, 4500], sort=False, repeats=True, in_place=True)
 
 
+# Rows in no order, all different or with a single one stored twice, far apart: few entries, and so many that the rows are told
+# apart in ranges.
+@pytest.mark.parametrize("V,lengths", [(1000, [64, 63, 65, 200]), (40000, [399, 401, 900, 20000]), (140000, [70, 700, 800, 40000])])
+@pytest.mark.parametrize("twice", [False, True])
+def test_distill_rows_in_no_order(hip, V, lengths, twice):
+    rng = np.random.default_rng(V + twice)
+    T, ir, jc = teacher(rng, V, lengths, sort=False)
+    if twice:
+        for a, b in zip(jc[:-1], jc[1:]):
+            ir[b - 1] = ir[a]
+    T = np.minimum(T, 6)
+    for t in (0, 2):
+        distill_case(hip, np.random.default_rng(V), V, len(lengths), t, lengths, T=T, ir=ir)
+        distill_case(hip, np.random.default_rng(V), V, len(lengths), t, lengths, T=T, ir=ir, in_place=True)
+
+
 @pytest.mark.parametrize("V", [300, 40000])
 def test_distill_masks_and_rows_outside(hip, V):
     """Student logits of -inf, teacher logits of -inf (some, and all of a column), rows outside the matrix, weight 0."""
@@ -647,6 +663,28 @@ def test_dsmult_q8_heights(hip, k, group):
     q8_case(hip, rng, k, 50, [0, 1, 5, 64, 65, 0, 200, 2], group)
     q8_case(hip, rng, k, 50, [3, 0, 130], group, beta=1, pad=5, shift=3)
     q8_case(hip, rng, k, 9, [1], group)
+
+
+def test_dsmult_q8_more_columns_than_a_launch_takes(hip):
+    rng = np.random.default_rng(73)
+    m, rows, long = (1 << 24) + 777, 50, 3000
+    lengths = np.zeros(m, np.int64)
+    lengths[rng.integers(0, m, 100000)] = rng.integers(1, 4, 100000)
+    lengths[[0, (1 << 24) - 1, 1 << 24, m - 1]] = long             # cut into segments on both sides of the border
+    jc = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    ir = rng.integers(0, rows, int(jc[-1])).astype(np.int32)
+    S = rng.standard_normal(ir.size).astype(F)
+    codes = rng.integers(0, 0x7F, (rows, 1)).astype(np.uint8)
+    scales = (0.01 + rng.random((rows, 1))).astype(F)
+    q, s, v, i, j = dev(codes.reshape(-1)), dev(scales.reshape(-1)), dev(S), dev(ir), dev(jc)
+    C = dev(np.full(m, 7, F))
+    ok(hip.bidmat_dsmult_q8_csc(1, m, ir.size, q.ptr, 1, s.ptr, 0, v.ptr, i.ptr, j.ptr, C.ptr, 0, None))
+    ok(hip.bidmat_synchronize())
+    A, _ = ref.q8_product(codes, scales, 0, np.ones(rows, F), np.arange(rows, dtype=np.int32), np.arange(rows + 1, dtype=np.int32))
+    terms = S.astype(np.float64) * A[ir, 0]
+    cols = np.repeat(np.arange(m), lengths)
+    want, size = np.bincount(cols, terms, m), np.bincount(cols, np.abs(terms), m)
+    within(C.numpy().astype(np.float64), want, (long + 14) * EPS24 * size, "C")
 
 
 @pytest.mark.parametrize("k", [48, 256, 1024])
