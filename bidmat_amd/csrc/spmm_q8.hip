@@ -4,8 +4,8 @@
 // longer than a segment is cut at the multiples of the segment length in the array of nonzeros: its own wave goes up to the
 // first of them, the wave of every multiple inside it takes the segment that begins there, found by a search in jc, and
 // leaves a partial sum; these are added in order. Sums are fp32. A segment is an eighth of "seglen" nonzeros, so that no
-// wave is still walking when the others are done (k = 1024, columns of power-law lengths up to 2000: 364 us at 128 nonzeros,
-// 377 at 256, 483 at 1024), or a quarter where a wave takes eight nonzeros and more at a time (k = 64: 74 us at 256, 82 at 128).
+// wave is still walking when the others are done (k = 1024, columns of power-law lengths up to 2000: 352 us at 128 nonzeros,
+// 364 at 256, 470 at 1024), or a quarter where a wave takes eight nonzeros and more at a time (k = 64: 74 us at 256, 82 at 128).
 // LPN lanes cover 16 * LPN rows with one 16-byte load each; a wave works on 64 / LPN nonzeros at a time.
 //
 // What bounds it: lines of A that miss L2, which come at 7.0 to 7.7 TB/s whatever lies behind it. k = 1024, 200000 columns
@@ -234,8 +234,9 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
 }
 
 // C[:,c] += the partial sums of column c's segments, in order. A workgroup looks at kLook columns and adds those that were
-// cut with all of its threads.
+// cut with all of its threads, W rows each (k = 1024: 15 us with four rows, 27 with one; k = 250: one is 2 us faster).
 constexpr int kLook = 16;
+template <int W>
 __global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
     const int lane = threadIdx.x & 63;
     const long long first = (long long)blockIdx.x * kLook;
@@ -245,11 +246,28 @@ __global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
         const long long c = first + __builtin_ctzll(cut);
         const int s0 = segment_from(a, a.jc[c]);
         const int s1 = min(segment_from(a, a.jc[c + 1]), a.nsegs);
-        for (int el = threadIdx.x; el < a.k; el += BM_BLOCK) {
-            float acc = a.C[c * a.k + el];
+        for (int el = (int)threadIdx.x * W; el < a.k; el += BM_BLOCK * W) {
+            const int rows = min(W, a.k - el);
+            float acc[W];
+            float* col = a.C + c * a.k + el;
+            const float* part = a.partial + el;
+            if (rows == W) {
+                __builtin_memcpy(acc, col, sizeof(acc));
 #pragma unroll 8
-            for (int s = s0; s < s1; ++s) acc += a.partial[(long long)s * a.k + el];
-            a.C[c * a.k + el] = acc;
+                for (int s = s0; s < s1; ++s) {
+                    float p[W];
+                    __builtin_memcpy(p, part + (long long)s * a.k, sizeof(p));
+#pragma unroll
+                    for (int j = 0; j < W; ++j) acc[j] += p[j];
+                }
+                __builtin_memcpy(col, acc, sizeof(acc));
+            } else {
+                for (int j = 0; j < rows; ++j) {
+                    float x = col[j];
+                    for (int s = s0; s < s1; ++s) x += part[(long long)s * a.k + j];
+                    col[j] = x;
+                }
+            }
         }
     }
 }
@@ -295,7 +313,7 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     else if (nnz < 12LL * ncols) err = launch_q8<64, true>(a, nwaves, s);
     else err = launch_q8<64>(a, nwaves, s);
     if (err == hipSuccess && a.nsegs > 0) {
-        hipLaunchKernelGGL(k_add_segments, dim3((unsigned)(((long long)ncols + kLook - 1) / kLook)), dim3(BM_BLOCK), 0, s, a);
+        hipLaunchKernelGGL((k > BM_BLOCK ? k_add_segments<4> : k_add_segments<1>), dim3((unsigned)(((long long)ncols + kLook - 1) / kLook)), dim3(BM_BLOCK), 0, s, a);
         err = hipGetLastError();
     }
     return err;
