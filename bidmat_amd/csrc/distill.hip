@@ -22,6 +22,9 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // workgroup of its own takes about 20 us, and below this many columns the chunks win (131072 bf16 rows: 64 columns 22 us
 // against 17, 128 columns 24 against 22, 256 columns 33 against 45).
 constexpr int kColumnsMin = 160;
+// With the log-sums kept from an earlier call, columns of up to so many bytes (16384 columns bf16: 1000 rows 18 us against 38 by
+// chunks, 2000 rows 35 against 50, 4000 rows 67 against 61).
+constexpr size_t kKeptBytes = 6 << 10;
 constexpr long long kSlabParts = 1 << 22;      // workgroups of one launch, at most
 
 // Differences of logits are taken before they are scaled: a mask of the type's lowest value stays finite, and large
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
 }
 
 // A whole column in the registers of one workgroup of BLOCK threads, NV vectors of eight logits each: read once, written
-// once. The last wave takes the teacher's entries before its share of the column. Log-sums run along with the loads;
+// once; or the gradient alone, where log-sums are given. The last wave takes the teacher's entries before its share of the column. Log-sums run along with the loads;
 // afterwards the logits are still there as they were read.
 // An entry's gradient goes over the one written for its row by the wave that wrote that one, whose stores take effect
 // in order: no barrier has to wait for the column's stores.
@@ -361,21 +364,26 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     Raw8<T> x[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) x[v] = load_col8(z, (v * BLOCK + t) * 8, n, (T)(-INFINITY));
+    const bool kept = a.lse_in != nullptr;
     LogSum s = {-INFINITY, 0.f};
+    if (kept) {
+        __syncthreads();
+    } else {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) s = add_eight(s, x[v].wide(), k);
-    s = block_join(s, k, sh, WAVES);
+        for (int v = 0; v < NV; ++v) s = add_eight(s, x[v].wide(), k);
+        s = block_join(s, k, sh, WAVES);
+    }
     // 16-bit logits are widened again below: kept from above as floats they would take twice the registers
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(x[v].v));
     }
     const Teacher tc = teacher;
-    if (t == 0) write_loss(a, c, s, it, tc);
+    if (t == 0 && !kept) write_loss(a, c, s, it, tc);
     if (a.dZ == nullptr) return;
     T* dz = (T*)a.dZ + c * a.lddz;
     const float w = column_scale(a, c) * a.temperature;
-    const Share q = share_of(s, k);
+    const Share q = kept ? share_of_lse(a.lse_in[c], k) : share_of(s, k);
     const bool none = !tc.some || w == 0.f;
     int e0, e1;
     column_entries(a, c, e0, e1);
@@ -408,7 +416,8 @@ hipError_t launch_column(const DistillArgs& a, float* at, hipStream_t s) {
 template <class T>
 bool by_column(const DistillArgs& a) {
     const size_t bytes = sizeof(T) * (size_t)a.nrows;
-    return a.lse_in == nullptr && (bytes <= (128 << 10) || (bytes <= (256 << 10) && a.ncols >= kColumnsMin));
+    if (a.lse_in != nullptr) return bytes <= kKeptBytes;
+    return (bytes <= (128 << 10) || (bytes <= (256 << 10) && a.ncols >= kColumnsMin));
 }
 template <class T>
 hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {
@@ -456,7 +465,7 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
         const hipError_t e = distill_typed<T>(x, s);
         return e != hipSuccess ? e : distill_typed<T>(y, s);
     }
-    if (a.lse_in != nullptr && a.dZ != a.Z) {
+    if (a.lse_in != nullptr && a.dZ != a.Z && !by_column<T>(a)) {
         hipLaunchKernelGGL((k_distill_grad<T, true>), dim3((unsigned)nparts), dim3(BM_BLOCK + 64), 0, s, a, nchunks, chunk, nullptr, nullptr, nullptr);
         return hipGetLastError();
     }
