@@ -59,6 +59,30 @@ __device__ __forceinline__ Raw8<T> load_col8(const T* col, int i, int n, T fill 
     }
     return r;
 }
+// The same in two steps, so that nothing between loads waits for one of them. RAGGED: n is not a multiple of eight; a short
+// last part is loaded as the column's last eight elements, and moved to its place by settle_col8 when its turn comes.
+template <bool RAGGED, class T>
+__device__ __forceinline__ Raw8<T> fetch_col8(const T* col, int i, int n, T fill = T(0.f)) {
+    if (RAGGED) return n < 8 ? load_col8(col, i, n, fill) : Raw8<T>::load(col + min(i, n - 8));
+    Raw8<T> r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = fill;
+    if (i < n) r = Raw8<T>::load(col + i);
+    return r;
+}
+template <bool RAGGED, class T>
+__device__ __forceinline__ Raw8<T> settle_col8(Raw8<T> r, int i, int n, T fill = T(0.f)) {
+    const int s = i + 8 - n;                    // elements in front of row i
+    if (!RAGGED || s <= 0 || n < 8) return r;
+    typename Eight<T>::type f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = fill;
+    if (s >= 8) return {f};
+    if (s & 4) r.v = __builtin_shufflevector(r.v, f, 4, 5, 6, 7, 8, 9, 10, 11);
+    if (s & 2) r.v = __builtin_shufflevector(r.v, f, 2, 3, 4, 5, 6, 7, 8, 9);
+    if (s & 1) r.v = __builtin_shufflevector(r.v, f, 1, 2, 3, 4, 5, 6, 7, 8);
+    return r;
+}
 template <class T>
 __device__ __forceinline__ void store_col8(T* col, int i, int n, float8_t x) {
     Raw8<T> r = Raw8<T>::narrow(x);
@@ -78,6 +102,12 @@ __device__ __forceinline__ void store_col8(T* col, int i, int n, float8_t x) {
         r.v[0] = r.v[2];
     }
     if (rem & 1) *p = r.v[0];
+}
+
+template <bool RAGGED, class T>
+__device__ __forceinline__ void put_col8(T* col, int i, int n, float8_t x) {
+    if (RAGGED) store_col8(col, i, n, x);
+    else if (i < n) Raw8<T>::narrow(x).store(col + i);
 }
 
 // Largest value over aligned groups of N lanes (the steps of group_allsum); a NaN loses against any number.

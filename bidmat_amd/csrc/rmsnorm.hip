@@ -135,7 +135,7 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 //   dx = rs * (g - u * mean(g * u)) + dh,   dw_i = sum over columns of dy_i * u_i
 // Every workgroup walks columns c0, c0 + slots, ... and keeps its share of dw in registers; the shares go to partial
 // (one row of nrows floats per workgroup) and are added in a fixed order by k_add_shares.
-template <class T, int TPC, int NV>
+template <class T, int TPC, int NV, bool RAGGED>
 __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
     constexpr int CPB = norm_block(TPC) / TPC;
     __shared__ float sh[2][3][TPC > 64 ? TPC / 64 : 1];
@@ -152,27 +152,33 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
     auto fetch = [&](long long col) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            h[v] = load_col8((const T*)a.H + col * a.ldh, (v * TPC + t) * 8, n);
-            g[v] = load_col8((const T*)a.dY + col * a.lddy, (v * TPC + t) * 8, n);
-            if (AHEAD && a.dH != nullptr) r[v] = load_col8((const T*)a.dH + col * a.lddh, (v * TPC + t) * 8, n);
+            h[v] = fetch_col8<RAGGED>((const T*)a.H + col * a.ldh, (v * TPC + t) * 8, n);
+            g[v] = fetch_col8<RAGGED>((const T*)a.dY + col * a.lddy, (v * TPC + t) * 8, n);
+            if (AHEAD && a.dH != nullptr) r[v] = fetch_col8<RAGGED>((const T*)a.dH + col * a.lddh, (v * TPC + t) * 8, n);
         }
     };
+    auto weight = [&](int v) { return settle_col8<RAGGED>(fetch_col8<RAGGED>(a.w, (v * TPC + t) * 8, n), (v * TPC + t) * 8, n).wide(); };
     float8_t w[NV];
     if (AHEAD) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) w[v] = load_col8(a.w, (v * TPC + t) * 8, n).wide();
+        for (int v = 0; v < NV; ++v) w[v] = weight(v);
     }
     if (AHEAD && c < a.ncols) fetch(c);
     for (; c < a.ncols; c += step) {
         if (!AHEAD) fetch(c);
         Raw8<T> hc[NV], gc[NV], rc[NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) { hc[v] = h[v]; gc[v] = g[v]; rc[v] = r[v]; }
+        for (int v = 0; v < NV; ++v) {
+            const int i = (v * TPC + t) * 8;
+            hc[v] = settle_col8<RAGGED>(h[v], i, n);
+            gc[v] = settle_col8<RAGGED>(g[v], i, n);
+            if (AHEAD && a.dH != nullptr) rc[v] = settle_col8<RAGGED>(r[v], i, n);
+        }
         if (AHEAD && c + step < a.ncols) fetch(c + step);
         float hh = 0.f, gh = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const float8_t x = hc[v].wide(), y = gc[v].wide() * (AHEAD ? w[v] : load_col8(a.w, (v * TPC + t) * 8, n).wide());
+            const float8_t x = hc[v].wide(), y = gc[v].wide() * (AHEAD ? w[v] : weight(v));
             hh += square_sum(x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) gh = fmaf(x[j], y[j], gh);
@@ -193,10 +199,10 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         for (int v = 0; v < NV; ++v) {
             const int i = (v * TPC + t) * 8;
             const float8_t x = hc[v].wide(), y = gc[v].wide();
-            float8_t d = rs * (y * (AHEAD ? w[v] : load_col8(a.w, i, n).wide()) - x * k);
+            float8_t d = rs * (y * (AHEAD ? w[v] : weight(v)) - x * k);
             dw[v] += y * x * rs;
-            if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : load_col8((const T*)a.dH + c * a.lddh, i, n).wide();
-            store_col8(o, i, n, d);
+            if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : settle_col8<RAGGED>(fetch_col8<RAGGED>((const T*)a.dH + c * a.lddh, i, n), i, n).wide();
+            put_col8<RAGGED>(o, i, n, d);
         }
     }
     if (a.dw == nullptr) return;
@@ -273,7 +279,7 @@ hipError_t launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
         partial = (float*)ws_get(WS_NORM_SHARES, sizeof(float) * (size_t)grid * (size_t)a.nrows, &err, s);
         if (!partial) return err;
     }
-    hipLaunchKernelGGL((k_rmsnorm_grad<T, TPC, NV>), dim3(grid), dim3(norm_block(TPC)), 0, s, a, partial);
+    hipLaunchKernelGGL((a.nrows % 8 != 0 ? k_rmsnorm_grad<T, TPC, NV, true> : k_rmsnorm_grad<T, TPC, NV, false>), dim3(grid), dim3(norm_block(TPC)), 0, s, a, partial);
     if (a.dw != nullptr && grid > 1)
         hipLaunchKernelGGL((a.nrows >= 1024 ? k_add_shares<16> : k_add_shares<4>), dim3(a.nrows >= 1024 ? (a.nrows + 15) / 16 : (a.nrows + 3) / 4),
                            dim3(1024), 0, s, a.nrows, (int)grid, partial, a.dw, a.beta);
