@@ -695,6 +695,8 @@ void sameShape(const GMat& a, const GMatP& b, const char* what) {
 void vectorOf(const GMatP& v, long long n, const char* what) {
     if (v && v->length() != n) fail(fmt("%s: a vector of %lld is wanted, not %d x %d", what, n, v->nrows, v->ncols));
 }
+// A cached output belongs to all operands and settings of a call: those that the cache's own key has no room for go into the name.
+long long guidOf(const GMatP& a) { return a ? a->GUID : 0; }
 void finished(int err, const char* what) {
     if (err == 0) err = bidmat_stream_synchronize(nullptr);
     if (err != 0) fail(std::string("HIP error in ") + what + " " + bidmat_error_string(err));
@@ -705,8 +707,8 @@ GMatP GMat::rmsnorm(const GMatP& w, float eps, const GMatP& residual, GMatP oldm
     if (!w) fail("GMat.rmsnorm: no weights");
     vectorOf(w, nrows, "GMat.rmsnorm");
     sameShape(*this, residual, "GMat.rmsnorm");
-    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, residual ? residual->GUID : 0, opHash("rmsnorm"));
-    if (h) *h = newOrCheckGMat(nrows, ncols, *h, GUID, residual ? residual->GUID : 0, opHash("rmsnorm sum"));
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, guidOf(residual), opHash(fmt("rmsnorm %lld %a", w->GUID, eps).c_str()));
+    if (h) *h = newOrCheckGMat(nrows, ncols, *h, GUID, guidOf(residual), opHash("rmsnorm sum"));
     Mat::nflops += 4LL * length();
     finished(bidmat_rmsnorm(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(residual), nrows, w->pdata, eps, h ? (*h)->pdata : nullptr, nrows,
                             out->pdata, nrows, nullptr, nrows, nullptr, 0, nullptr), "GMat.rmsnorm");
@@ -719,7 +721,7 @@ GMatP GMat::rmsnormGrad(const GMatP& w, float eps, const GMatP& dy, const GMatP&
     vectorOf(dw, nrows, "GMat.rmsnormGrad");
     sameShape(*this, dy, "GMat.rmsnormGrad");
     sameShape(*this, dh, "GMat.rmsnormGrad");
-    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dy->GUID, opHash("rmsnormGrad"));
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dy->GUID, opHash(fmt("rmsnormGrad %lld %lld %a", w->GUID, guidOf(dh), eps).c_str()));
     Mat::nflops += 10LL * length();
     finished(bidmat_rmsnorm_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, w->pdata, eps, dy->pdata, nrows, devptr(dh), nrows, out->pdata, nrows,
                                  dw ? dw->pdata : nullptr, 1, nullptr), "GMat.rmsnormGrad");
@@ -730,8 +732,8 @@ GSMatP GMat::route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, 
     vectorOf(bias, nrows, "GMat.route");
     if (topk < 1 || (long long)ncols * topk > 0x7fffffffLL) fail(fmt("GMat.route: %d of %d experts for %d columns", topk, nrows, ncols));
     const int nnz = ncols * topk;
-    GSMatP out = GSMat::newOrCheckGSMat(nrows, ncols, nnz, nnz, oldmat, GUID, bias ? bias->GUID : 0, topk,
-                                        opHash(fmt("route %d %d %d %d %g", sigmoid, ngroups, topgroups, renorm, scale).c_str()));
+    GSMatP out = GSMat::newOrCheckGSMat(nrows, ncols, nnz, nnz, oldmat, GUID, guidOf(bias), topk,
+                                        opHash(fmt("route %d %d %d %d %a", sigmoid, ngroups, topgroups, renorm, scale).c_str()));
     out->nnz0 = nnz;
     out->ownPattern();                                     // new indices: nothing shared, any older plan is stale
     Mat::nflops += 6LL * length();
@@ -744,7 +746,7 @@ GMatP GMat::routeGrad(const GSMatP& gate, const GSMatP& dgate, bool sigmoid, boo
     if (!gate || !dgate || gate->nrows != nrows || gate->ncols != ncols || dgate->nnz() != gate->nnz())
         fail("GMat.routeGrad dimensions mismatch");
     if (ncols == 0 || gate->nnz() % ncols != 0) fail("GMat.routeGrad: the gate's columns differ in length");
-    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dgate->GUID, opHash("routeGrad"));
+    GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dgate->GUID, opHash(fmt("routeGrad %lld %d %d %a", gate->GUID, sigmoid, renorm, scale).c_str()));
     Mat::nflops += 6LL * length();
     finished(bidmat_route_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, gate->nnz() / ncols, renorm,
                                scale, gate->pdata, gate->pir, dgate->pdata, out->pdata, nrows, nullptr), "GMat.routeGrad");
@@ -755,7 +757,7 @@ GMatP GMat::distill(const GSMatP& teacher, float temperature, const GMatP& weigh
     if (!teacher || teacher->nrows != nrows || teacher->ncols != ncols) fail("GMat.distill dimensions mismatch");
     vectorOf(weight, ncols, "GMat.distill");
     sameShape(*this, grad, "GMat.distill");
-    GMatP out = newOrCheckGMat(1, ncols, oldmat, GUID, teacher->GUID, opHash("distill"));
+    GMatP out = newOrCheckGMat(1, ncols, oldmat, GUID, teacher->GUID, opHash(fmt("distill %lld %a", guidOf(weight), temperature).c_str()));
     Mat::nflops += 8LL * length();
     finished(bidmat_distill(nrows, ncols, BIDMAT_F32, pdata, nrows, teacher->nnz(), teacher->pdata, teacher->pir, teacher->pjc, temperature,
                             devptr(weight), out->pdata, nullptr, grad ? grad->pdata : nullptr, nrows, nullptr), "GMat.distill");

@@ -207,3 +207,30 @@ def test_the_matrix_interface(hip):
                 lambda: logits.distill(gate), lambda: logits.distill(T, -1.0), lambda: z.routeGrad(T, dgate)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_cached_outputs_belong_to_all_operands_and_settings(hip):
+    """With the operator cache on, calls that differ in any operand or setting have outputs of their own."""
+    rng = np.random.default_rng(9)
+    n, m, k = 24, 10, 4
+    x, w1, w2, dy, dh = (GMat.from_numpy(rng.standard_normal(s).astype(np.float32)) for s in ((n, m), (n, 1), (n, 1), (n, m), (n, m)))
+    teacher = GMat.from_numpy(rng.standard_normal((n, m)).astype(np.float32)).route(3)
+    weight = GMat.from_numpy(rng.random((1, m)).astype(np.float32))
+
+    def calls():
+        g1, g2 = x.route(k), x.route(k, sigmoid=True)
+        return [x.rmsnorm(w1)[0], x.rmsnorm(w2)[0], x.rmsnorm(w1, eps=0.5)[0], x.rmsnorm(w1, residual=dy)[0],
+                x.rmsnormGrad(w1, dy), x.rmsnormGrad(w2, dy), x.rmsnormGrad(w1, dy, eps=0.5), x.rmsnormGrad(w1, dy, dh=dh),
+                x.route(k).contents(), x.route(k, scale=1.0 + 2.0 ** -20).contents(), x.route(k, renorm=False).contents(),
+                x.routeGrad(g1, g1), x.routeGrad(g2, g1, sigmoid=True), x.routeGrad(g1, g1, renorm=False), x.routeGrad(g1, g1, scale=2.0),
+                x.distill(teacher), x.distill(teacher, 2.0), x.distill(teacher, weight=weight)]
+
+    plain = [a.numpy().copy() for a in calls()]
+    Mat.set("useGPUcache", 1)
+    try:
+        kept = calls()
+        for i, (a, b) in enumerate(zip(kept, plain)):
+            assert np.array_equal(a.numpy(), b), i
+    finally:
+        Mat.set("useGPUcache", 0)
+        Mat.clear_caches()
