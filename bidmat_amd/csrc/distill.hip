@@ -6,6 +6,12 @@
 //
 // A column without stored entries, or with weight 0, has loss 0 and gradient 0, whatever its logits hold. A row may be
 // stored twice; its shares add. Entries whose row lies outside the matrix are left out.
+//
+// What bounds it: memory. Loss and gradient of 131072 rows x 4096 columns in bf16: 430 us, 5.0 TB/s, every logit read once and
+// written once; the gradient alone 368 us, 5.8 TB/s. Columns above 256 KiB (and above 128 KiB where there are few) are cut
+// into chunks and read twice: 262144 x 512 fp32 312 us, 5.2 TB/s of what is moved. Taking such columns in slabs that
+// would stay in the 256 MB cache until the second time cost more than it gave (70000 x 2048 fp32: 344 us in slabs of 96 MiB, 399
+// of 48, 324 without). Few columns: two launches that leave no wait between them (100003 x 5 fp32: 3.9 and 5.0 us).
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"

@@ -8,6 +8,11 @@
 // code overflows; 2^-126 keeps 1 / scale finite for a group of zeros (whose codes are zeros).
 // TPC threads share a column and keep all of it in registers (8 * NV elements each): every input is read once and every
 // output written once, also where an output overwrites its input.
+//
+// What bounds it: memory, as long as columns of a multiple of 128 bytes let every load take whole lines (8192 rows x 16384
+// columns bf16 with residual and codes: 160 us, 5.9 TB/s; 1001 x 7777 fp32, read, written and in codes: 13.7 us, 5.1 TB/s; 1001 x
+// 15554 bf16: 24.5 us, 4.5 TB/s); a few columns, the launch. A workgroup of its own per column from 1025 rows on, more than
+// one column per wave up to 256.
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
@@ -150,6 +155,9 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 //   dx = rs * (g - u * mean(g * u)) + dh,   dw_i = sum over columns of dy_i * u_i
 // Every workgroup walks columns c0, c0 + slots, ... and keeps its share of dw in registers; the shares go to partial
 // (one row of nrows floats per workgroup) and are added in a fixed order by k_add_shares.
+// What bounds it: memory (4096 rows x 16384 columns bf16: 103 us with the shares' addition, 5.2 TB/s). Above 8192 rows a
+// thread's registers do not hold the next column, above 16384 not the present one either (16384 rows x 4096: 125 us, 4.3 TB/s;
+// 32768 x 2048: 227 us, 2.4 TB/s).
 template <class T, int TPC, int NV, bool RAGGED>
 __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
     constexpr int CPB = norm_block(TPC) / TPC;

@@ -16,6 +16,9 @@
 // a threshold: a count of the keys that reach a value is a compare per slot, the rest runs on the scalar unit, and the value
 // that exactly topk keys reach takes about ten counts whatever topk is. Keys are compared in fp32 with a bound on their
 // error; only a column with another key within that bound of the border is decided from keys in fp64 (take_exact).
+// 256 experts in 8 groups, 65536 columns bf16, 8 taken: 43 us with 16 lanes per column, 200 vector and 46 scalar instructions
+// per column (a wave per column 80 us; its bytes alone would take 8 us); 60 experts, 32768 columns fp32: 13 us, and 4 us to
+// add up the counts. Above 256 experts a wave per column: 512 experts, 32768 columns fp32 45 us, 1000 experts, 16384 columns 48 us.
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
