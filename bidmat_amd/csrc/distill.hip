@@ -8,10 +8,10 @@
 // stored twice; its shares add. Entries whose row lies outside the matrix are left out.
 //
 // What bounds it: memory. Loss and gradient of 131072 rows x 4096 columns in bf16: 430 us, 5.0 TB/s, every logit read once and
-// written once; the gradient alone 368 us, 5.8 TB/s. Columns above 256 KiB (and above 128 KiB where there are few) are cut
+// written once; the gradient alone 368 us, 5.8 TB/s. Columns above 384 or 400 KiB (and above 128 KiB where there are few) are cut
 // into chunks and read twice: 262144 x 512 fp32 312 us, 5.2 TB/s of what is moved. Taking such columns in slabs that
 // would stay in the 256 MB cache until the second time cost more than it gave (70000 x 2048 fp32: 344 us in slabs of 96 MiB, 399
-// of 48, 324 without). Few columns: two launches that leave no wait between them (100003 x 5 fp32: 3.9 and 5.0 us).
+// of 48, 324 in one). Few columns: two launches that leave no wait between them (100003 x 5 fp32: 3.9 and 5.0 us).
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
@@ -28,6 +28,11 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // workgroup of its own takes about 20 us, and below this many columns the chunks win (131072 bf16 rows: 64 columns 22 us
 // against 17, 128 columns 24 against 22, 256 columns 33 against 45).
 constexpr int kColumnsMin = 160;
+// Columns of more than 256 KiB put their first vectors of eight into LDS, up to so many per thread (128 or 144 KiB): 1000 columns of
+// 200064 bf16 rows 180 us, in chunks 238; 151936 rows 145 and 186; 70000 fp32 rows x 2048 columns 248 and 322. (A second round of
+// the 256 CUs that is nearly empty costs some of it: 300 columns of 160000 rows 65 and 58.)
+template <class T>
+constexpr int kInLds = sizeof(T) == 2 ? 9 : 4;
 // With the log-sums kept from an earlier call, columns of up to so many bytes (16384 columns bf16: 1000 rows 18 us against 38 by
 // chunks, 2000 rows 35 against 50, 4000 rows 67 against 61).
 constexpr size_t kKeptBytes = 6 << 10;
@@ -349,16 +354,18 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
 }
 
 // A whole column in the registers of one workgroup of BLOCK threads, NV vectors of eight logits each: read once, written
-// once; or the gradient alone, where log-sums are given. The last wave takes the teacher's entries before its share of the column. Log-sums run along with the loads;
+// once; or the gradient alone, where log-sums are given. LV more vectors wait in LDS, each read back by the thread that put it
+// there. The last wave takes the teacher's entries before its share of the column. Log-sums run along with the loads;
 // afterwards the logits are still there as they were read.
 // An entry's gradient goes over the one written for its row by the wave that wrote that one, whose stores take effect
 // in order: no barrier has to wait for the column's stores.
-template <class T, int BLOCK, int NV>
+template <class T, int BLOCK, int NV, int LV>
 __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* at) {
     constexpr int WAVES = BLOCK / 64;
     __shared__ LogSum sh[WAVES];
     __shared__ Teacher teacher;
     __shared__ unsigned table[kTableWords];
+    __shared__ Raw8<T> kept_here[LV > 0 ? LV : 1][LV > 0 ? BLOCK : 1];
     const long long c = blockIdx.x;
     const int t = threadIdx.x, lane = t & 63, wave = wave_uniform(t >> 6), n = a.nrows;
     const float it = 1.f / a.temperature, k = it * kLog2e;
@@ -368,10 +375,21 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
         if (lane == 0) teacher = r;
     }
     Raw8<T> x[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) x[v] = load_col8(z, (v * BLOCK + t) * 8, n, (T)(-INFINITY));
     const bool kept = a.lse_in != nullptr;
     LogSum s = {-INFINITY, 0.f};
+    if constexpr (LV > 0) {
+        Raw8<T> y[LV];
+#pragma unroll
+        for (int v = 0; v < LV; ++v) y[v] = load_col8(z, (v * BLOCK + t) * 8, n, (T)(-INFINITY));
+#pragma unroll
+        for (int v = 0; v < LV; ++v) {
+            s = add_eight(s, y[v].wide(), k);
+            kept_here[v][t] = y[v];
+        }
+        asm volatile("" : "+s"(z) : "v"(s.sum) : "memory");          // the rest is loaded when these registers are free
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v] = load_col8(z, ((LV + v) * BLOCK + t) * 8, n, (T)(-INFINITY));
     if (kept) {
         __syncthreads();
     } else {
@@ -396,16 +414,21 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     const bool first = !none && e0 + lane < e1;
     const int r0 = first ? a.tir[e0 + lane] : -1;
     const float x0 = first ? at[e0 + lane] : 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
+    int again = t;
+    asm volatile("" : "+v"(again));          // read from LDS again, not kept in registers from above
+    auto put = [&](const Raw8<T>& z8, int v) {
         float8_t d = (float8_t)(0.f);
         if (!none) {
-            const float8_t y = x[v].wide();
+            const float8_t y = z8.wide();
 #pragma unroll
             for (int j = 0; j < 8; ++j) d[j] = w * q(y[j]);
         }
         store_col8(dz, (v * BLOCK + t) * 8, n, d);
-    }
+    };
+#pragma unroll
+    for (int v = 0; v < LV; ++v) put(kept_here[v][again], v);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) put(x[v], LV + v);
     if (none) return;
     for (int j = e0 + lane; j < e1; j += 64) {
         const int r = j < e0 + 64 ? r0 : a.tir[j];
@@ -414,16 +437,16 @@ __global__ __launch_bounds__(BLOCK) void k_distill_column(DistillArgs a, float* 
     }
 }
 
-template <class T, int BLOCK, int NV>
+template <class T, int BLOCK, int NV, int LV = 0>
 hipError_t launch_column(const DistillArgs& a, float* at, hipStream_t s) {
-    hipLaunchKernelGGL((k_distill_column<T, BLOCK, NV>), dim3((unsigned)a.ncols), dim3(BLOCK), 0, s, a, at);
+    hipLaunchKernelGGL((k_distill_column<T, BLOCK, NV, LV>), dim3((unsigned)a.ncols), dim3(BLOCK), 0, s, a, at);
     return hipGetLastError();
 }
 template <class T>
 bool by_column(const DistillArgs& a) {
     const size_t bytes = sizeof(T) * (size_t)a.nrows;
     if (a.lse_in != nullptr) return bytes <= kKeptBytes;
-    return (bytes <= (128 << 10) || (bytes <= (256 << 10) && a.ncols >= kColumnsMin));
+    return bytes <= (128 << 10) || (bytes <= (256 << 10) + kInLds<T> * 1024 * 8 * sizeof(T) && a.ncols >= kColumnsMin);
 }
 template <class T>
 hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {
@@ -446,6 +469,9 @@ hipError_t distill_columns(const DistillArgs& a, float* at, hipStream_t s) {
     if (vecs <= 1024 * M) return launch_column<T, 512, M * 2>(a, at, s);
     if (vecs <= 1536 * M) return launch_column<T, 1024, M * 3 / 2>(a, at, s);
     if (vecs <= 2048 * M) return launch_column<T, 1024, M * 2>(a, at, s);
+    if constexpr (sizeof(T) == 2)
+        if (vecs <= 1024 * (2 * M + 4)) return launch_column<T, 1024, M * 2, 4>(a, at, s);
+    if (vecs <= 1024 * (2 * M + kInLds<T>)) return launch_column<T, 1024, M * 2, kInLds<T>>(a, at, s);
     return hipErrorInvalidValue;
 }
 

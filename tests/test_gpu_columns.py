@@ -484,6 +484,15 @@ def test_distill_repeated_rows_add(hip, t, V):
     distill_case(hip, rng, V, 6, t, [9, 64, 65, 300, 0, 2], repeats=True, sort=False, in_place=True)
 
 
+# Many columns too tall for a workgroup's registers: the first part waits in LDS; the tallest are cut into chunks.
+@pytest.mark.parametrize("V,t", [(65544, 0), (98304, 0), (98305, 0), (131073, 2), (163840, 1), (163841, 2), (204800, 1), (204801, 2)])
+def test_distill_tall_columns(hip, V, t):
+    rng = np.random.default_rng(V)
+    m = 160
+    lengths = rng.integers(0, 30, m)
+    distill_case(hip, rng, V, m, t, lengths, tau=1.5, weight=rng.random(m), sort=False, repeats=True, in_place=V % 2 == 0)
+
+
 def test_distill_long_teacher_columns(hip):
     rng = np.random.default_rng(50)
     distill_case(hip, rng, 9000, 3, 0, [9000, 5000, 3], sort=True)
