@@ -24,6 +24,11 @@ namespace {
 
 // Columns of S per launch, and segments at most: together they stay below 2^32 threads.
 constexpr int kSlab = 1 << 24, kSegsMax = 1 << 25;
+// Few nonzeros: segments are halved, down to kSegMin, until there are kWavesMin of them, since a wave's nonzeros follow one
+// another with the whole way to memory (k = 612, 800 nonzeros in 63 columns of power-law lengths: 12 us, 28 with segments of
+// 128; k = 1650, 4300 in 717: 17 and 60; for 2048 waves k = 1024, 2000 columns of 40: 27 against 20). Workgroups that add
+// partial sums, at least as many, where there are so many columns.
+constexpr int kSegMin = 16, kWavesMin = 1024, kLookWgs = 2048;
 
 struct Q8Args {
     int k, ncols, nnz, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
@@ -174,8 +179,9 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
         hi = end - lo > a.seglen ? lo + a.seglen : end;
         out = a.partial + w * a.k;
     }
-    for (int k0 = 0; k0 < a.k; k0 += 16 * LPN) {
-        const int i = k0 + 16 * l, left = a.k - i;
+    // (long columns of A: workgroups of their own for every 1024 rows, k = 2500, 10000 columns of 40: 228 us, one after another 276)
+    for (long long from = (long long)blockIdx.y * 16 * LPN; from < a.k; from += (long long)gridDim.y * 16 * LPN) {
+        const int k0 = (int)from, i = k0 + 16 * l, left = a.k - i;
         const int sg = a.shift < 31 && left > 0 ? i >> a.shift : 0;
         float acc[16];
 #pragma unroll
@@ -233,15 +239,14 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
     }
 }
 
-// C[:,c] += the partial sums of column c's segments, in order. A workgroup looks at kLook columns and adds those that were
+// C[:,c] += the partial sums of column c's segments, in order. A workgroup looks at `look` columns and adds those that were
 // cut with all of its threads, W rows each (k = 1024: 15 us with four rows, 27 with one; k = 250: one is 2 us faster).
-constexpr int kLook = 16;
 template <int W>
-__global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
+__global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a, int look) {
     const int lane = threadIdx.x & 63;
-    const long long first = (long long)blockIdx.x * kLook;
+    const long long first = (long long)blockIdx.x * look;
     bool long_ = false;
-    if (lane < kLook && first + lane < a.ncols) long_ = a.jc[first + lane + 1] - a.jc[first + lane] > a.seglen;
+    if (lane < look && first + lane < a.ncols) long_ = a.jc[first + lane + 1] - a.jc[first + lane] > a.seglen;
     for (unsigned long long cut = __ballot(long_); cut != 0; cut &= cut - 1) {
         const long long c = first + __builtin_ctzll(cut);
         const int s0 = segment_from(a, a.jc[c]);
@@ -274,7 +279,8 @@ __global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a) {
 
 template <int LPN, bool STAGED = false>
 hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
-    hipLaunchKernelGGL((k_dsmult_q8<LPN, STAGED>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK)), dim3(BM_BLOCK), 0, s, a);
+    hipLaunchKernelGGL((k_dsmult_q8<LPN, STAGED>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK), (unsigned)std::min((a.k + 16LL * LPN - 1) / (16 * LPN), 65535LL)),
+                       dim3(BM_BLOCK), 0, s, a);
     return hipGetLastError();
 }
 
@@ -295,6 +301,7 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     a.partial = nullptr;
     a.nsegs = 0;
     hipError_t err;
+    while (a.seglen > kSegMin && nnz < kWavesMin * (long long)a.seglen) a.seglen >>= 1;
     if (nnz > a.seglen) {
         a.nsegs = (nnz + a.seglen - 1) / a.seglen;
         a.partial = (float*)ws_get(WS_PARTIAL, sizeof(float) * (size_t)a.nsegs * (size_t)k, &err, s);
@@ -313,7 +320,8 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     else if (nnz < 12LL * ncols) err = launch_q8<64, true>(a, nwaves, s);
     else err = launch_q8<64>(a, nwaves, s);
     if (err == hipSuccess && a.nsegs > 0) {
-        hipLaunchKernelGGL((k > BM_BLOCK ? k_add_segments<4> : k_add_segments<1>), dim3((unsigned)(((long long)ncols + kLook - 1) / kLook)), dim3(BM_BLOCK), 0, s, a);
+        const int look = std::min(std::max(ncols / kLookWgs, 1), 16);
+        hipLaunchKernelGGL((k > BM_BLOCK ? k_add_segments<4> : k_add_segments<1>), dim3((unsigned)((ncols + look - 1LL) / look)), dim3(BM_BLOCK), 0, s, a, look);
         err = hipGetLastError();
     }
     return err;
