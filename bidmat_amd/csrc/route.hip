@@ -18,7 +18,8 @@
 // error; only a column with another key within that bound of the border is decided from keys in fp64 (take_exact).
 // 256 experts in 8 groups, 65536 columns bf16, 8 taken: 43 us with 16 lanes per column, 200 vector and 46 scalar instructions
 // per column (a wave per column 80 us; its bytes alone would take 8 us); 60 experts, 32768 columns fp32: 13 us, and 4 us to
-// add up the counts. Above 256 experts a wave per column: 512 experts, 32768 columns fp32 45 us, 1000 experts, 16384 columns 48 us.
+// add up the counts; 512 experts, 32768 columns fp32: 34 us. Above 512 experts, or more than 16 taken, a wave per column: 1000
+// experts, 16384 columns 48 us.
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
@@ -475,8 +476,8 @@ __device__ __forceinline__ void exact_column(const RouteArgs& a, const Deal& d, 
 }
 
 // ---- 16 lanes per column
-// The same for up to 256 experts in up to 16 groups and up to 16 of them taken: four columns per wave, so that what lanes do
-// together costs a quarter per column and needs no step across rows of 16 lanes. A lane holds up to 16 experts; counts
+// The same for up to 512 experts in up to 16 groups and up to 16 of them taken: four columns per wave, so that what lanes do
+// together costs a quarter per column and needs no step across rows of 16 lanes. A lane holds up to 32 experts; counts
 // run on the vector unit (a compare and an addition per slot).
 template <int CTRL>
 __device__ __forceinline__ int row_move(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true); }
@@ -553,7 +554,7 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             int k = ordered(z[j]);
-            if constexpr (sizeof(T) == 2) k = ((k >> (__is_same(T, f16_t) ? 13 : 16)) << 8) | (255 - first - j);
+            if constexpr (sizeof(T) == 2) k = ((k >> (__is_same(T, f16_t) ? 13 : 16)) << 9) | (511 - first - j);
             key[j] = z[j] > -INFINITY ? k : kShut;
         }
     } else {
@@ -691,7 +692,7 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
 template <class T, int VPL, int BLOCK, bool ONE>
 __global__ __launch_bounds__(BLOCK) void k_route_rows(RouteArgs a, Deal d, Deal d64, int* shares) {
     constexpr int WAVES = BLOCK / 64;
-    __shared__ int hist[256];
+    __shared__ int hist[16 * VPL < 256 ? 256 : 16 * VPL];
     __shared__ Chosen chosen[WAVES];
     __shared__ int two_largest[WAVES][4][16];
     extern __shared__ double exact_keys[];      // 64 * d64.each per wave
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(BLOCK) void k_route_rows(RouteArgs a, Deal d, Deal 
             int upto = row_prefix(__popc(taken));
             const int have = row_sum(__popc(taken));
             if (__ballot(have < a.topk) != 0) {
-                unsigned rest = own > 0 ? ~taken & ((1u << own) - 1u) : 0u;
+                unsigned rest = own > 0 ? ~taken & (own >= 32 ? ~0u : (1u << own) - 1u) : 0u;
                 int left = a.topk - have - (row_prefix(__popc(rest)) - __popc(rest));
                 for (; rest != 0 && left > 0; rest &= rest - 1, --left) taken |= rest & -rest;
                 upto = row_prefix(__popc(taken));
@@ -942,7 +943,7 @@ hipError_t launch_route(const RouteArgs& a, Deal d, hipStream_t s) {
 template <class T, int VPL>
 hipError_t launch_route_rows(const RouteArgs& a, Deal d, const Deal& d64, hipStream_t s) {
     const size_t keys = 64 * sizeof(double) * d64.each;      // of one wave
-    if (a.ncols <= kOneRows) {
+    if constexpr (VPL <= 16) if (a.ncols <= kOneRows) {
         d.batch = 4;
         hipLaunchKernelGGL((k_route_rows<T, VPL, 1024, true>), dim3(1), dim3(1024), 16 * keys, s, a, d, d64, (int*)nullptr);
         return hipGetLastError();
@@ -972,13 +973,15 @@ Deal deal(const RouteArgs& a, int lanes) {
 template <class T>
 hipError_t route_typed(const RouteArgs& a, hipStream_t s) {
     const Deal d = deal(a, 64), d16 = deal(a, 16);
-    // four columns per wave, once a workgroup's sixteen waves have a column each
-    if (a.ncols > 16 && d16.each <= 16 && a.nexperts <= 256 && a.topk <= 16) {
+    // four columns per wave, once a workgroup's sixteen waves have a column each (with up to 32 experts in a lane, four times as
+    // many: 512 experts, 17 columns 15.7 us, by a wave per column 12.2, 100 columns 15.5 and 16.6, 32768 columns bf16 48 and 70)
+    if (a.ncols > (d16.each <= 16 ? 16 : 64) && d16.each <= 32 && a.nexperts <= 512 && a.topk <= 16) {
         if (d16.each <= 1) return launch_route_rows<T, 1>(a, d16, d, s);
         if (d16.each <= 2) return launch_route_rows<T, 2>(a, d16, d, s);
         if (d16.each <= 4) return launch_route_rows<T, 4>(a, d16, d, s);
         if (d16.each <= 8) return launch_route_rows<T, 8>(a, d16, d, s);
-        return launch_route_rows<T, 16>(a, d16, d, s);
+        if (d16.each <= 16) return launch_route_rows<T, 16>(a, d16, d, s);
+        return launch_route_rows<T, 32>(a, d16, d, s);
     }
     if (d.each <= 1) return launch_route<T, 1>(a, d, s);
     if (d.each <= 2) return launch_route<T, 2>(a, d, s);

@@ -364,6 +364,23 @@ def test_route_few_columns(hip, E, groups, tg, k, m):
         route_case(hip, rng, E, m, t, 1, np.zeros(E, np.float32), groups, tg, k, True, Z=steps)
 
 
+# Up to 32 experts in a lane: ties (decided in 64 bits), closed columns, biases, every kind of weights.
+@pytest.mark.parametrize("E,groups,tg,k", [(272, 1, 1, 5), (300, 4, 3, 16), (384, 8, 4, 8), (512, 16, 5, 16), (512, 1, 1, 1), (511, 7, 2, 9)])
+def test_route_up_to_512_experts(hip, E, groups, tg, k):
+    rng = np.random.default_rng(E + k)
+    m = 260
+    for t in TYPES:
+        for kind in (0, 1):
+            route_case(hip, rng, E, m, t, kind, True, groups, tg, k, True)
+            route_case(hip, rng, E, m, t, kind, None, groups, tg, k, False, pad=1, shift=1)
+            steps = np.round(rng.standard_normal((m, E)) * 2) / 2
+            steps[rng.random((m, E)) < 0.3] = -np.inf
+            steps[5] = -np.inf
+            steps[6, 3:] = -np.inf
+            route_case(hip, rng, E, m, t, kind, None, groups, tg, k, True, Z=steps)
+            route_case(hip, rng, E, m, t, kind, np.zeros(E, np.float32), groups, tg, k, True, Z=steps)
+
+
 def route_grad_case(hip, rng, E, m, t, kind, k, renorm, pad=0, shift=0, in_place=False, Z=None):
     z = rng.standard_normal((m, E)) * 1.5 if Z is None else Z
     d, G, ir = route_case(hip, rng, E, m, t, kind, True, 1, 1, k, renorm, pad, shift, Z=z)
