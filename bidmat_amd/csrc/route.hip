@@ -542,19 +542,34 @@ __device__ __forceinline__ void row_before(int key, int& before) {
     }
 }
 
-// Exact keys (scores of 16 bits, no bias, no groups) get the expert's number into their lower bits, so that no two are
-// equal and the lower expert stands higher. Other keys are p + bias + bmax: never negative, so that their bits are in
-// order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
+// Scores as keys: those of 16 bits get the expert's number into their lower bits, so that no two are equal and the lower
+// expert stands higher. score_key: the lowest key that a score of at least x can have.
+template <class T> constexpr int kScoreShift = sizeof(T) == 4 ? 0 : __is_same(T, f16_t) ? 13 : 16;
+template <class T>
+__device__ __forceinline__ float key_score(int key) {
+    if constexpr (sizeof(T) == 4) return number(key);
+    const int o = (int)((unsigned)(key >> 9) << kScoreShift<T>);
+    return number(o < 0 ? o | ((1 << kScoreShift<T>) - 1) : o);
+}
+template <class T>
+__device__ __forceinline__ int score_key(float x) {
+    const int o = ordered(x);
+    if constexpr (sizeof(T) == 4) return o;
+    return ((o < 0 ? o : o + (1 << kScoreShift<T>) - 1) >> kScoreShift<T>) * 512;
+}
+
+// Without a bias the scores themselves are compared: p rises with them. Other keys are p + bias + bmax: never negative, so that
+// their bits are in order as they are. Returns the taken slots; fine = false where a key lies too close to a border.
 template <class T, int VPL>
 __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, const float (&z)[VPL], const float (&bias)[VPL], float bmax,
                                              float top, float by, int first, bool shut, int* sixteen, bool& fine) {
-    const bool plain = a.bias == nullptr && a.ngroups == 1;
+    const bool direct = a.bias == nullptr;
     int key[VPL];
-    if (plain) {
+    if (direct) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             int k = ordered(z[j]);
-            if constexpr (sizeof(T) == 2) k = ((k >> (__is_same(T, f16_t) ? 13 : 16)) << 9) | (511 - first - j);
+            if constexpr (sizeof(T) == 2) k = (int)((unsigned)(k >> kScoreShift<T>) << 9) | (511 - first - j);
             key[j] = z[j] > -INFINITY ? k : kShut;
         }
     } else {
@@ -589,8 +604,14 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
         if (d.lanes >= 2) merge(row_move<DPP_QUAD_XOR1>(b1), row_move<DPP_QUAD_XOR1>(b2));
         if (d.lanes >= 4) merge(row_move<DPP_QUAD_XOR2>(b1), row_move<DPP_QUAD_XOR2>(b2));
         if (d.lanes >= 8) merge(row_move<DPP_ROW_HALF_MIRROR>(b1), row_move<DPP_ROW_HALF_MIRROR>(b2));
+        float p1 = __int_as_float(b1), p2 = __int_as_float(b2);
+        if (direct) {
+            const float z1 = key_score<T>(b1), z2 = key_score<T>(b2);
+            p1 = a.kind == 0 ? __builtin_amdgcn_exp2f((z1 - top) * kLog2e) * by : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z1 * kLog2e));
+            p2 = a.kind == 0 ? __builtin_amdgcn_exp2f((z2 - top) * kLog2e) * by : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z2 * kLog2e));
+        }
         // each key carries bmax once: a group with a single open expert gets its second one here
-        const float score = b1 == kShut ? -INFINITY : __int_as_float(b1) + (b2 == kShut ? bmax : __int_as_float(b2));
+        const float score = b1 == kShut ? -INFINITY : p1 + (b2 == kShut ? bmax : p2);
         const float e = 2.f * fminf(2.f * most + 0x1p-22f * score, 0x1p-14f * score);
         int reach = 0, pass = 0;
         switch (d.lanes) {
@@ -681,7 +702,13 @@ __device__ __forceinline__ unsigned take_row(const RouteArgs& a, const Deal& d, 
     for (int j = VPL - 1; j >= 0; --j) taken = taken + taken + (unsigned)(key[j] >= lo);      // lo is above kShut, INT_MAX without open keys
     const int have = row_sum(__popc(taken));
     if (have != n) fine = false;                 // equal keys at the border
-    if (!plain) {
+    if (direct && a.ngroups > 1 && have > 0) {
+        // the values p in 64 bits are in the scores' order unless they saturate or two scores nearly meet at the border
+        const float t = key_score<T>(lo);
+        if (!(a.kind == 0 ? t - top > -700.f : t > -700.f && t < 20.f)) fine = false;
+        if (row_count(key, score_key<T>(t - 0x1p-20f)) != row_count(key, score_key<T>(t))) fine = false;
+    }
+    if (!direct) {
         // no other key within the errors of two keys below the smallest taken one
         const float t = __int_as_float(lo), e = 2.f * fminf(most, 0x1p-15f * t);
         if (row_count(key, max(kShut + 1, __float_as_int(t - e))) != have) fine = false;

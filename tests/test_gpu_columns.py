@@ -381,6 +381,25 @@ def test_route_up_to_512_experts(hip, E, groups, tg, k):
             route_case(hip, rng, E, m, t, kind, np.zeros(E, np.float32), groups, tg, k, True, Z=steps)
 
 
+# Groups without a bias compare p = softmax or sigmoid in 64 bits, where it saturates (ties go to the lower expert) and where
+# scores differ by less than it can show.
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("E,groups,tg,k", [(64, 4, 2, 6), (256, 4, 3, 10), (172, 4, 4, 12), (480, 8, 5, 16)])
+def test_route_scores_whose_values_meet(hip, E, groups, tg, k, kind):
+    rng = np.random.default_rng(E + kind)
+    m = 210
+    z = rng.standard_normal((m, E))
+    z[::7] = rng.choice([15, 19.5, 20.5, 25, 36, 37, 40, 50, 60, 100], (len(z[::7]), E))
+    z[1::7] = -rng.choice([0, 600, 690, 710, 730, 744, 746, 760, 900, 2000], (len(z[1::7]), E))
+    z[2::7] = rng.integers(-20, 20, (len(z[2::7]), E)) * 1e-20
+    z[3::7] = 1 + rng.integers(-20, 20, (len(z[3::7]), E)) * 2.0 ** -23
+    z[4::7] = np.round(z[4::7] * 4) / 4
+    z[5::7] = -8 + rng.integers(-20, 20, (len(z[5::7]), E)) * 2.0 ** -6
+    for t in TYPES:
+        for renorm in (False, True):
+            route_case(hip, rng, E, m, t, kind, None, groups, tg, k, renorm, Z=z)
+
+
 def route_grad_case(hip, rng, E, m, t, kind, k, renorm, pad=0, shift=0, in_place=False, Z=None):
     z = rng.standard_normal((m, E)) * 1.5 if Z is None else Z
     d, G, ir = route_case(hip, rng, E, m, t, kind, True, 1, 1, k, renorm, pad, shift, Z=z)
