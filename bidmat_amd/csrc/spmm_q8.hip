@@ -32,6 +32,7 @@ constexpr int kSegMin = 16, kWavesMin = 1024, kLookWgs = 2048;
 
 struct Q8Args {
     int k, ncols, nnz, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
+    int row0, row1;                                       // rows of this launch
     int nsegs;                                            // waves in front of the columns', one per multiple of seglen
     long long ldq;
     const unsigned char* Q;
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
         out = a.partial + w * a.k;
     }
     // (long columns of A: workgroups of their own for every 1024 rows, k = 2500, 10000 columns of 40: 228 us, one after another 276)
-    for (long long from = (long long)blockIdx.y * 16 * LPN; from < a.k; from += (long long)gridDim.y * 16 * LPN) {
+    for (long long from = a.row0 + (long long)blockIdx.y * 16 * LPN; from < a.row1; from += (long long)gridDim.y * 16 * LPN) {
         const int k0 = (int)from, i = k0 + 16 * l, left = a.k - i;
         const int sg = a.shift < 31 && left > 0 ? i >> a.shift : 0;
         float acc[16];
@@ -279,9 +280,23 @@ __global__ __launch_bounds__(BM_BLOCK) void k_add_segments(Q8Args a, int look) {
 
 template <int LPN, bool STAGED = false>
 hipError_t launch_q8(const Q8Args& a, long long nwaves, hipStream_t s) {
-    hipLaunchKernelGGL((k_dsmult_q8<LPN, STAGED>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK), (unsigned)std::min((a.k + 16LL * LPN - 1) / (16 * LPN), 65535LL)),
+    hipLaunchKernelGGL((k_dsmult_q8<LPN, STAGED>), dim3((unsigned)((nwaves + BM_WAVES_PER_BLOCK - 1) / BM_WAVES_PER_BLOCK), (unsigned)std::min((a.row1 - a.row0 + 16LL * LPN - 1) / (16 * LPN), 65535LL)),
                        dim3(BM_BLOCK), 0, s, a);
     return hipGetLastError();
+}
+
+hipError_t q8_rows(const Q8Args& a, long long nwaves, hipStream_t s) {
+    const int lanes = pow2ceil((a.row1 - a.row0 + 15) / 16);
+    if (lanes <= 1) return launch_q8<1>(a, nwaves, s);
+    if (lanes <= 2) return launch_q8<2>(a, nwaves, s);
+    if (lanes <= 4) return launch_q8<4>(a, nwaves, s);
+    if (lanes <= 8) return launch_q8<8>(a, nwaves, s);
+    if (lanes <= 16) return launch_q8<16>(a, nwaves, s);
+    if (lanes <= 32) return launch_q8<32>(a, nwaves, s);
+    // Few nonzeros per column: C's stores are what counts (k = 1024, 100000 columns of 2: 123 us staged, 158 not; of 8: 204 and
+    // 223). With more, the gathers do, and they run faster beside the scattered stores (of 16: 329 and 319; 50000 of 32: 297 and 291).
+    if (a.nnz < 12LL * a.ncols) return launch_q8<64, true>(a, nwaves, s);
+    return launch_q8<64>(a, nwaves, s);
 }
 
 }  // namespace
@@ -308,17 +323,18 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
         if (!a.partial) return err;
     }
     const long long nwaves = (long long)ncols + a.nsegs;
-    const int lanes = pow2ceil((k + 15) / 16);
-    if (lanes <= 1) err = launch_q8<1>(a, nwaves, s);
-    else if (lanes <= 2) err = launch_q8<2>(a, nwaves, s);
-    else if (lanes <= 4) err = launch_q8<4>(a, nwaves, s);
-    else if (lanes <= 8) err = launch_q8<8>(a, nwaves, s);
-    else if (lanes <= 16) err = launch_q8<16>(a, nwaves, s);
-    else if (lanes <= 32) err = launch_q8<32>(a, nwaves, s);
-    // Few nonzeros per column: C's stores are what counts (k = 1024, 100000 columns of 2: 123 us staged, 158 not; of 8: 204 and
-    // 223). With more, the gathers do, and they run faster beside the scattered stores (of 16: 329 and 319; 50000 of 32: 297 and 291).
-    else if (nnz < 12LL * ncols) err = launch_q8<64, true>(a, nwaves, s);
-    else err = launch_q8<64>(a, nwaves, s);
+    // Up to 256 rows past a multiple of 1024, which would leave most of a wave without work, get a launch of their own with fewer
+    // lanes per nonzero (600000 nonzeros, k = 1025: 152 us instead of 175, k = 1280: 155 and 164; more rows lose: 1500: 203 and 196),
+    // where the nonzeros are worth one (1500 nonzeros, k = 1056: 15 us, in one launch 12).
+    const int tail = k > 1024 && k % 1024 <= 256 && nnz >= (1 << 16) ? k % 1024 : 0;
+    a.row0 = 0;
+    a.row1 = k - tail;
+    err = q8_rows(a, nwaves, s);
+    if (err == hipSuccess && tail > 0) {
+        a.row0 = k - tail;
+        a.row1 = k;
+        err = q8_rows(a, nwaves, s);
+    }
     if (err == hipSuccess && a.nsegs > 0) {
         const int look = std::min(std::max(ncols / kLookWgs, 1), 16);
         hipLaunchKernelGGL((k > BM_BLOCK ? k_add_segments<4> : k_add_segments<1>), dim3((unsigned)((ncols + look - 1LL) / look)), dim3(BM_BLOCK), 0, s, a, look);

@@ -710,6 +710,17 @@ def test_dsmult_q8_heights(hip, k, group):
     q8_case(hip, rng, k, 9, [1], group)
 
 
+# More rows than a wave takes at once, and enough nonzeros for the rest to be a launch of its own.
+@pytest.mark.parametrize("k,group", [(1025, 0), (1040, 32), (1280, 128), (1281, 64), (2049, 0), (2304, 32)])
+@pytest.mark.parametrize("beta", [0, 1])
+def test_dsmult_q8_rows_past_a_wave(hip, k, group, beta):
+    rng = np.random.default_rng(k)
+    lengths = rng.integers(0, 90, 1500)
+    lengths[[3, 700]] = 700
+    assert lengths.sum() >= 65536
+    q8_case(hip, rng, k, 40, lengths, group, beta=beta, pad=3, shift=1)
+
+
 def test_dsmult_q8_more_columns_than_a_launch_takes(hip):
     rng = np.random.default_rng(73)
     m, rows, long = (1 << 24) + 777, 50, 3000
