@@ -107,13 +107,18 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
     }
     if (a.Y == nullptr && a.Q == nullptr) return;
     ss = column_allsum<TPC>(ss, sh[0]);
-    float rs = 1.f / sqrtf(ss / (float)n + a.eps);
-    if (ss == INFINITY) {
-        // squares beyond fp32: the same from h * 2^-64, where eps is nothing (an infinite h leaves rs = 0)
+    const float d = ss / (float)n + a.eps;
+    float rs = 1.f / sqrtf(d);
+    if (!(d < INFINITY)) {
+        // the sum leaves fp32: again from h * 2^-96, whose squares stay inside with every row at its largest (an infinite h leaves
+        // rs = 0). The two factors of y take half of it each, so that neither has few digits.
         float small = 0.f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) small += square_sum(h[v] * 0x1p-64f);
-        rs = 0x1p-64f / sqrtf(column_allsum<TPC>(small, sh[2]) / (float)n);
+        for (int v = 0; v < NV; ++v) {
+            h[v] = h[v] * 0x1p-48f;
+            small += square_sum(h[v] * 0x1p-48f);
+        }
+        rs = 0x1p-48f / sqrtf(column_allsum<TPC>(small, sh[2]) / (float)n + a.eps * 0x1p-96f * 0x1p-96f);
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
