@@ -166,7 +166,7 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 template <class T, int TPC, int NV, bool RAGGED>
 __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
     constexpr int CPB = norm_block(TPC) / TPC;
-    __shared__ float sh[2][3][TPC > 64 ? TPC / 64 : 1];
+    __shared__ float sh[2][4][TPC > 64 ? TPC / 64 : 1];
     const int t = threadIdx.x % TPC, n = a.nrows;
     float8_t dw[NV];
 #pragma unroll
@@ -213,22 +213,34 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
         }
         hh = column_allsum<TPC>(hh, sh[turn][0]);
         gh = column_allsum<TPC>(gh, sh[turn][1]);
-        float rs = 1.f / sqrtf(hh / (float)n + a.eps);
-        if (hh == INFINITY) {          // as in k_rmsnorm
+        const float dd = hh / (float)n + a.eps;
+        float rs = 1.f / sqrtf(dd), by = 1.f;          // u = h * by * rs
+        if (!(dd < INFINITY)) {          // as in k_rmsnorm
+            by = 0x1p-48f;
             float small = 0.f;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) small += square_sum(hc[v].wide() * 0x1p-64f);
-            rs = 0x1p-64f / sqrtf(column_allsum<TPC>(small, sh[turn][2]) / (float)n);
+            for (int v = 0; v < NV; ++v) small += square_sum(hc[v].wide() * 0x1p-96f);
+            rs = 0x1p-48f / sqrtf(column_allsum<TPC>(small, sh[turn][2]) / (float)n + a.eps * 0x1p-96f * 0x1p-96f);
+        }
+        float mean = gh / (float)n * rs;               // of g * u
+        if (!(fabsf(gh) < INFINITY) || by != 1.f) {    // products beyond fp32, where those with u are not
+            mean = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const float8_t u = hc[v].wide() * by * rs * (1.f / (float)n), y = gc[v].wide() * (AHEAD ? w[v] : weight(v));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mean = fmaf(u[j], y[j], mean);
+            }
+            mean = column_allsum<TPC>(mean, sh[turn][3]);
         }
         turn ^= 1;
-        const float k = gh / (float)n * rs * rs;
         T* o = (T*)a.dX + c * a.lddx;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int i = (v * TPC + t) * 8;
-            const float8_t x = hc[v].wide(), y = gc[v].wide();
-            float8_t d = rs * (y * (AHEAD ? w[v] : weight(v)) - x * k);
-            dw[v] += y * x * rs;
+            const float8_t u = hc[v].wide() * by * rs, y = gc[v].wide();
+            float8_t d = rs * (y * (AHEAD ? w[v] : weight(v)) - u * mean) * by;
+            dw[v] += y * u;
             if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : settle_col8<RAGGED>(fetch_col8<RAGGED>((const T*)a.dH + c * a.lddh, i, n), i, n).wide();
             put_col8<RAGGED>(o, i, n, d);
         }

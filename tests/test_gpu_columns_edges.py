@@ -38,3 +38,42 @@ def test_rmsnorm_of_the_largest_values(hip, n, t):
     for eps in (0.0, 1e-5, 1e36, 3.4e38):
         for group in (0, 32):
             norm_case(hip, rng, n, 6, t, False, True, True, group, x=x, eps=eps)
+
+
+def grad_edge(hip, H, dY, w, eps, t):
+    m, n = H.shape
+    w = w.astype(F)
+    H, dY = encode(H, t), encode(dY, t)
+    h, dy, dx, dw, dww = Columns(H), Columns(dY), empty(m, n, np_type(t)), dev(w), dev(np.zeros(n, F))
+    ok(hip.bidmat_rmsnorm_grad(n, m, t, h.ptr, n, dw.ptr, eps, dy.ptr, n, None, n, dx.ptr, n, dww.ptr, 0, None))
+    want, wantw, size, sizew = ref.rmsnorm_grad(decode(H, t), w.astype(np.float64), float(F(eps)), decode(dY, t), None)
+    with np.errstate(over="ignore"):
+        fits = np.abs(want) * (1 + 2.0 ** -7) < MOST[t]          # the rest may be rounded to an infinity
+    got = decode(dx.get(), t)
+    within(np.where(fits, got, 0), np.where(fits, want, 0), HALF_STEP[t] * 1.01 * np.abs(want) + TINY[t] + 2 * NORM_DEPTH * EPS24 * size, "dx")
+    within(dww.numpy().astype(np.float64), wantw, (NORM_DEPTH + 48) * EPS24 * sizew + 2.0 ** -149, "dw")
+
+
+def grad_edges(hip, h, g, w, t, scales):
+    """Columns one by one (so that none hides behind another in dw) and together."""
+    for eps in scales:
+        for c in range(len(h)):
+            grad_edge(hip, h[c:c + 1], g[c:c + 1], w, eps, t)
+        grad_edge(hip, h, g, w, eps, t)
+
+
+@pytest.mark.parametrize("n", HEIGHTS + [20000])
+@pytest.mark.parametrize("t", [0, 2])
+def test_rmsnorm_grad_of_the_largest_values(hip, n, t):
+    """Sums of squares and of products that leave fp32, h aligned with the gradient or not."""
+    rng = np.random.default_rng(n * 2 + t)
+    w = 1 + 0.1 * rng.standard_normal(n)
+    sign = np.sign(rng.standard_normal((7, n)))
+    h, g = sign * (0.5 + rng.random((7, n))), rng.standard_normal((7, n))
+    h[0], g[0] = 1e35, 1
+    h[1], g[1] = MOST[t] * sign[1], sign[1]
+    h[2, n // 2], g[2, n // 2] = 2e38, 2
+    h[3] = 1e37
+    h[4], g[4] = 1e3, 1e36
+    h[5] *= 1e19
+    grad_edges(hip, h, g, w, t, (0.0, 1e-5, 1e36))
