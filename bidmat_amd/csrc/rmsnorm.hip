@@ -39,6 +39,17 @@ __device__ __forceinline__ float abs_max(float8_t x) {
     return s;
 }
 
+// The sum of a column's squares may leave fp32 on either side: d = mean(h^2) + eps is infinite, or so small (below 2^-126) that
+// squares which count in it have few digits or vanished. It is taken again from h * by * rest = h * 2^-96 or h * 2^96, whose
+// squares and their sums stay inside for every h of fp32, and y = (h * by) * rs * w: with h of the largest values half of the
+// factor stays with rs, so that neither it nor h * by has few digits. (An infinite h leaves rs = 0.)
+__device__ __forceinline__ bool in_range(float d) { return d >= 0x1p-126f && d < INFINITY; }
+struct Rescale {
+    float by, rest;
+    __device__ __forceinline__ float rs(float mean, float eps) const { return rest / sqrtf(mean + eps * (by * rest) * (by * rest)); }
+};
+__device__ __forceinline__ Rescale rescale(float d) { return d < 1.f ? Rescale{0x1p96f, 1.f} : Rescale{0x1p-48f, 0x1p-48f}; }
+
 // Eight e4m3 codes (OCP, round to nearest even).
 __device__ __forceinline__ uint2 e4m3_codes(float8_t x) {
     int a = 0, b = 0;
@@ -109,16 +120,15 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
     ss = column_allsum<TPC>(ss, sh[0]);
     const float d = ss / (float)n + a.eps;
     float rs = 1.f / sqrtf(d);
-    if (!(d < INFINITY)) {
-        // the sum leaves fp32: again from h * 2^-96, whose squares stay inside with every row at its largest (an infinite h leaves
-        // rs = 0). The two factors of y take half of it each, so that neither has few digits.
-        float small = 0.f;
+    if (!in_range(d)) {
+        const Rescale r = rescale(d);
+        float sum = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            h[v] = h[v] * 0x1p-48f;
-            small += square_sum(h[v] * 0x1p-48f);
+            h[v] = h[v] * r.by;
+            sum += square_sum(h[v] * r.rest);
         }
-        rs = 0x1p-48f / sqrtf(column_allsum<TPC>(small, sh[2]) / (float)n + a.eps * 0x1p-96f * 0x1p-96f);
+        rs = r.rs(column_allsum<TPC>(sum, sh[2]) / (float)n, a.eps);
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -163,15 +173,77 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 // What bounds it: memory (4096 rows x 16384 columns bf16: 103 us with the shares' addition, 5.2 TB/s). Above 8192 rows a
 // thread's registers do not hold the next column, above 16384 not the present one either (16384 rows x 4096: 125 us, 4.3 TB/s;
 // 32768 x 2048: 227 us, 2.4 TB/s).
+// A column whose sums leave fp32, of squares or of products (which count on the small side where rs is large).
+__device__ __forceinline__ bool outside(float d, float gh) {
+    return !in_range(d) || !(fabsf(gh) < INFINITY) || (d < 0x1p-20f && fabsf(gh) < 0x1p-100f);
+}
+// Those among a workgroup's columns, by the marks that the loop over all of them left: with u = h * by * rs, which is at most
+// sqrt(n), and the mean of g * u. They are read again behind the others, which so keep their registers (within that loop this
+// cost heights above 16384 12 to 46 %), and their part of dw is added to the share in memory, one column after the other.
 template <class T, int TPC, int NV, bool RAGGED>
-__global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
+__device__ __forceinline__ void odd_columns(const NormGradArgs& a, float* share, const unsigned char* marks, float (*sh)[4][TPC > 64 ? TPC / 64 : 1]) {
+    constexpr int CPB = norm_block(TPC) / TPC;
+    const int t = threadIdx.x % TPC, n = a.nrows;
+    int turn = 0;
+    for (long long c0 = (long long)blockIdx.x * CPB; c0 < a.ncols; c0 += (long long)gridDim.x * CPB, marks += CPB)
+        for (int q = 0; q < CPB; ++q) {
+            const long long c = c0 + q;
+            if (c >= a.ncols || marks[q] == 0) continue;          // the same for all threads of the workgroup
+            if (threadIdx.x / TPC == q) {
+                auto part = [&](const auto* col, int v) {
+                    return settle_col8<RAGGED>(fetch_col8<RAGGED>(col, (v * TPC + t) * 8, n), (v * TPC + t) * 8, n).wide();
+                };
+                const T *h = (const T*)a.H + c * a.ldh, *dy = (const T*)a.dY + c * a.lddy;
+                float sum = 0.f, by = 1.f, mean = 0.f;
+#pragma unroll 1
+                for (int v = 0; v < NV; ++v) sum += square_sum(part(h, v));
+                const float d2 = column_allsum<TPC>(sum, sh[turn][0]) / (float)n + a.eps;
+                float rs = 1.f / sqrtf(d2);
+                if (!in_range(d2)) {
+                    const Rescale r = rescale(d2);
+                    by = r.by;
+                    sum = 0.f;
+#pragma unroll 1
+                    for (int v = 0; v < NV; ++v) sum += square_sum(part(h, v) * by * r.rest);
+                    rs = r.rs(column_allsum<TPC>(sum, sh[turn][1]) / (float)n, a.eps);
+                }
+#pragma unroll 1
+                for (int v = 0; v < NV; ++v) {
+                    const float8_t u = part(h, v) * by * rs * (1.f / (float)n), g = part(dy, v) * part(a.w, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mean = fmaf(u[j], g[j], mean);
+                }
+                mean = column_allsum<TPC>(mean, sh[turn][2]);
+#pragma unroll 1
+                for (int v = 0; v < NV; ++v) {
+                    const int i = (v * TPC + t) * 8;
+                    const float8_t u = part(h, v) * by * rs, y = part(dy, v);
+                    float8_t d = rs * (y * part(a.w, v) - u * mean) * by;
+                    if (a.dH != nullptr) d += part((const T*)a.dH + c * a.lddh, v);
+                    put_col8<RAGGED>((T*)a.dX + c * a.lddx, i, n, d);
+                    if (share != nullptr) store_col8(share, i, n, load_col8(share, i, n).wide() + y * u);
+                }
+            }
+            turn ^= 1;
+            if constexpr (CPB > 1) __syncthreads();
+        }
+}
+
+// Columns of one launch, per workgroup at most: a byte marks each of them (LDS).
+constexpr int kNormMarks = 8192;
+
+template <class T, int TPC, int NV, bool RAGGED>
+__global__ __launch_bounds__(norm_block(TPC), 4) void k_rmsnorm_grad(NormGradArgs a, float* partial) {
     constexpr int CPB = norm_block(TPC) / TPC;
     __shared__ float sh[2][4][TPC > 64 ? TPC / 64 : 1];
+    __shared__ unsigned char marks[kNormMarks];
     const int t = threadIdx.x % TPC, n = a.nrows;
     float8_t dw[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) dw[v] = (float8_t)(0.f);
     int turn = 0;
+    bool odd = false;          // a column was left to odd_columns
+    unsigned char* mark = marks + threadIdx.x / TPC;
     // A column's data are requested while the one before is worked on, where a thread's registers hold both.
     constexpr bool AHEAD = TPC < 1024 || NV == 1;
     const long long step = (long long)gridDim.x * CPB;
@@ -212,67 +284,58 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm_grad(NormGradArgs a
             for (int j = 0; j < 8; ++j) gh = fmaf(x[j], y[j], gh);
         }
         hh = column_allsum<TPC>(hh, sh[turn][0]);
+        const float d2 = hh / (float)n + a.eps, rs = 1.f / sqrtf(d2);
         gh = column_allsum<TPC>(gh, sh[turn][1]);
-        const float dd = hh / (float)n + a.eps;
-        float rs = 1.f / sqrtf(dd), by = 1.f;          // u = h * by * rs
-        if (!(dd < INFINITY)) {          // as in k_rmsnorm
-            by = 0x1p-48f;
-            float small = 0.f;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) small += square_sum(hc[v].wide() * 0x1p-96f);
-            rs = 0x1p-48f / sqrtf(column_allsum<TPC>(small, sh[turn][2]) / (float)n + a.eps * 0x1p-96f * 0x1p-96f);
-        }
-        float mean = gh / (float)n * rs;               // of g * u
-        if (!(fabsf(gh) < INFINITY) || by != 1.f) {    // products beyond fp32, where those with u are not
-            mean = 0.f;
+        const float mean = gh / (float)n * rs;          // of g * u
+        const bool out = outside(d2, gh);
+        if (t == 0) *mark = out;
+        mark += CPB;
+        if (TPC >= 64 ? __ballot(out) != 0 : out) {
+            odd = true;
+        } else {
+            T* o = (T*)a.dX + c * a.lddx;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const float8_t u = hc[v].wide() * by * rs * (1.f / (float)n), y = gc[v].wide() * (AHEAD ? w[v] : weight(v));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) mean = fmaf(u[j], y[j], mean);
+                const int i = (v * TPC + t) * 8;
+                const float8_t u = hc[v].wide() * rs, y = gc[v].wide();
+                float8_t d = rs * (y * (AHEAD ? w[v] : weight(v)) - u * mean);
+                dw[v] += y * u;
+                if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : settle_col8<RAGGED>(fetch_col8<RAGGED>((const T*)a.dH + c * a.lddh, i, n), i, n).wide();
+                put_col8<RAGGED>(o, i, n, d);
             }
-            mean = column_allsum<TPC>(mean, sh[turn][3]);
         }
         turn ^= 1;
-        T* o = (T*)a.dX + c * a.lddx;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int i = (v * TPC + t) * 8;
-            const float8_t u = hc[v].wide() * by * rs, y = gc[v].wide();
-            float8_t d = rs * (y * (AHEAD ? w[v] : weight(v)) - u * mean) * by;
-            dw[v] += y * u;
-            if (a.dH != nullptr) d += AHEAD ? rc[v].wide() : settle_col8<RAGGED>(fetch_col8<RAGGED>((const T*)a.dH + c * a.lddh, i, n), i, n).wide();
-            put_col8<RAGGED>(o, i, n, d);
-        }
     }
-    if (a.dw == nullptr) return;
     // a single workgroup's share is the gradient (partial == nullptr)
-    float* share = partial != nullptr ? partial + (size_t)blockIdx.x * n : a.dw;
+    float* share = a.dw == nullptr ? nullptr : partial != nullptr ? partial + (size_t)blockIdx.x * n : a.dw;
     const bool add = partial == nullptr && a.beta != 0;
-    if constexpr (CPB > 1) {
-        // the columns of a wave first, then the workgroup's four waves
-        __shared__ float sum[BM_WAVES_PER_BLOCK][TPC * 8 * NV];
+    if (share != nullptr) {
+        if constexpr (CPB > 1) {
+            // the columns of a wave first, then the workgroup's four waves
+            __shared__ float sum[BM_WAVES_PER_BLOCK][TPC * 8 * NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float d = dw[v][j];
+                for (int j = 0; j < 8; ++j) {
+                    float d = dw[v][j];
 #pragma unroll
-                for (int m = TPC; m < 64; m <<= 1) d += __shfl_xor(d, m, 64);
-                if ((threadIdx.x & 63) < TPC) sum[threadIdx.x >> 6][(v * TPC + t) * 8 + j] = d;
+                    for (int m = TPC; m < 64; m <<= 1) d += __shfl_xor(d, m, 64);
+                    if ((threadIdx.x & 63) < TPC) sum[threadIdx.x >> 6][(v * TPC + t) * 8 + j] = d;
+                }
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += BM_BLOCK) {
+                const float d = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+                share[i] = add ? share[i] + d : d;
             }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += BM_BLOCK) {
-            const float d = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
-            share[i] = add ? share[i] + d : d;
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int i = (v * TPC + t) * 8;
-            store_col8(share, i, n, add ? load_col8(share, i, n).wide() + dw[v] : dw[v]);
+            for (int v = 0; v < NV; ++v) {
+                const int i = (v * TPC + t) * 8;
+                store_col8(share, i, n, add ? load_col8(share, i, n).wide() + dw[v] : dw[v]);
+            }
         }
     }
+    if (__syncthreads_or(odd)) odd_columns<T, TPC, NV, RAGGED>(a, share, marks, sh);
 }
 
 // dw[i] = beta * dw[i] + sum over shares of partial[share][i]: ROWS rows x 1024 / ROWS threads per workgroup; thread (x, y)
@@ -391,10 +454,23 @@ hipError_t rmsnorm(const NormArgs& all, hipStream_t s) {
     return hipSuccess;
 }
 
-hipError_t rmsnorm_grad(const NormGradArgs& a, hipStream_t s) {
-    const int n = a.nrows;
-    NormGrad f{a, s};
-    return a.type == ELEM_F32 ? by_height_grad<float>(n, f) : a.type == ELEM_F16 ? by_height_grad<f16_t>(n, f) : by_height_grad<bf16_t>(n, f);
+hipError_t rmsnorm_grad(const NormGradArgs& all, hipStream_t s) {
+    // columns of one launch: kNormMarks for every workgroup of the largest grid (256 threads and less, and 1024)
+    const int n = all.nrows, slab = kNormMarks * (n <= 2048 ? norm_shares(256) : norm_shares(1024));
+    const long long size = (long long)elem_size(all.type);
+    for (long long c = 0; c < all.ncols; c += slab) {
+        NormGradArgs a = all;
+        a.ncols = (int)(all.ncols - c < slab ? all.ncols - c : slab);
+        a.H = (const char*)all.H + c * all.ldh * size;
+        a.dY = (const char*)all.dY + c * all.lddy * size;
+        if (all.dH) a.dH = (const char*)all.dH + c * all.lddh * size;
+        a.dX = (char*)all.dX + c * all.lddx * size;
+        if (c > 0) a.beta = 1;
+        NormGrad f{a, s};
+        const hipError_t e = a.type == ELEM_F32 ? by_height_grad<float>(n, f) : a.type == ELEM_F16 ? by_height_grad<f16_t>(n, f) : by_height_grad<bf16_t>(n, f);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace bm

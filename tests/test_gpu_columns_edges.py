@@ -40,11 +40,13 @@ def test_rmsnorm_of_the_largest_values(hip, n, t):
             norm_case(hip, rng, n, 6, t, False, True, True, group, x=x, eps=eps)
 
 
-def grad_edge(hip, H, dY, w, eps, t):
+def grad_edge(hip, H, dY, w, eps, t, over=None):
+    """over: what dX lies on ('h' or 'dy')."""
     m, n = H.shape
     w = w.astype(F)
     H, dY = encode(H, t), encode(dY, t)
-    h, dy, dx, dw, dww = Columns(H), Columns(dY), empty(m, n, np_type(t)), dev(w), dev(np.zeros(n, F))
+    h, dy, dw, dww = Columns(H), Columns(dY), dev(w), dev(np.zeros(n, F))
+    dx = h if over == "h" else dy if over == "dy" else empty(m, n, np_type(t))
     ok(hip.bidmat_rmsnorm_grad(n, m, t, h.ptr, n, dw.ptr, eps, dy.ptr, n, None, n, dx.ptr, n, dww.ptr, 0, None))
     want, wantw, size, sizew = ref.rmsnorm_grad(decode(H, t), w.astype(np.float64), float(F(eps)), decode(dY, t), None)
     with np.errstate(over="ignore"):
@@ -55,11 +57,12 @@ def grad_edge(hip, H, dY, w, eps, t):
 
 
 def grad_edges(hip, h, g, w, t, scales):
-    """Columns one by one (so that none hides behind another in dw) and together."""
+    """Columns one by one (so that none hides behind another in dw) and together, the result by itself and in place."""
     for eps in scales:
         for c in range(len(h)):
             grad_edge(hip, h[c:c + 1], g[c:c + 1], w, eps, t)
-        grad_edge(hip, h, g, w, eps, t)
+        for over in (None, "h", "dy"):
+            grad_edge(hip, h, g, w, eps, t, over)
 
 
 @pytest.mark.parametrize("n", HEIGHTS + [20000])
@@ -77,3 +80,48 @@ def test_rmsnorm_grad_of_the_largest_values(hip, n, t):
     h[4], g[4] = 1e3, 1e36
     h[5] *= 1e19
     grad_edges(hip, h, g, w, t, (0.0, 1e-5, 1e36))
+
+
+@pytest.mark.parametrize("n", HEIGHTS)
+@pytest.mark.parametrize("t", [0, 2])
+def test_rmsnorm_of_the_smallest_values(hip, n, t):
+    """Squares that fp32 holds with few digits or as 0, without an eps that would hide it and with one of their size."""
+    rng = np.random.default_rng(n + t)
+    x = np.sign(rng.standard_normal((8, n))) * (0.5 + rng.random((8, n)))
+    x *= np.array([1, 1e-18, 1e-19, 3e-22, 1e-23, 1e-30, 1e-37, 1e-40])[:, None]
+    x[3, 0] = 1e-19
+    for eps in (0.0, 1e-45, 1e-43, 1e-38):
+        for group in (0, 32):
+            norm_case(hip, rng, n, 8, t, False, True, True, group, x=x, eps=eps)
+
+
+@pytest.mark.parametrize("n", HEIGHTS + [20000])
+@pytest.mark.parametrize("t", [0, 2])
+def test_rmsnorm_grad_of_the_smallest_values(hip, n, t):
+    """Squares and products that fp32 holds with few digits or as 0."""
+    rng = np.random.default_rng(n * 2 + t)
+    w = 1 + 0.1 * rng.standard_normal(n)
+    sign = np.sign(rng.standard_normal((6, n)))
+    h, g = sign * (0.5 + rng.random((6, n))), rng.standard_normal((6, n))
+    h[0] *= 1e-23
+    h[1] *= 3e-22
+    h[2], g[2] = 1e-18 * h[2], 1e-27 * sign[2]
+    h[3], g[3] = 1e-41 if t == 0 else 1e-39, 1e-4          # below the normal numbers
+    h[4] *= 1e-19
+    grad_edges(hip, h, g, w, t, (0.0, 1e-45, 1e-38, 1e-5))
+
+
+@pytest.mark.parametrize("t", [0, 2])
+@pytest.mark.parametrize("n,m", [(3, 8500000), (70, 40000), (1001, 5000), (3000, 2500), (9000, 700)])
+def test_rmsnorm_grad_of_columns_out_of_range_among_many(hip, t, n, m):
+    """Columns of many magnitudes, some of which leave fp32 and some of the gradients' products, in every workgroup (and in more
+    columns than one launch takes)."""
+    rng = np.random.default_rng(n)
+    w = 1 + 0.1 * rng.standard_normal(n)
+    h = rng.standard_normal((m, n)).astype(F)
+    g = rng.standard_normal((m, n)).astype(F)
+    odd = rng.random(m) < 0.1
+    h[odd] *= (10.0 ** rng.choice([-30, -25, -21, -12, 19, 25, 35], odd.sum())).astype(F)[:, None]
+    g[rng.random(m) < 0.02] *= F(1e-25)
+    for over in (None, "h", "dy"):
+        grad_edge(hip, h, g, w, 0.0, t, over)
