@@ -125,3 +125,46 @@ def test_rmsnorm_grad_of_columns_out_of_range_among_many(hip, t, n, m):
     g[rng.random(m) < 0.02] *= F(1e-25)
     for over in (None, "h", "dy"):
         grad_edge(hip, h, g, w, 0.0, t, over)
+
+
+# ---------------------------------------------------------------- distillation: the gradient from a kept log-sum
+@pytest.mark.parametrize("V", [70, 1000, 5000, 140000])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
+def test_distill_grad_of_large_logits(hip, V, t, tau):
+    """Common offsets and masks of the type's lowest value: q = exp(x - lse) for the lse that is given, never above 1. A column
+    of masks alone has an lse without the digits of log V: its q are 0 or 1, not infinite."""
+    rng = np.random.default_rng(V)
+    m, k = 6, 9
+    z = rng.standard_normal((m, V))
+    T, ir, jc = teacher(rng, V, [k] * m)
+    z[0] += 1000
+    z[1] = -MOST[t]
+    z[2] = -MOST[t]
+    z[2, ir[2 * k]] = 0.5
+    z[3, rng.choice(V, V // 2, replace=False)] = -MOST[t]
+    z[4] = 30000 + 8 * z[4]
+    a = Columns(encode(z, t))
+    dT, di, dj, loss, lse = dev(T), dev(ir), dev(jc), dev(np.zeros(m, F)), dev(np.zeros(m, F))
+    dZ = empty(m, V, np_type(t))
+    base = (V, m, t, a.ptr, V, ir.size, dT.ptr, di.ptr, dj.ptr, tau, None)
+    ok(hip.bidmat_distill(*base, loss.ptr, lse.ptr, None, V, None))
+    ok(hip.bidmat_distill_grad(*base, lse.ptr, dZ.ptr, V, None))
+    ok(hip.bidmat_distill_grad(*base, lse.ptr, a.ptr, V, None))
+    zd, l = decode(encode(z, t), t), lse.numpy().astype(np.float64)
+    # products of 24-bit numbers are exact in 64 bits, and so is the difference up to its own rounding
+    x = np.minimum((zd - l[:, None] * tau) / tau, 0)
+    q = np.exp(x)
+    p, share, ptot = np.zeros((m, V)), np.zeros((m, V)), np.zeros((m, 1))
+    for c in range(m):
+        s = T[jc[c]:jc[c + 1]].astype(np.float64) / tau
+        e = np.exp(s - s.max())
+        p[c, ir[jc[c]:jc[c + 1]]] = e / e.sum()
+        ptot[c] = np.abs(s).max() + abs(s.max() + np.log(e.sum()))
+    want = tau * (q - p)
+    with np.errstate(invalid="ignore"):
+        eq = np.where(q > 0, q * (8 * np.abs(x) + 20), 0)
+    # a q below 2^-126 (exponent below the normal numbers) is 0: |q - 0| < 2^-126, tau times that in dz
+    bound = HALF_STEP[t] * 1.01 * np.abs(want) + TINY[t] + tau * (2.0 ** -126 + EPS24 * (eq + p * (8 * ptot + 160 + k)))
+    for d in (dZ, a):
+        within(decode(d.get(), t), want, bound, "dz")
