@@ -347,7 +347,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     };
     // Two instructions less per logit where they change nothing: an lse of up to 2^16 is right to 2^-8, so that no q passes 1 by
     // more, and a scale within 2^+-24 goes into the exponent at the cost of less than 2^-20 of the value (50001 x 2048 fp16: 83 us, without 85).
-    if constexpr (ALONE) {
+    if constexpr (KEPT) {
         if (fabsf(q.at) <= 0x1p16f && w >= 0x1p-24f && w <= 0x1p24f) {
             const float up = __log2f(w);
             rows([&](float v) { return __builtin_amdgcn_exp2f(fmaf(fmaf(q.at, q.by, v), k, up)); });

@@ -164,7 +164,7 @@ def test_distill_grad_of_large_logits(hip, V, t, tau):
     want = tau * (q - p)
     with np.errstate(invalid="ignore"):
         eq = np.where(q > 0, q * (8 * np.abs(x) + 20), 0)
-    # a q below 2^-126 (exponent below the normal numbers) is 0: |q - 0| < 2^-126, tau times that in dz
-    bound = HALF_STEP[t] * 1.01 * np.abs(want) + TINY[t] + tau * (2.0 ** -126 + EPS24 * (eq + p * (8 * ptot + 160 + k)))
+    # the exponential is 0 below 2^-126, and is taken of q or of weight * tau * q: off by less than max(tau, 1) * 2^-126 in dz
+    bound = HALF_STEP[t] * 1.01 * np.abs(want) + TINY[t] + max(tau, 1) * 2.0 ** -126 + tau * (EPS24 * (eq + p * (8 * ptot + 160 + k)))
     for d in (dZ, a):
         within(decode(d.get(), t), want, bound, "dz")
