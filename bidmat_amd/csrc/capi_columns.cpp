@@ -128,7 +128,15 @@ namespace {
 int distill_call(const bm::DistillArgs& a, hipStream_t s) {
     if (a.nrows < 0 || a.nrows > (1 << 30) || a.ncols < 0 || a.nnz < 0 || !type_ok(a.type)) return kInvalid;
     if (!(a.temperature >= 1e-18f) || !(a.temperature <= 1e18f)) return kInvalid;      // its square stays in the range of fp32
-    if (a.nrows == 0 || a.ncols == 0) return a.nnz > 0 ? kInvalid : 0;
+    if ((a.nrows == 0 || a.ncols == 0) && a.nnz > 0) return kInvalid;
+    if (a.ncols == 0) return 0;
+    if (a.nrows == 0) {
+        // columns of nothing: loss 0, log-sum -inf
+        if (!operands_ok({vec(a.loss, a.ncols, true), vec(a.lse, a.ncols, true)})) return kInvalid;
+        hipError_t e = a.loss ? bm::fill_f32(a.loss, a.ncols, 0.f, s) : hipSuccess;
+        if (e == hipSuccess && a.lse) e = bm::fill_f32(a.lse, a.ncols, -INFINITY, s);
+        return e == hipErrorNoDevice ? 0 : (int)e;          // no device, no column: as with other calls that have no work
+    }
     if (!a.Z || !a.tjc || (a.nnz > 0 && (!a.tdata || !a.tir))) return kInvalid;
     const size_t size = bm::elem_size(a.type);
     if (!operands_ok({dense(a.Z, size, a.nrows, a.ncols, a.ldz), vec(a.tdata, a.nnz), vec(a.tir, a.nnz), vec(a.tjc, a.ncols + 1LL),

@@ -12,6 +12,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+def pytest_runtest_setup(item):
+    """The calls without work in test_columns_refusals.py pass made-up addresses for results that some of them write (the losses of
+    columns without rows): they run where no device is, and what is written is tested in test_gpu_columns_edges.py."""
+    if item.path.name == "test_columns_refusals.py" and item.name == "test_nothing_to_do_is_no_error":
+        from bidmat_amd import device
+        if device.device_available():
+            pytest.skip("passes made-up addresses: only where no device can write there")
+
+
 @pytest.fixture(scope="session")
 def hip():
     """The loaded C-ABI library; GPU tests fail loudly if it is missing or finds no device."""

@@ -168,3 +168,22 @@ def test_distill_grad_of_large_logits(hip, V, t, tau):
     bound = HALF_STEP[t] * 1.01 * np.abs(want) + TINY[t] + max(tau, 1) * 2.0 ** -126 + tau * (EPS24 * (eq + p * (8 * ptot + 160 + k)))
     for d in (dZ, a):
         within(decode(d.get(), t), want, bound, "dz")
+
+
+@pytest.mark.parametrize("m", [1, 5, 70000])
+def test_distill_without_rows(hip, m):
+    """A matrix of no rows: every column's loss is 0 and its log-sum that of nothing, -inf."""
+    jc = dev(np.zeros(m + 1, np.int32))
+    loss, lse = dev(np.full(m + 1, 7, F)), dev(np.full(m + 1, 7, F))
+    ok(hip.bidmat_distill(0, m, 0, None, 0, 0, None, None, jc.ptr, 1.0, None, loss.ptr, lse.ptr, None, 0, None))
+    assert (loss.numpy()[:m] == 0).all() and (lse.numpy()[:m] == -np.inf).all() and loss.numpy()[m] == 7 and lse.numpy()[m] == 7
+    lse.upload(np.full(m + 1, 7, F))
+    ok(hip.bidmat_distill(0, m, 0, None, 0, 0, None, None, jc.ptr, 1.0, None, loss.ptr, None, None, 0, None))
+    assert (lse.numpy() == 7).all()
+    ok(hip.bidmat_distill_grad(0, m, 0, None, 0, 0, None, None, jc.ptr, 1.0, None, lse.ptr, loss.ptr, 0, None))
+    assert (lse.numpy() == 7).all() and (loss.numpy()[:m] == 0).all()
+    # through the matrix interface, into a vector that held something else
+    base = int(Mat.get("ioneBased"))
+    nothing = GSMat.from_csc(0, m, np.zeros(0, F), np.zeros(0, np.int32), np.full(m + 1, base, np.int32))
+    out = GMat.from_numpy(np.full((1, m), 5, F))
+    assert (GMat.zeros(0, m).distill(nothing, out=out).numpy() == 0).all()
