@@ -434,6 +434,7 @@ void GSMat::ownPattern() {
         pattern = std::make_shared<Pattern>(ncols, realnnz);
         pir = pattern->pir; pic = pattern->pic; pjc = pattern->pjc;
     }
+    pattern->each = -1;
     planHolder = std::make_shared<PlanHolder>();      // new indices: any older plan is stale
 }
 
@@ -697,6 +698,40 @@ void vectorOf(const GMatP& v, long long n, const char* what) {
 }
 // A cached output belongs to all operands and settings of a call: those that the cache's own key has no room for go into the name.
 long long guidOf(const GMatP& a) { return a ? a->GUID : 0; }
+// The rows of a column where all columns have as many and none has a row twice, otherwise 0: known of what route wrote, looked up
+// once per pattern of others.
+int rowsPerColumn(const GSMat& s) {
+    if (s.pattern->each < 0) {
+        std::vector<int> jc((size_t)s.ncols + 1), ir((size_t)s.nnz()), last((size_t)s.nrows, -1);
+        Staging st;
+        st.download(jc.data(), s.pjc, sizeof(int) * jc.size());
+        st.download(ir.data(), s.pir, sizeof(int) * ir.size());
+        const int each = s.ncols > 0 ? s.nnz() / s.ncols : 0;
+        bool even = true;
+        for (int c = 0; c < s.ncols && even; ++c) {
+            even = jc[c] == c * each && jc[c + 1] == (c + 1) * each;
+            for (int j = c * each; even && j < (c + 1) * each; ++j) {
+                even = last[ir[j]] != c;
+                last[ir[j]] = c;
+            }
+        }
+        s.pattern->each = even ? each : 0;
+    }
+    return s.pattern->each;
+}
+bool equalPatterns(const GSMat& a, const GSMat& b) {
+    if (a.nrows != b.nrows || a.ncols != b.ncols || a.nnz() != b.nnz()) return false;
+    if (a.pattern == b.pattern) return true;
+    std::vector<int> x[2];
+    for (const GSMat* s : {&a, &b}) {
+        std::vector<int>& to = x[s == &b];
+        to.resize((size_t)s->ncols + 1 + s->nnz());
+        Staging st;
+        st.download(to.data(), s->pjc, sizeof(int) * ((size_t)s->ncols + 1));
+        st.download(to.data() + s->ncols + 1, s->pir, sizeof(int) * (size_t)s->nnz());
+    }
+    return x[0] == x[1];
+}
 void finished(int err, const char* what) {
     if (err == 0) err = bidmat_stream_synchronize(nullptr);
     if (err != 0) fail(std::string("HIP error in ") + what + " " + bidmat_error_string(err));
@@ -739,16 +774,19 @@ GSMatP GMat::route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, 
     Mat::nflops += 6LL * length();
     finished(bidmat_route(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(bias), sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, ngroups, topgroups,
                           topk, renorm, scale, out->pdata, out->pir, out->pic, out->pjc, nullptr, nullptr), "GMat.route");
+    out->pattern->each = topk;
     return out;
 }
 
 GMatP GMat::routeGrad(const GSMatP& gate, const GSMatP& dgate, bool sigmoid, bool renorm, float scale, GMatP oldmat) {
-    if (!gate || !dgate || gate->nrows != nrows || gate->ncols != ncols || dgate->nnz() != gate->nnz())
-        fail("GMat.routeGrad dimensions mismatch");
-    if (ncols == 0 || gate->nnz() % ncols != 0) fail("GMat.routeGrad: the gate's columns differ in length");
+    if (!gate || !dgate || gate->nrows != nrows || gate->ncols != ncols) fail("GMat.routeGrad dimensions mismatch");
+    const int topk = rowsPerColumn(*gate);
+    if (ncols > 0 && topk == 0) fail("GMat.routeGrad: the gate's columns differ in length, or one has a row twice");
+    if (!equalPatterns(*gate, *dgate)) fail("GMat.routeGrad: the gradient of the gate's values has another pattern");
     GMatP out = newOrCheckGMat(nrows, ncols, oldmat, GUID, dgate->GUID, opHash(fmt("routeGrad %lld %d %d %a", gate->GUID, sigmoid, renorm, scale).c_str()));
+    if (ncols == 0) return out;
     Mat::nflops += 6LL * length();
-    finished(bidmat_route_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, gate->nnz() / ncols, renorm,
+    finished(bidmat_route_grad(nrows, ncols, BIDMAT_F32, pdata, nrows, sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, topk, renorm,
                                scale, gate->pdata, gate->pir, dgate->pdata, out->pdata, nrows, nullptr), "GMat.routeGrad");
     return out;
 }

@@ -142,7 +142,8 @@ public:
     GMatP rmsnormGrad(const GMatP& w, float eps, const GMatP& dy, const GMatP& dh, const GMatP& dw, GMatP oldmat);
     // this = scores (experts x columns): a sparse matrix of weights, topk rows per column; sigmoid: kind of the scores
     GSMatP route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, int topk, bool renorm, float scale, GSMatP oldmat);
-    // this = scores: their gradient from dgate, the gradient of gate's values (a GSMat with gate's pattern, as DDS returns it)
+    // this = scores: their gradient from dgate, the gradient of gate's values (a GSMat with gate's pattern, as DDS returns it); a
+    // gate that route did not write, and a pattern that the two do not share, are read back to be checked
     GMatP routeGrad(const GSMatP& gate, const GSMatP& dgate, bool sigmoid, bool renorm, float scale, GMatP oldmat);
     // this = student logits: the loss of every column (1 x ncols) against the teacher's stored logits; grad (optional, like
     // this) receives the gradient, weight (optional) holds one factor per column
@@ -171,6 +172,7 @@ struct Pattern {
     int* pir = nullptr;
     int* pic = nullptr;
     int* pjc = nullptr;
+    int each = -1;                         // rows in every column, none twice; 0: not so, -1: not looked up
     Pattern(int ncols, int realnnz);       // allocates; throws on failure
     ~Pattern();
     Pattern(const Pattern&) = delete;

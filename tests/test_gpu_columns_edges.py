@@ -187,3 +187,42 @@ def test_distill_without_rows(hip, m):
     nothing = GSMat.from_csc(0, m, np.zeros(0, F), np.zeros(0, np.int32), np.full(m + 1, base, np.int32))
     out = GMat.from_numpy(np.full((1, m), 5, F))
     assert (GMat.zeros(0, m).distill(nothing, out=out).numpy() == 0).all()
+
+
+# ---------------------------------------------------------------- the matrix interface
+def gate_of(data, ir, jc, rows):
+    base = int(Mat.get("ioneBased"))
+    return GSMat.from_csc(rows, len(jc) - 1, np.asarray(data, F), np.asarray(ir, np.int32) + base, np.asarray(jc, np.int32) + base)
+
+
+def test_route_grad_wants_a_gate(hip):
+    """routeGrad takes what route returned, or a matrix that has such a pattern, and values of that very pattern."""
+    rng = np.random.default_rng(4)
+    E, m, k = 12, 6, 2
+    z = GMat.from_numpy(rng.standard_normal((E, m)).astype(F))
+    gate = z.route(k)
+    data, ir, jc = gate.to_csc()
+    base = int(Mat.get("ioneBased"))
+    ir, jc = ir.reshape(-1) - base, jc - base
+    values = GMat.from_numpy(rng.standard_normal((1, m * k)).astype(F))
+    dgate = gate.with_values(values)
+    want = z.routeGrad(gate, dgate).numpy()
+    # the same pattern from the host, shared or not
+    same = gate_of(data, ir, jc, E)
+    for a, b in ((same, same.with_values(values)), (same, dgate), (gate, same.with_values(values))):
+        assert np.array_equal(z.routeGrad(a, b).numpy(), want)
+    other = ir.copy()
+    other[:2] = [r for r in range(E) if r not in ir[:2]][:2]
+    twice = ir.copy()
+    twice[1] = twice[0]
+    uneven = jc.copy()
+    uneven[1] += 1                                       # columns of 3 and 1
+    for a, b in ((gate, gate_of(data, other, jc, E)), (gate_of(data, twice, jc, E),) * 2, (gate_of(data, ir, uneven, E),) * 2,
+                 (gate, gate_of(data, ir, uneven, E))):
+        with pytest.raises(RuntimeError):
+            z.routeGrad(a, b)
+    # a matrix whose indices are written again is looked at again
+    reused = gate.with_values(values)
+    gate2 = GMat.from_numpy(rng.standard_normal((E, m)).astype(F)).route(k, out=gate)
+    with pytest.raises(RuntimeError):
+        z.routeGrad(gate2, reused)
