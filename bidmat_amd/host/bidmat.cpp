@@ -767,13 +767,18 @@ GSMatP GMat::route(const GMatP& bias, bool sigmoid, int ngroups, int topgroups, 
     vectorOf(bias, nrows, "GMat.route");
     if (topk < 1 || (long long)ncols * topk > 0x7fffffffLL) fail(fmt("GMat.route: %d of %d experts for %d columns", topk, nrows, ncols));
     const int nnz = ncols * topk;
+    // the settings are looked at before the output is: a refused call leaves it as it was
+    const int kind = sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX;
+    if (bidmat_route(nrows, 0, BIDMAT_F32, nullptr, nrows, nullptr, kind, ngroups, topgroups, topk, renorm, scale, nullptr, nullptr, nullptr, nullptr,
+                     nullptr, nullptr) != 0)
+        fail(fmt("GMat.route: %d of %d experts, %d of %d groups, scale %g", topk, nrows, topgroups, ngroups, scale));
     GSMatP out = GSMat::newOrCheckGSMat(nrows, ncols, nnz, nnz, oldmat, GUID, guidOf(bias), topk,
                                         opHash(fmt("route %d %d %d %d %a", sigmoid, ngroups, topgroups, renorm, scale).c_str()));
     out->nnz0 = nnz;
     out->ownPattern();                                     // new indices: nothing shared, any older plan is stale
     Mat::nflops += 6LL * length();
-    finished(bidmat_route(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(bias), sigmoid ? BIDMAT_SIGMOID : BIDMAT_SOFTMAX, ngroups, topgroups,
-                          topk, renorm, scale, out->pdata, out->pir, out->pic, out->pjc, nullptr, nullptr), "GMat.route");
+    finished(bidmat_route(nrows, ncols, BIDMAT_F32, pdata, nrows, devptr(bias), kind, ngroups, topgroups, topk, renorm, scale, out->pdata, out->pir,
+                          out->pic, out->pjc, nullptr, nullptr), "GMat.route");
     out->pattern->each = topk;
     return out;
 }

@@ -226,3 +226,16 @@ def test_route_grad_wants_a_gate(hip):
     gate2 = GMat.from_numpy(rng.standard_normal((E, m)).astype(F)).route(k, out=gate)
     with pytest.raises(RuntimeError):
         z.routeGrad(gate2, reused)
+
+
+
+def test_a_refused_route_leaves_its_output_alone(hip):
+    rng = np.random.default_rng(5)
+    E, m = 12, 6
+    z = GMat.from_numpy(rng.standard_normal((E, m)).astype(F))
+    gate = z.route(4)
+    before = [a.copy() for a in gate.to_csc()]
+    for bad in (dict(topk=2, ngroups=5), dict(topk=3, scale=0.0), dict(topk=2, ngroups=3, topgroups=4), dict(topk=13)):
+        with pytest.raises(RuntimeError):
+            z.route(**bad, out=gate)
+        assert all(np.array_equal(a, b) for a, b in zip(gate.to_csc(), before))
