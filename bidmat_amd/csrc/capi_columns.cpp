@@ -164,7 +164,7 @@ API int bidmat_distill_grad(int nrows, int ncols, int type, const void* Z, int l
 API int bidmat_dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, int ldq, const float* scales, int group, const float* Sdata,
                              const int* Sir, const int* Sjc, float* C, int beta, void* stream) {
     auto lock = bm::device_lock();
-    if (k < 0 || ncols < 0 || nnz < 0 || !group_ok(group) || (beta != 0 && beta != 1)) return kInvalid;
+    if (k < 0 || k > (1 << 30) || ncols < 0 || nnz < 0 || !group_ok(group) || (beta != 0 && beta != 1)) return kInvalid;
     if (k == 0 || ncols == 0) return 0;
     if (ldq < k || !Sjc || !C || (nnz > 0 && (!Q || !scales || !Sdata || !Sir))) return kInvalid;
     // (the columns of A are not counted in the call: only its first one is known to be there)

@@ -188,8 +188,9 @@ __global__ __launch_bounds__(BM_BLOCK) void k_dsmult_q8(Q8Args a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[j] = 0.f;
         constexpr int U = LPN < 4 ? LPN : 4;
-        for (int j0 = lo; j0 < hi; j0 += 64) {
-            const int rem = hi - j0 < 64 ? hi - j0 : 64;
+        // (by what is left: hi may be the last int)
+        for (int j0 = lo, after = hi - lo; after > 0; j0 = (int)(j0 + 64u), after -= 64) {
+            const int rem = after < 64 ? after : 64;
             int row = 0;
             float val = 0.f;
             if (lane < rem) {
@@ -318,7 +319,7 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     hipError_t err;
     while (a.seglen > kSegMin && nnz < kWavesMin * (long long)a.seglen) a.seglen >>= 1;
     if (nnz > a.seglen) {
-        a.nsegs = (nnz + a.seglen - 1) / a.seglen;
+        a.nsegs = (int)((nnz + (long long)a.seglen - 1) / a.seglen);
         a.partial = (float*)ws_get(WS_PARTIAL, sizeof(float) * (size_t)a.nsegs * (size_t)k, &err, s);
         if (!a.partial) return err;
     }

@@ -239,3 +239,28 @@ def test_a_refused_route_leaves_its_output_alone(hip):
         with pytest.raises(RuntimeError):
             z.route(**bad, out=gate)
         assert all(np.array_equal(a, b) for a, b in zip(gate.to_csc(), before))
+
+
+# ---------------------------------------------------------------- the 8-bit product
+def put(d, first, a):
+    ok(d.lib.bidmat_memcpy_h2d(d.ptr + first * d.dtype.itemsize, np.ascontiguousarray(a, d.dtype).ctypes.data, a.size * d.dtype.itemsize))
+
+
+def test_dsmult_q8_with_almost_2_to_the_31_nonzeros(hip):
+    """As many nonzeros as an int counts, zeros but for the first and the last ones."""
+    rng = np.random.default_rng(8)
+    k, rows, m, nnz, some = 4, 50, 65536, 2 ** 31 - 1, 1000
+    jc = np.minimum(np.arange(m + 1, dtype=np.int64) * (nnz // m + 1), nnz).astype(np.int32)
+    assert jc[-1] == nnz and (np.diff(jc) > 0).all()
+    codes, scales = rng.integers(0, 0x7F, (rows, k)).astype(np.uint8), (0.01 + rng.random((rows, 1))).astype(F)
+    ir, v = DeviceArray.zeros(nnz, np.int32), DeviceArray.zeros(nnz, F)
+    want, size = np.zeros((m, k)), np.zeros((m, k))
+    for first, col in ((0, 0), (nnz - some, m - 1)):
+        r, x = rng.integers(0, rows, some).astype(np.int32), rng.standard_normal(some).astype(F)
+        put(ir, first, r)
+        put(v, first, x)
+        a, b = ref.q8_product(codes, scales, 0, x, r, np.array([0, some], np.int32))
+        want[col], size[col] = a[0], b[0]
+    q, s, j, c = Columns(codes), dev(scales), dev(jc), empty(m, k, F)
+    ok(hip.bidmat_dsmult_q8_csc(k, m, nnz, q.ptr, k, s.ptr, 0, v.ptr, ir.ptr, j.ptr, c.ptr, 0, None))
+    within(c.get().astype(np.float64), want, 1100 * EPS24 * size, "C")
