@@ -18,6 +18,7 @@
 #include "kernels.hpp"
 #include "workspace.hpp"
 #include <algorithm>
+#include <limits.h>
 
 namespace bm {
 namespace {
@@ -29,6 +30,10 @@ constexpr int kSlab = 1 << 24, kSegsMax = 1 << 25;
 // 128; k = 1650, 4300 in 717: 17 and 60; for 2048 waves k = 1024, 2000 columns of 40: 27 against 20). Workgroups that add
 // partial sums, at least as many, where there are so many columns.
 constexpr int kSegMin = 16, kWavesMin = 1024, kLookWgs = 2048;
+// Bytes of partial sums, at most: which columns are cut is known to the device alone, so that room is for every segment. Longer
+// segments rather than more of it: 98 M nonzeros in 100000 columns, k = 256, take 3.20 ms with 256 MiB (segments of 376), 3.31 with
+// the 0.8 GB of segments of 128; 9.9 M in 20000, k = 1024, 1.23 ms (152) and 1.25.
+constexpr long long kPartialMax = 256LL << 20;
 
 struct Q8Args {
     int k, ncols, nnz, seglen, beta, nscales, shift;      // shift: log2 of the rows per scale; 31: one scale per column
@@ -318,6 +323,8 @@ hipError_t dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char* Q, long
     a.nsegs = 0;
     hipError_t err;
     while (a.seglen > kSegMin && nnz < kWavesMin * (long long)a.seglen) a.seglen >>= 1;
+    const long long most = kPartialMax / ((long long)sizeof(float) * k);          // segments
+    if (nnz > most * a.seglen) a.seglen = most > 0 ? (int)((nnz + most - 1) / most) : INT_MAX;
     if (nnz > a.seglen) {
         a.nsegs = (int)((nnz + (long long)a.seglen - 1) / a.seglen);
         a.partial = (float*)ws_get(WS_PARTIAL, sizeof(float) * (size_t)a.nsegs * (size_t)k, &err, s);

@@ -433,7 +433,8 @@ int bidmat_distill_grad(int nrows, int ncols, int type, const void *Z, int ldz, 
 /* C = beta*C + A*S with A in 8 bits, A[i, r] = scales[i / group, r] * e4m3(Q[i, r]): codes and scales as bidmat_rmsnorm
  * writes them (Q k x nrowsS with leading dimension ldq, scales ceil(k / group) x nrowsS, group 0 = one per column); k <= 2^30.
  * Otherwise bidmat_dsmult_csc: S and C fp32, the same bits every time.  Columns longer than an eighth of
- * "seglen" (k <= 128: a quarter; where nnz is small, down to 16) are cut at the multiples of that number in the array of nonzeros. */
+ * "seglen" (k <= 128: a quarter; where nnz is small, down to 16; where partial sums would take more than 256 MiB of scratch,
+ * longer) are cut at the multiples of that number in the array of nonzeros. */
 int bidmat_dsmult_q8_csc(int k, int ncols, int nnz, const unsigned char *Q, int ldq, const float *scales, int group,
                          const float *Sdata, const int *Sir, const int *Sjc, float *C, int beta, void *stream);
 

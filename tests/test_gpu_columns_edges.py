@@ -264,3 +264,30 @@ def test_dsmult_q8_with_almost_2_to_the_31_nonzeros(hip):
     q, s, j, c = Columns(codes), dev(scales), dev(jc), empty(m, k, F)
     ok(hip.bidmat_dsmult_q8_csc(k, m, nnz, q.ptr, k, s.ptr, 0, v.ptr, ir.ptr, j.ptr, c.ptr, 0, None))
     within(c.get().astype(np.float64), want, 1100 * EPS24 * size, "C")
+
+
+def test_dsmult_q8_scratch_is_bounded(hip):
+    """Partial sums take 256 MiB and the growth of a scratch buffer at most, however many nonzeros there are."""
+    rng = np.random.default_rng(6)
+    k, rows, m, each = 2048, 300, 50000, 320
+    lengths = np.full(m, each)
+    lengths[[7, m - 1]] = 5000
+    jc = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    nnz = int(jc[-1])                                    # at 128 nonzeros a partial sum these were 1.0 GB
+    ir, S = rng.integers(0, rows, nnz).astype(np.int32), rng.standard_normal(nnz).astype(F)
+    codes, scales = rng.integers(0, 0x7F, (rows, k)).astype(np.uint8), (0.01 + rng.random((rows, 1))).astype(F)
+    q, s, v, i, j, c = Columns(codes), dev(scales), dev(S), dev(ir), dev(jc), DeviceArray(m * k, F)
+    st, free, total = C.c_void_p(), C.c_longlong(), C.c_longlong()
+    ok(hip.bidmat_stream_create(C.byref(st)))
+    ok(hip.bidmat_mem_info(C.byref(free), C.byref(total)))
+    before = free.value
+    ok(hip.bidmat_dsmult_q8_csc(k, m, nnz, q.ptr, k, s.ptr, 0, v.ptr, i.ptr, j.ptr, c.ptr, 0, st))
+    ok(hip.bidmat_stream_synchronize(st))
+    ok(hip.bidmat_mem_info(C.byref(free), C.byref(total)))
+    assert before - free.value <= 1.2 * 2 ** 28 + 2 ** 25
+    ok(hip.bidmat_stream_destroy(st))
+    got = c.numpy().reshape(m, k)
+    for col in (0, 7, 8, 12345, m - 2, m - 1):
+        a, b = jc[col], jc[col + 1]
+        want, size = ref.q8_product(codes, scales, 0, S[a:b], ir[a:b], np.array([0, b - a], np.int32))
+        within(got[col].astype(np.float64), want[0], 1100 * EPS24 * size[0], "C")
