@@ -126,7 +126,8 @@ API int bidmat_route_grad(int nexperts, int ncols, int type, const void* Z, int 
 
 namespace {
 int distill_call(const bm::DistillArgs& a, hipStream_t s) {
-    if (a.nrows < 0 || a.nrows > (1 << 30) || a.ncols < 0 || a.nnz < 0 || !type_ok(a.type)) return kInvalid;
+    if (a.nrows < 0 || a.nrows > (1 << 30) || a.ncols < 0 || !type_ok(a.type)) return kInvalid;
+    if (a.nnz < 0 || a.nnz > INT_MAX - 1024) return kInvalid;          // the kernels count past a column's end, by a workgroup at most
     if (!(a.temperature >= 1e-18f) || !(a.temperature <= 1e18f)) return kInvalid;      // its square stays in the range of fp32
     if ((a.nrows == 0 || a.ncols == 0) && a.nnz > 0) return kInvalid;
     if (a.ncols == 0) return 0;
