@@ -333,7 +333,7 @@ __device__ __forceinline__ void write_weights(const RouteArgs& a, const Deal& d,
             p = a.kind == 0 || high < -30.f ? exp_of(z - high) : sigmoid_of(z);
             p = valid ? p : 0.f;
             const float sum = lanes_sum_rt(p, d.kp);
-            p = sum > 0.f ? p * (a.scale * __builtin_amdgcn_rcpf(sum)) : 0.f;
+            p = sum > 0.f ? a.scale * (p * __builtin_amdgcn_rcpf(sum)) : 0.f;          // (scale / sum may leave fp32)
         } else {
             p = a.scale * (a.kind == 0 ? exp_of(z - top) * by : sigmoid_of(z));
             p = valid ? p : 0.f;

@@ -291,3 +291,18 @@ def test_dsmult_q8_scratch_is_bounded(hip):
         a, b = jc[col], jc[col + 1]
         want, size = ref.q8_product(codes, scales, 0, S[a:b], ir[a:b], np.array([0, b - a], np.int32))
         within(got[col].astype(np.float64), want[0], 1100 * EPS24 * size[0], "C")
+
+
+# ---------------------------------------------------------------- routing
+@pytest.mark.parametrize("E,k", [(64, 6), (1000, 20)])
+@pytest.mark.parametrize("m", [3, 100])
+@pytest.mark.parametrize("scale", [1e30, 2.5, -1e-30])
+def test_route_renormalised_with_a_large_scale(hip, E, k, m, scale):
+    """Sigmoids whose sum is small: scale over that sum leaves fp32 where the weights do not."""
+    rng = np.random.default_rng(E)
+    z = encode(-28 + 0.5 * rng.standard_normal((m, E)), 0)
+    a, G, ir = Columns(z), empty(m, k, F), empty(m, k, np.int32)
+    ok(hip.bidmat_route(E, m, 0, a.ptr, E, None, 1, 1, 1, k, 1, scale, G.ptr, ir.ptr, None, None, None, None))
+    wi, ww, _ = ref.route(decode(z, 0), None, 1, 1, 1, k, True, float(F(scale)))
+    assert np.array_equal(ir.get(), wi)
+    within(G.get().astype(np.float64), ww, (2 * 30 + 60) * EPS24 * np.abs(ww), "weights")
