@@ -24,15 +24,23 @@ bool type_ok(int type) { return type == BIDMAT_F32 || type == BIDMAT_F16 || type
 struct Operand {
     const void* p;
     size_t size, n;
-    long long ld;            // 0: a vector
+    long long rows, ld;      // ld 0: a vector
     bool out, aligned;
 };
 template <class T>
 Operand vec(const T* p, long long n, bool out = false) {
-    return {p, sizeof(T), (size_t)n, 0, out, (uintptr_t)p % sizeof(T) == 0};
+    return {p, sizeof(T), (size_t)n, n, 0, out, (uintptr_t)p % sizeof(T) == 0};
 }
 Operand dense(const void* p, size_t size, int nrows, int ncols, long long ld, bool out = false) {
-    return {p, size, (size_t)(ncols - 1) * (size_t)ld + nrows, ld, out, (uintptr_t)p % size == 0 && ld >= nrows};
+    return {p, size, (size_t)(ncols - 1) * (size_t)ld + nrows, nrows, ld, out, (uintptr_t)p % size == 0 && ld >= nrows};
+}
+// Whether two dense operands are different rows of one matrix: the same bytes from column to column, and no byte in common.
+bool different_rows(const Operand& x, const Operand& y) {
+    const size_t stride = (size_t)x.ld * x.size, wx = (size_t)x.rows * x.size, wy = (size_t)y.rows * y.size;
+    if (x.ld == 0 || y.ld == 0 || stride != (size_t)y.ld * y.size) return false;
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    const size_t apart = (a < b ? b - a : a - b) % stride, from = a < b ? apart : (stride - apart) % stride;      // y's first byte behind x's
+    return from >= wx && from + wy <= stride;
 }
 // Every operand given (p not null) lies at a multiple of its element, with columns apart; and no output shares memory with
 // another operand, except a dense one that is a dense input, element by element.
@@ -43,7 +51,7 @@ bool operands_ok(std::initializer_list<Operand> all) {
         for (const Operand* y = all.begin(); y != x; ++y) {
             if (!y->p || (!x->out && !y->out)) continue;
             const uintptr_t x0 = (uintptr_t)x->p, x1 = x0 + x->n * x->size, y0 = (uintptr_t)y->p, y1 = y0 + y->n * y->size;
-            if (x0 >= y1 || y0 >= x1) continue;
+            if (x0 >= y1 || y0 >= x1 || different_rows(*x, *y)) continue;
             const bool same = x->ld != 0 && x0 == y0 && x->ld == y->ld && x->size == y->size;
             if (!same || (x->out && y->out)) return false;
         }

@@ -369,7 +369,8 @@ int bidmat_applyop_flat(const float *A, const float *B, float *C, long long n, i
  *    element.  Everything is computed and summed in fp32 and rounded to nearest even once, when it is written.  Weights,
  *    scales and values of sparse matrices are fp32.  They only enqueue work on `stream`.  A dense output may
  *    be one of the call's dense inputs of its type (same address and leading dimension); any other overlap of an output
- *    returns hipErrorInvalidValue.
+ *    returns hipErrorInvalidValue.  Dense operands that are different rows of one matrix (as many bytes from column to
+ *    column, no element in common) do not overlap.
  * ------------------------------------------------------------------------------------ */
 enum { BIDMAT_F32 = 0, BIDMAT_F16 = 1, BIDMAT_BF16 = 2 };
 enum { BIDMAT_SOFTMAX = 0, BIDMAT_SIGMOID = 1 };

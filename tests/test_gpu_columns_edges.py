@@ -306,3 +306,23 @@ def test_route_renormalised_with_a_large_scale(hip, E, k, m, scale):
     wi, ww, _ = ref.route(decode(z, 0), None, 1, 1, 1, k, True, float(F(scale)))
     assert np.array_equal(ir.get(), wi)
     within(G.get().astype(np.float64), ww, (2 * 30 + 60) * EPS24 * np.abs(ww), "weights")
+
+
+# ---------------------------------------------------------------- operands that lie between one another
+def test_row_slices_of_one_matrix(hip):
+    """Operands that are different rows of one matrix (one leading dimension, no element in common) are no overlap."""
+    rng = np.random.default_rng(3)
+    n, m, gap = 100, 40, 7
+    ld = 2 * n + gap
+    both = np.full((m, ld), 5, F)
+    both[:, :n] = rng.standard_normal((m, n))
+    a, w = dev(both), dev(np.ones(n, F))
+    ok(hip.bidmat_rmsnorm(n, m, 0, a.ptr, ld, None, n, w.ptr, 1e-5, None, n, a.ptr + 4 * n, ld, None, n, None, 0, None))
+    got = a.numpy().reshape(m, ld)
+    _, y, _ = ref.rmsnorm(both[:, :n].astype(np.float64), None, np.ones(n), float(F(1e-5)))
+    assert np.array_equal(got[:, :n], both[:, :n]) and (got[:, 2 * n:] == 5).all()
+    within(got[:, n:2 * n], y, (NORM_DEPTH + 1) * EPS24 * np.abs(y), "y")
+    # a row in common, other leading dimensions, a vector in between
+    for args in ((a.ptr + 4 * (n - 1), ld), (a.ptr + 4 * (ld - n + 1), ld), (a.ptr + 4 * n, ld - 1)):
+        assert hip.bidmat_rmsnorm(n, m, 0, a.ptr, ld, None, n, w.ptr, 1e-5, None, n, *args, None, n, None, 0, None) == 1
+    assert hip.bidmat_rmsnorm(n, m, 0, a.ptr, ld, None, n, a.ptr + 4 * n, 1e-5, None, n, a.ptr + 4 * n, ld, None, n, None, 0, None) == 1
