@@ -422,7 +422,7 @@ int bidmat_route_grad(int nexperts, int ncols, int type, const void *Z, int ldz,
  * gradient 0 whatever its logits are (with nrows = 0: loss 0, lse -inf).  Rows need not be sorted; the shares of a row
  * stored twice add.  Entries whose row lies outside the matrix are left out.  A row whose student logit is -inf has q = 0
  * (with p > 0: loss +inf); a column of them has no softmax: NaN.  temperature from 1e-18 to 1e18, nrows <= 2^30,
- * nnz <= 2^31 - 1025.
+ * nnz <= 2^31 - 1025: how many values Tdata and Tir hold, also where a range of columns is passed as Tjc + col1.
  * Columns whose rows ascend are fastest; one with a row stored twice takes time with the square of its entries. */
 int bidmat_distill(int nrows, int ncols, int type, const void *Z, int ldz, int nnz, const float *Tdata, const int *Tir,
                    const int *Tjc, float temperature, const float *weight, float *loss, float *lse, void *dZ, int lddz,
