@@ -304,8 +304,9 @@ __device__ __forceinline__ float lanes_max_rt(float x, int n) {
     if (n >= 64) x = fmaxf(x, __shfl_xor(x, 32, 64));
     return x;
 }
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x)); }
+// Of the weights: expf and divisions, right to a few units however far a score lies below the largest (the hardware's exponential
+// of x * log2(e) is off by |x| units, and saves nothing: 256 experts x 65536 columns 42.3 us, with these 42.2; 60 x 32768 14.3, 14.4).
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
 
 constexpr int kRouteBatch = 8;           // columns whose weights one wave writes together, at most
 struct Chosen {                          // of one wave
@@ -330,12 +331,12 @@ __device__ __forceinline__ void write_weights(const RouteArgs& a, const Deal& d,
             const float high = lanes_max_rt(z, d.kp);
             // Far below 0 sigmoid(z) is exp(z) to within a factor 1 + exp(z): with all taken scores below -30 their
             // shares are a softmax's, where the sigmoids themselves may have left the range of fp32.
-            p = a.kind == 0 || high < -30.f ? exp_of(z - high) : sigmoid_of(z);
+            p = a.kind == 0 || high < -30.f ? expf(z - high) : sigmoid_of(z);
             p = valid ? p : 0.f;
             const float sum = lanes_sum_rt(p, d.kp);
-            p = sum > 0.f ? a.scale * (p * __builtin_amdgcn_rcpf(sum)) : 0.f;          // (scale / sum may leave fp32)
+            p = sum > 0.f ? a.scale * (p / sum) : 0.f;          // (scale / sum may leave fp32)
         } else {
-            p = a.scale * (a.kind == 0 ? exp_of(z - top) * by : sigmoid_of(z));
+            p = a.scale * (a.kind == 0 ? expf(z - top) * by : sigmoid_of(z));
             p = valid ? p : 0.f;
         }
         if (on) {

@@ -444,3 +444,22 @@ def test_rmsnorm_grad_of_columns_out_of_range_with_every_operand(hip, n, m, over
             within(dw.numpy().astype(np.float64), wantw + beta * dw0, (NORM_DEPTH + 48 + m / 512) * EPS24 * (sizew + np.abs(dw0)), "dw")
         else:
             assert np.array_equal(dw.numpy(), dw0)
+
+
+@pytest.mark.parametrize("E,groups,k,m", [(64, 1, 12, 5), (64, 1, 12, 300), (256, 4, 16, 300), (1000, 1, 40, 100)])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_weights_far_below_the_largest(hip, E, groups, k, m, kind, renorm):
+    """Whole scores, whose differences are exact: the weights are right to a few units however small they are. expf is off by one
+    unit (2 * 2^-24), the sum over a column (terms e^-x, each off by (x + 2) * 2^-24: 3 * 2^-24 of the sum; at most 10 additions that
+    count) by 13, the reciprocal, the product and the scale by one each."""
+    rng = np.random.default_rng(E + k)
+    z = -rng.choice(np.arange(1, 80), (m, E)).astype(np.float64)
+    z[:, 3] = 0
+    z[:, 5] = -70                                        # few open experts: the far ones are taken too
+    z[:, 6 + k:] = -np.inf
+    a, G, ir = Columns(encode(z, 0)), empty(m, k, F), empty(m, k, np.int32)
+    ok(hip.bidmat_route(E, m, 0, a.ptr, E, None, kind, groups, groups, k, int(renorm), 1.0, G.ptr, ir.ptr, None, None, None, None))
+    wi, ww, _ = ref.route(z, None, kind, groups, groups, k, renorm, 1.0)
+    assert np.array_equal(ir.get(), wi)
+    within(G.get().astype(np.float64), ww, 18 * EPS24 * np.abs(ww), "weights")
