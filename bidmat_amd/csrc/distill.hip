@@ -8,8 +8,9 @@
 // stored twice; its shares add. Entries whose row lies outside the matrix are left out.
 //
 // What bounds it: memory. Loss and gradient of 131072 rows x 4096 columns in bf16: 430 us, 5.0 TB/s, every logit read once and
-// written once; the gradient alone 368 us, 5.8 TB/s. Columns above 384 or 400 KiB (and above 128 KiB where there are few) are cut
-// into chunks and read twice: 262144 x 512 fp32 312 us, 5.2 TB/s of what is moved. Taking such columns in slabs that
+// written once; the gradient alone 355 us, 6.1 TB/s; the loss alone 253 us, 4.2 TB/s (128256 x 2048 fp32: 180 us, 5.9). Columns
+// above 384 or 400 KiB (and above 128 KiB where there are few) are cut into chunks and read twice: 262144 x 512 fp32 299 us,
+// 5.4 TB/s of what is moved; 128256 x 2048 fp32 584 us. Taking such columns in slabs that
 // would stay in the 256 MB cache until the second time cost more than it gave (70000 x 2048 fp32: 344 us in slabs of 96 MiB, 399
 // of 48, 324 in one). Few columns: two launches that leave no wait between them (100003 x 5 fp32: 3.9 and 5.0 us).
 #include "columns.hpp"
@@ -279,6 +280,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     int e0, e1;
     column_entries(a, c, e0, e1);
     const float w = column_scale(a, c) * a.temperature;
+    const float lse = KEPT ? a.lse_in[c] : 0.f;
     bool none = e0 == e1 || w == 0.f;
     const bool extra = ALONE && threadIdx.x >= BM_BLOCK;
     const int i0 = extra ? hi : lo + (int)threadIdx.x * 8;
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     Share<KEPT> q;
     Teacher t;
     if constexpr (ALONE) {
-        q = share_of_lse(a.lse_in[c], a.temperature, k);
+        q = share_of_lse(lse, a.temperature, k);
         if (extra && !none) {
             const int lane = threadIdx.x & 63;
             float sum = 0.f;
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
     } else {
         t = stats[c];
         if constexpr (KEPT) {
-            q = share_of_lse(a.lse_in[c], a.temperature, k);
+            q = share_of_lse(lse, a.temperature, k);
         } else {
             const LogSum s = block_join(join_parts(parts + c * nchunks, nchunks, threadIdx.x, BM_BLOCK, k), k, sh, BM_WAVES_PER_BLOCK);
             q = share_of(s, k);
@@ -327,6 +329,7 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
         none = none || !t.some;
     }
     auto rows = [&](auto part) {
+#pragma unroll 1
         for (int i = i0; i < hi;) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -345,14 +348,29 @@ __global__ __launch_bounds__(ALONE ? BM_BLOCK + 64 : BM_BLOCK) void k_distill_gr
                 if (!none && i + u * STEP < hi) x[u] = load_col8(z, i + u * STEP, hi);
         }
     };
-    // Two instructions less per logit where they change nothing: an lse of up to 2^16 is right to 2^-8, so that no q passes 1 by
-    // more, and a scale within 2^+-24 goes into the exponent at the cost of less than 2^-20 of the value (50001 x 2048 fp16: 83 us, without 85).
     if constexpr (KEPT) {
-        if (fabsf(q.at) <= 0x1p16f && w >= 0x1p-24f && w <= 0x1p24f) {
-            const float up = __log2f(w);
-            rows([&](float v) { return __builtin_amdgcn_exp2f(fmaf(fmaf(q.at, q.by, v), k, up)); });
+        // An lse of up to 2^16 is right to 2^-8, so that no q passes 1 by more, and its product with k is kept in two parts: the
+        // first beside z * k with one rounding, the second (2^-24 of it) in the scale. That leaves a logit the instructions of an
+        // exponential; the difference first, and the limit, cost two more (50001 x 2048 fp16: 85 us, so 84).
+        const float base = q.at * a.temperature, most = base * k;
+        const float wl = w * __builtin_amdgcn_exp2f(-fmaf(base, k, -most) - fmaf(q.at, a.temperature, -base) * k);
+        const bool far = !none && !(fabsf(q.at) <= 0x1p16f);
+        auto near_rows = [&] { rows([&](float v) { return wl * __builtin_amdgcn_exp2f(fmaf(v, k, -most)); }); };
+        auto far_rows = [&] {
+#pragma unroll 1
+            for (int i = i0; i < hi; i += STEP) {
+                float8_t v = load_col8(z, i, hi).wide();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = w * q(v[j]);
+                store_col8(dz, i, hi, v);
+            }
+        };
+        if constexpr (ALONE) {          // dZ is not Z: a second pass, so that the first one stands by itself
+            near_rows();
+            if (far) far_rows();
         } else {
-            rows([&](float v) { return w * q(v); });
+            if (far) far_rows();
+            else near_rows();
         }
     } else {
         rows([&](float v) { return w * q(v); });
