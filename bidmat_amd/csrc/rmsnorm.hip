@@ -2,7 +2,7 @@
 // 8 bits with scales behind, and its gradient.
 //
 //   h = x + r,   rs = 1 / sqrt(mean(h^2) + eps),   y_i = h_i * rs * w_i
-//   scale_g = max(max over group g of |y|) / 448, 2^-126),   q_i = e4m3(y_i / scale_g)
+//   scale_g = max(max over group g of |y| / 448, 2^-126),   q_i = e4m3(y_i / scale_g)
 //
 // y is formed from the sum in fp32, not from the rounded h that is written. 448 is the largest number of e4m3, so that no
 // code overflows; 2^-126 keeps 1 / scale finite for a group of zeros (whose codes are zeros).
@@ -10,9 +10,11 @@
 // output written once, also where an output overwrites its input.
 //
 // What bounds it: memory, as long as columns of a multiple of 128 bytes let every load take whole lines (8192 rows x 16384
-// columns bf16 with residual and codes: 160 us, 5.9 TB/s; 1001 x 7777 fp32, read, written and in codes: 13.7 us, 5.1 TB/s; 1001 x
-// 15554 bf16: 24.5 us, 4.5 TB/s); a few columns, the launch. A workgroup of its own per column from 1025 rows on, more than
-// one column per wave up to 256.
+// columns bf16 with residual and codes: 160 us, 5.9 TB/s). Odd heights: 1001 x 155540 bf16, read and written, 120 us, 5.2 TB/s; 1001
+// x 77777 fp32, with codes too, 141 us, 5.0. A tenth of these columns stays in the 256 MB cache, which is no faster here (13.7
+// us, 4.5 TB/s and 13.5 us, 5.2, in a run of calls; a dispatch of the latter by itself 17.5): the start and the end of a
+// launch of 14 us are most of what is lost against the cache's 8. A few columns: the launch. A workgroup of its own per
+// column from 1025 rows on, more than one column per wave up to 256.
 #include "columns.hpp"
 #include "elems.hpp"
 #include "kernels.hpp"
@@ -171,8 +173,9 @@ __global__ __launch_bounds__(norm_block(TPC)) void k_rmsnorm(NormArgs a) {
 // Every workgroup walks columns c0, c0 + slots, ... and keeps its share of dw in registers; the shares go to partial
 // (one row of nrows floats per workgroup) and are added in a fixed order by k_add_shares.
 // What bounds it: memory (4096 rows x 16384 columns bf16: 103 us with the shares' addition, 5.2 TB/s). Above 8192 rows a
-// thread's registers do not hold the next column, above 16384 not the present one either (16384 rows x 4096: 125 us, 4.3 TB/s;
-// 32768 x 2048: 227 us, 2.4 TB/s).
+// thread's registers do not hold the next column, above 16384 not the present one either (16384 rows x 4096: 118 us, 4.5 TB/s;
+// 32768 x 2048: 202 us, 2.7 TB/s, spilling). Medium sizes: the shares and the second launch (1001 x 15554 bf16: 31 us for 93 MB,
+// 37 with dH; 8192 x 2000: 27 us for 98 MB).
 // A column whose sums leave fp32, of squares or of products (which count on the small side where rs is large).
 __device__ __forceinline__ bool outside(float d, float gh) {
     return !in_range(d) || !(fabsf(gh) < INFINITY) || (d < 0x1p-20f && fabsf(gh) < 0x1p-100f);
@@ -388,7 +391,11 @@ hipError_t launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Threads per column and vectors per thread: the fewest that hold n elements.
+// Threads per column and vectors per thread: the fewest that hold n elements. Forward, two vectors per thread cost little (4096
+// rows x 16384 columns bf16 with residual 92.4 us, with 512 threads of one vector 89.7; 1000 x 15000 18.7 and 20.0; 768 x 20000 19.8
+// and 19.0). The gradient keeps two or three columns at once, and one vector per thread leaves it registers (4096 x 16384 bf16
+// 102 us, with 256 threads of two 123; 8192 x 8192 102 and 177; 1024 x 32768 fp32 108 and 281; 45 and 148 for 1000 x 15000;
+// in 16 bits 128 threads are as good as 64 of two, 27.6 and 26.4).
 template <class T, class F>
 hipError_t by_height(int n, F&& f) {
     const int vecs = (n + 7) / 8;

@@ -941,8 +941,8 @@ hipError_t add_counts(const RouteArgs& a, unsigned grid, const int* shares, hipS
 
 // Few columns are left to one workgroup, which writes the counts itself and saves the second launch (7.4 us a call instead of
 // 9.8): up to two columns per wave (384 experts: 16 columns 10.7 us, 32 17.2 us against 10.9 by many workgroups), or, with
-// 16 lanes to a column, kOneRows (128 experts: 32 columns 7.3 us, by one column per wave 9.3; 64 columns 9.1; 256 experts in 8
-// groups: 48 columns 13.2 us, by many workgroups 10.7, ungrouped 8.4 against 9.8).
+// 16 lanes to a column, kOneRows (128 experts: 32 columns 7.3 us, by one column per wave 9.3; 64 columns 9.1; 256 experts: 48
+// columns 8.4 us against 9.8 by many workgroups, but in 8 groups, for which there is no border of its own, 13.2 against 10.7).
 constexpr int kOneRows = 48, kOneColumns = 2;
 // Waves per workgroup: as many as leave the keys of take_exact 32 KiB of LDS.
 constexpr int route_waves(int vpl, bool one) { return vpl <= 4 ? (one ? 16 : 8) : 64 / vpl; }
