@@ -380,8 +380,9 @@ enum { BIDMAT_SOFTMAX = 0, BIDMAT_SIGMOID = 1 };
  * H (nullable) receives h, Y (nullable) y.  Q and scales (both or neither) receive y in 8 bits: e4m3 codes (OCP, nrows x
  * ncols, leading dimension ldq) and one scale per `group` rows (0 = the column; 32, 64 or 128; the last group of a column
  * may be short; scales is ceil(nrows / group) x ncols): scale = max(largest |y| / 448, 2^-126), code = e4m3(y / scale).
- * y is formed from the unrounded sum.  In a column of h with a NaN every y and code is NaN,
- * with an infinity that row's y and code is NaN and the others are 0.
+ * y is formed from the unrounded sum.  Squares that leave fp32 on either side are summed from scaled columns, so that the
+ * formula holds for every finite h.  In a column of h with a NaN every y and code is NaN, with an infinity that row's y and
+ * code is NaN and the others are 0; a column of zeros with eps = 0 is NaN.
  * nrows <= 32768 (a column stays in the registers of one workgroup). */
 int bidmat_rmsnorm(int nrows, int ncols, int type, const void *X, int ldx, const void *R, int ldr, const float *w,
                    float eps, void *H, int ldh, void *Y, int ldy, unsigned char *Q, int ldq, float *scales, int group,
